@@ -18,7 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libclutor_b200.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "clb200.h")
 
-T_F32, T_F16, T_Q8_0, T_Q4_K, T_Q6_K = 0, 1, 8, 12, 14
+T_F32, T_F16, T_Q8_0, T_Q4_K, T_Q6_K, T_BF16 = 0, 1, 8, 12, 14, 30
 
 
 class CLW(C.Structure):
@@ -106,6 +106,39 @@ class SmartStats(C.Structure):
         return {f: getattr(self, f) for f, _ in self._fields_}
 
 
+class KvStruct(C.Structure):
+    """clb200_kv (include/clb200.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_uint32), ("n_pages", C.c_int), ("page_size", C.c_int),
+                ("n_kv", C.c_int), ("head_dim", C.c_int), ("page_stride", C.c_int64), ("slot_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("table", C.c_void_p), ("table_stride", C.c_int), ("table_width", C.c_int),
+                ("n_seq", C.c_int), ("q_start", C.c_void_p), ("kv_len", C.c_void_p)]
+
+
+class QkStruct(C.Structure):
+    """clb200_qk (include/clb200.h)."""
+    _fields_ = [("T", C.c_int), ("n_head", C.c_int), ("src_type", C.c_uint32), ("q", C.c_void_p), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("norm", C.c_int), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("eps", C.c_float), ("rope", C.c_void_p),
+                ("n_pos", C.c_int), ("pairs", C.c_int), ("out", C.c_void_p), ("out_stride", C.c_int64)]
+
+
+class AttnStruct(C.Structure):
+    """clb200_attn (include/clb200.h)."""
+    _fields_ = [("T", C.c_int), ("n_head", C.c_int), ("max_q", C.c_int), ("q", C.c_void_p), ("q_stride", C.c_int64),
+                ("out", C.c_void_p), ("out_type", C.c_uint32), ("out_stride", C.c_int64), ("scale", C.c_float),
+                ("window", C.c_int), ("sinks", C.c_int), ("work", C.c_void_p), ("work_bytes", C.c_size_t)]
+
+
+class SamplingStruct(C.Structure):
+    """clb200_sampling (include/clb200.h)."""
+    _fields_ = [("rows", C.c_int), ("vocab", C.c_int), ("type", C.c_uint32), ("logits", C.c_void_p), ("stride", C.c_int64),
+                ("u", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p),
+                ("min_p", C.c_void_p), ("token", C.c_void_p), ("prob", C.c_void_p)]
+
+
+QK_NORM_NONE, QK_NORM_ROW, QK_NORM_HEAD = 0, 1, 2
+
+
 def header_functions() -> list[str]:
     """Names of the functions include/clb200.h declares."""
     text = open(HEADER).read()
@@ -191,6 +224,12 @@ def lib() -> C.CDLL:
         L.clb200_store_smart_stats.argtypes = [C.c_void_p]
         L.clb200_store_smart_stats.restype = SmartStats
         L.clb200_store_route.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]
+        serving = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]
+        L.clb200_qk_rope.argtypes = serving
+        L.clb200_attention.argtypes = serving
+        L.clb200_attention_work.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+        L.clb200_attention_work.restype = C.c_size_t
+        L.clb200_sample.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]
         L.clb200_store_failed.argtypes = [C.c_void_p]
         L.clb200_store_inject_fill_failure.argtypes = [C.c_void_p, C.c_int]
         _lib = L
@@ -363,6 +402,165 @@ class Context:
         return lib().clb200_route_dev(self.handle, _ptr(logits), T, E, K, C.addressof(sm) if sm else None,
                                       None if resident is None else _ptr(resident), resident_stride, _ptr(out),
                                       C.c_void_p(_stream(stream)))
+
+    def qk_rope(self, q, k, v, pages: "KvPages", q_start, kv_len, rope, *, q_norm=None, k_norm=None,
+                norm: int = QK_NORM_HEAD, pairs: bool = False, eps: float = 1e-6, out=None, stream=None):
+        """clb200_qk_rope on torch CUDA tensors: q [T, n_head, head_dim], k and v [T, n_kv, head_dim] (float32 or the cache's
+        type; rows any stride apart) are normalised, turned by position and, k and v, stored into `pages`; q_start [n_seq + 1]
+        and kv_len [n_seq] int32; rope [n_pos, head_dim] float32 (cosines, then sines). Returns the turned q, [T, n_head,
+        head_dim] of the cache's type (`out`, or a new tensor); asynchronous."""
+        import torch
+        st = _torch_stream(stream, self.device)
+        self._tensors(pages=pages.k, q=q, k=k, v=v, rope=rope, q_start=q_start, kv_len=kv_len, q_norm=q_norm, k_norm=k_norm, out=out)
+        T, H, D = q.shape
+        if k.shape != (T, pages.n_kv, D) or v.shape != k.shape or D != pages.head_dim:
+            raise ClutorError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit a cache of "
+                              f"{pages.n_kv} heads of {pages.head_dim}")
+        if k.dtype != q.dtype or v.dtype != q.dtype:
+            raise ClutorError("q, k and v must have one type")
+        if rope.dtype != torch.float32 or rope.dim() != 2 or rope.shape[1] != D or not rope.is_contiguous():
+            raise ClutorError("rope must be a contiguous float32 [n_pos, head_dim] tensor")
+        if norm:
+            nq, nk = (D, D) if norm == QK_NORM_HEAD else (H * D, pages.n_kv * D)
+            for w, n in ((q_norm, nq), (k_norm, nk)):
+                if w is None or w.dtype != torch.float32 or w.numel() != n or not w.is_contiguous():
+                    raise ClutorError(f"the norm's weights must be contiguous float32 tensors of {nq} and {nk} elements")
+        out = _out(out, (T, H, D), pages.k.dtype, q.device, st, stream)
+        kv = pages.struct(q_start, kv_len)
+        a = QkStruct(T, H, _dtype(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), _rows(q), _rows(k), _rows(v), int(norm),
+                     _ptr(q_norm), _ptr(k_norm), eps, rope.data_ptr(), rope.shape[0], int(pairs), out.data_ptr(), _rows(out))
+        self._check(lib().clb200_qk_rope(self.handle, C.byref(kv), C.byref(a), st.cuda_stream or CUDA_STREAM_LEGACY,
+                                         self._err, 512))
+        return out
+
+    def attention(self, q, pages: "KvPages", q_start, kv_len, *, max_q: int | None = None, scale: float | None = None,
+                  window: int = 0, sinks: int = 0, out=None, out_dtype=None, stream=None):
+        """clb200_attention on torch CUDA tensors: q [T, n_head, head_dim] of the cache's type, the new rows of sequences whose
+        keys and values (the new ones included) are in `pages`; max_q bounds the new rows of a sequence (default: T); scale
+        defaults to head_dim ** -0.5. Returns [T, n_head, head_dim] (`out`, or a new tensor of out_dtype, by default q's type);
+        asynchronous. The call's workspace is allocated for the stream, so calls may overlap."""
+        import torch
+        st = _torch_stream(stream, self.device)
+        self._tensors(pages=pages.k, q=q, q_start=q_start, kv_len=kv_len, out=out)
+        T, H, D = q.shape
+        if D != pages.head_dim or q.dtype != pages.k.dtype:
+            raise ClutorError(f"q {tuple(q.shape)} of {q.dtype} does not fit a {pages.k.dtype} cache of head_dim {pages.head_dim}")
+        out = _out(out, (T, H, D), out_dtype or (out.dtype if out is not None else q.dtype), q.device, st, stream)
+        kv = pages.struct(q_start, kv_len)
+        a = AttnStruct(T, H, T if max_q is None else int(max_q), q.data_ptr(), _rows(q), out.data_ptr(), _dtype(out), _rows(out),
+                       D ** -0.5 if scale is None else scale, int(window), int(sinks), None, 0)
+        n = lib().clb200_attention_work(self.handle, C.byref(kv), C.byref(a))
+        if n:
+            work = _empty(n, torch.uint8, q.device, st, stream)
+            a.work, a.work_bytes = work.data_ptr(), n
+        self._check(lib().clb200_attention(self.handle, C.byref(kv), C.byref(a), st.cuda_stream or CUDA_STREAM_LEGACY,
+                                           self._err, 512))
+        return out
+
+    def sample(self, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, *, token=None, prob=None, stream=None):
+        """clb200_sample on torch CUDA tensors: one token for each row of logits [rows, vocab] (float32, float16 or bfloat16)
+        from u [rows] float32 in [0, 1) and, each None or [rows], temperature, top_p, min_p (float32) and top_k (int32).
+        Returns (token [rows] int32, prob [rows] float32); asynchronous."""
+        import torch
+        st = _torch_stream(stream, self.device)
+        self._tensors(logits=logits, u=u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, token=token, prob=prob)
+        R, V = logits.shape
+        if V > 1 and logits.stride(1) != 1:
+            raise ClutorError("a row's logits must lie next to one another")
+        f32, i32 = torch.float32, torch.int32
+        for name, t, d in (("u", u, f32), ("temperature", temperature, f32), ("top_k", top_k, i32), ("top_p", top_p, f32),
+                           ("min_p", min_p, f32), ("token", token, i32), ("prob", prob, f32)):
+            if t is not None and (t.dtype != d or t.shape != (R,) or not t.is_contiguous()):
+                raise ClutorError(f"{name} must be a contiguous {d} tensor of {R} elements")
+        if token is None:
+            token = _empty(R, i32, logits.device, st, stream)
+        if prob is None:
+            prob = _empty(R, f32, logits.device, st, stream)
+        a = SamplingStruct(R, V, _dtype(logits), logits.data_ptr(), logits.stride(0), u.data_ptr(), _ptr(temperature), _ptr(top_k),
+                           _ptr(top_p), _ptr(min_p), token.data_ptr(), prob.data_ptr())
+        self._check(lib().clb200_sample(self.handle, C.byref(a), st.cuda_stream or CUDA_STREAM_LEGACY, self._err, 512))
+        return token, prob
+
+    def _tensors(self, **given) -> None:
+        """Raises unless every tensor given lies on this context's device."""
+        for name, t in given.items():
+            if t is not None and (not t.is_cuda or t.device.index != self.device):
+                raise ClutorError(f"{name} is on {t.device}, the context on cuda:{self.device}")
+
+
+def _torch_stream(stream, device: int):
+    import torch
+    return torch.cuda.current_stream(device) if stream is None else stream
+
+
+def _empty(shape, dtype, device, st, stream):
+    """A new tensor whose memory belongs to the stream `st` (given as `stream`, or the current one if that is None)."""
+    import torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(st):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _out(out, shape, dtype, device, st, stream):
+    if out is None:
+        return _empty(shape, dtype, device, st, stream)
+    if out.shape != shape or out.dtype != dtype:
+        raise ClutorError(f"out must be {list(shape)} of {dtype}")
+    return out
+
+
+def _dtype(t) -> int:
+    """The ggml type id of a tensor's type."""
+    import torch
+    d = t.dtype
+    if d is torch.float32:
+        return T_F32
+    if d is torch.float16:
+        return T_F16
+    if d is torch.bfloat16:
+        return T_BF16
+    raise ClutorError(f"{d} is not float32, float16 or bfloat16")
+
+
+def _rows(t) -> int:
+    """The stride of a [T, heads, head_dim] tensor's rows; the heads of a row must follow one another."""
+    T, H, D = t.shape
+    st = t.stride()
+    if st[2] != 1 or (H > 1 and st[1] != D):
+        raise ClutorError(f"the heads of a row must follow one another (strides {st} of {tuple(t.shape)})")
+    return st[0] if T > 1 else max(st[0], H * D)
+
+
+class KvPages:
+    """A paged key/value cache on the device (clb200_kv): k and v [n_pages, page_size, n_kv, head_dim] float16 or bfloat16 (the
+    same strides, head_dim contiguous), table [n_seq, width] int32: the pages of each sequence in order."""
+
+    def __init__(self, k, v, table):
+        import torch
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride() or k.stride(3) != 1:
+            raise ClutorError("k and v must be [n_pages, page_size, n_kv, head_dim] tensors of one type and layout")
+        if k.dtype not in (torch.float16, torch.bfloat16):
+            raise ClutorError(f"the cache is {k.dtype}: it must be float16 or bfloat16")
+        if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise ClutorError("table must be an int32 [n_seq, width] tensor")
+        if not k.is_cuda or v.device != k.device or table.device != k.device:
+            raise ClutorError("k, v and table must lie on one CUDA device")
+        self.k, self.v, self.table = k, v, table
+        self.n_pages, self.page_size, self.n_kv, self.head_dim = k.shape
+
+    def struct(self, q_start, kv_len) -> KvStruct:
+        """The clb200_kv of one call's sequences."""
+        import torch
+        k, t = self.k, self.table
+        n_seq, width = t.shape
+        if q_start.dtype != torch.int32 or kv_len.dtype != torch.int32 or q_start.shape != (n_seq + 1,) or kv_len.shape != (n_seq,) or \
+                not q_start.is_contiguous() or not kv_len.is_contiguous():
+            raise ClutorError(f"q_start and kv_len must be contiguous int32 tensors of {n_seq + 1} and {n_seq} elements")
+        ps, ss, hs, _ = k.stride()
+        return KvStruct(k.data_ptr(), self.v.data_ptr(), T_F16 if k.dtype is torch.float16 else T_BF16, self.n_pages, self.page_size,
+                        self.n_kv, self.head_dim, ps, ss, hs, t.data_ptr(), max(t.stride(0), width), width, n_seq,
+                        q_start.data_ptr(), kv_len.data_ptr())
 
 
 def backend() -> Backend:

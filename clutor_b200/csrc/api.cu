@@ -178,6 +178,8 @@ static const char *device_error_text(int code) {
     case ERR_WAIT_COPY: return "timed out waiting for a bulk copy into shared memory";
     case ERR_BAD_EXPERT: return "an expert id out of range reached the dispatch";
     case ERR_WAIT_PEER: return "timed out waiting for another GPU's rows or partial sums (does every rank take the same steps?)";
+    case ERR_BAD_PAGE: return "a position outside the page table, or a page id out of range";
+    case ERR_BAD_ROWS: return "rows out of range: a position below 0 or past the rotary table, or more new rows than max_q";
     default: return "unknown device error";
   }
 }

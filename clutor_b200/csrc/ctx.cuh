@@ -41,6 +41,7 @@ inline const char *type_name(uint32_t t) {
     case T_Q8_0: return "Q8_0";
     case T_F32: return "F32";
     case T_F16: return "F16";
+    case CLB200_T_BF16: return "BF16";
     default: return "an unsupported type";
   }
 }

@@ -31,7 +31,7 @@ extern "C" {
 #define CLB200_ABI_VERSION 1
 
 /* ggml tensor type ids, the values of the reference's CL_T_* (c/src/quant.h:7). Expert weights may be Q4_K, Q6_K or Q8_0. */
-enum { CLB200_T_F32 = 0, CLB200_T_F16 = 1, CLB200_T_Q8_0 = 8, CLB200_T_Q4_K = 12, CLB200_T_Q6_K = 14 };
+enum { CLB200_T_F32 = 0, CLB200_T_F16 = 1, CLB200_T_Q8_0 = 8, CLB200_T_Q4_K = 12, CLB200_T_Q6_K = 14, CLB200_T_BF16 = 30 };
 
 /* rows x cols weights of `type`, row-major, cols is the input width: the reference's cl_w (c/src/forward.h:18), same layout. */
 typedef struct { const uint8_t *p; uint32_t type; int rows, cols; } clb200_w;
@@ -316,6 +316,104 @@ clb200_smart_stats clb200_store_smart_stats(const clb200_store *s);
  * counters. Synchronous. Returns 0, or 1 with err set. */
 int clb200_store_route(clb200_ctx *c, clb200_store *s, int layer, const float *logits, clb200_route_result *out, char *err,
                        size_t errlen);
+
+/* ---- serving operators: many sequences over a paged key/value cache, and the choice of a token --------------------------- */
+/* For hosts that run their own step around clb200_moe_ffn_dev (several sequences in one batch, prompts in chunks, sampled
+ * tokens); clb200_model_prefill and clb200_model_generate_sampled run them on a model's own cache and logits. All take
+ * DEVICE pointers on the context's device, are asynchronous on `stream` (NULL: the context's stream), allocate nothing and
+ * may be captured in a CUDA graph. Arguments are checked at once (0, or 1 with err set and nothing launched); what only the
+ * device can see (a page id, a length, a position out of range) is skipped there and reported by clb200_status.
+ *
+ * A paged cache: n_pages pages of page_size slots (a multiple of 16), a slot holding a token's key (and value) of n_kv heads
+ * of head_dim (64, 128 or 256) half-precision elements (CLB200_T_F16 or CLB200_T_BF16). Element d of head h in slot i of page
+ * p is at k[p * page_stride + i * slot_stride + h * head_stride + d], v likewise (strides in elements, multiples of 8; k and v
+ * on 16-byte boundaries). Position t of sequence s lies in page table[s * table_stride + t / page_size], slot t % page_size;
+ * table_width ids of each row may be read. Several sequences may name the same page (a shared prefix).
+ *
+ * The step's new tokens stand in rows, sequence after sequence: q_start [n_seq + 1] (not descending) gives the first row of
+ * each, kv_len [n_seq] its length with the new tokens in. Row q_start[s] + i is position kv_len[s] - (q_start[s + 1] -
+ * q_start[s]) + i of sequence s. A sequence may have no rows. Rows at or past q_start[n_seq] (a padded batch) belong to
+ * nobody: their outputs are left as they were. Slots at or past kv_len may hold anything, infinities and NaN included. */
+typedef struct {
+  void *k, *v;
+  uint32_t type;
+  int n_pages, page_size, n_kv, head_dim;
+  int64_t page_stride, slot_stride, head_stride;
+  const int *table;          /* [n_seq][table_stride] */
+  int table_stride, table_width, n_seq;
+  const int *q_start, *kv_len;
+} clb200_kv;
+
+/* Norms of queries and keys, the rotation by position, and the store of keys and values into the cache, one pass over the
+ * T rows. For each row: x = q (n_head heads) and k (n_kv heads) are normalised -- CLB200_QK_NORM_HEAD: x / sqrt(mean of the
+ * head's squares + eps) * weight[head_dim], the weights shared by the heads; _ROW: the mean over all of the row's heads,
+ * weight[heads * head_dim]; _NONE: as they are -- then turned by the row's position: rope [n_pos][head_dim] holds head_dim / 2
+ * cosines and head_dim / 2 sines per position; elements (i, i + head_dim / 2) form a pair, or with pairs = 1 (2i, 2i + 1). q
+ * goes to out [T][n_head][head_dim] in the cache's type, k and v (v as it is) to the row's slot. q, k and v are of src_type
+ * (CLB200_T_F32, or the cache's type), rows q_stride / k_stride / v_stride elements apart, so one fused product's output can
+ * be passed as three. Sums and products are held in fp32 and rounded once, to the cache's type. out must not overlap the
+ * inputs, and the slots of new tokens must differ from one another. What the reference's forward pass does for one sequence
+ * at c/src/forward.c:1104-1112. */
+enum { CLB200_QK_NORM_NONE = 0, CLB200_QK_NORM_ROW = 1, CLB200_QK_NORM_HEAD = 2 };
+typedef struct {
+  int T, n_head;
+  uint32_t src_type;
+  const void *q, *k, *v;
+  int64_t q_stride, k_stride, v_stride;
+  int norm;
+  const float *q_norm, *k_norm;
+  float eps;
+  const float *rope;
+  int n_pos, pairs;
+  void *out;
+  int64_t out_stride;
+} clb200_qk;
+int clb200_qk_rope(clb200_ctx *c, const clb200_kv *kv, const clb200_qk *a, void *stream, char *err, size_t errlen);
+
+/* Attention of the T new rows over the cache (their own keys and values already stored): out[t][h] = sum_j p_j v_j, p =
+ * softmax over the visible j of scale * q[t][h] . k_j, head h reading key/value head h / (n_head / n_kv). Visible to position
+ * p: j <= p, and with window > 0 only j > p - window or j < sinks. A row that sees nothing gets zeros. q is of the cache's
+ * type, out of the cache's type or CLB200_T_F32 (scores and sums are fp32; the products of probabilities and values take the
+ * probabilities in the cache's type). The values of every slot below kv_len must be finite. max_q: no sequence has more new
+ * rows than this (it chooses the kernel; a longer one is reported by clb200_status and its rows are left as they were).
+ * n_head / n_kv at most 16. work: clb200_attention_work bytes of device memory (on a 256-byte boundary) that the call
+ * uses until it is done, so calls that may run at the same time, captured graphs among them, need one each. */
+typedef struct {
+  int T, n_head, max_q;
+  const void *q;
+  int64_t q_stride;
+  void *out;
+  uint32_t out_type;
+  int64_t out_stride;
+  float scale;
+  int window, sinks;
+  void *work;
+  size_t work_bytes;
+} clb200_attn;
+size_t clb200_attention_work(clb200_ctx *c, const clb200_kv *kv, const clb200_attn *a);
+int clb200_attention(clb200_ctx *c, const clb200_kv *kv, const clb200_attn *a, void *stream, char *err, size_t errlen);
+
+/* One token for each of `rows` rows of logits [rows][vocab] (CLB200_T_F32, _F16 or _BF16, rows `stride` elements apart; vocab
+ * up to 262144) from one given random number each, u [rows] in [0, 1). With x the row's logits (NaN counts as -infinity), M
+ * the largest and w_i = exp((x_i - M) / temperature), tokens are ordered by x descending, then id ascending, and kept when
+ * they are among the first top_k, inside the shortest prefix of those whose w sum to at least top_p of their total (one
+ * token at least), and have w_i >= min_p. token is the first kept id, ids ascending, at which the running sum of the kept w
+ * exceeds u times their total; prob its w over that total. Each setting has a value per row; a NULL array, top_k <= 0,
+ * top_p >= 1 and min_p <= 0 leave that filter out, temperature NULL is 1, and temperature <= 0 takes the arg-max (the lowest
+ * id on ties) with prob 1. A row with nothing above -infinity gives token -1, prob 0. prob may be NULL. The weights are
+ * summed as 64-bit integers in units of 2^-44, so the result does not depend on any order of execution. */
+typedef struct {
+  int rows, vocab;
+  uint32_t type;
+  const void *logits;
+  int64_t stride;
+  const float *u, *temperature;
+  const int *top_k;
+  const float *top_p, *min_p;
+  int *token;
+  float *prob;
+} clb200_sampling;
+int clb200_sample(clb200_ctx *c, const clb200_sampling *s, void *stream, char *err, size_t errlen);
 
 /* ---- the plugin seam: a cl_backend for cl_matvec_batch ------------------------------------------------------------------- */
 /* Layout-compatible copies of the reference's cl_q8k, cl_xq and cl_mv (c/src/quant.h:22-34) and cl_backend (backend.h:9-13). */
