@@ -1,84 +1,393 @@
 // clb200_attention: attention of chunks of new tokens over a paged key/value cache.
 #include <algorithm>
 
+#include "attn.cuh"
 #include "ctx.cuh"
 #include "serve.cuh"
 
 namespace clb {
 namespace {
 
-constexpr int AT = 128, AW = AT / 32;
+// ---- few rows: mma.sync ----------------------------------------------------------------------------------------------------
 
-struct AttnArgs {
-  clb200_kv kv;
-  clb200_attn a;
-  int *err;
+constexpr int RT = 128, RW = RT / 32, RN = 16 * RW;   // threads, warps, positions per tile (16 per warp)
+
+template <int HD, int MT>
+struct RowsShape {
+  static constexpr int ROWS = 16 * MT;
+  static constexpr int STAGES = HD == 64 ? 6 : 3;
+  static constexpr uint32_t HALF = 16 * HD * 2, STAGE = 2 * HALF;         // a warp's keys (then values) of one tile
+  static constexpr uint32_t Q = ROWS * HD * 2, KV = RW * STAGES * STAGE;  // KV: also the warps' states when they are joined
+  static constexpr uint32_t SMEM = Q + KV + 2 * RW * ROWS * 4;
+  static constexpr int PER_SM = HD == 256 ? 1 : 2;
+  static_assert(RW * ROWS * HD * 4 <= static_cast<int>(KV), "the joined states fit the stages");
 };
 
-// One CTA per (row, query head): warp w takes every AW-th visible position, a lane HD / 32 elements of the head, with a
-// running maximum and sum per warp; the warps' states are joined at the end.
-template <typename C, typename O, int HD>
-__global__ void __launch_bounds__(AT) attn_plain_kernel(const AttnArgs g) {
-  constexpr int EPL = HD / 32;
-  __shared__ float sm[AW], sl[AW], so[AW][HD];
+CLB_DEV void cp_async16(uint32_t dst, const void *src, bool take) {   // 16 bytes, or zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+CLB_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int K>
+CLB_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(K) : "memory"); }
+CLB_DEV void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+CLB_DEV void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename C>
+CLB_DEV void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (sizeof(C) == 2 && __is_same(C, __half))
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename C>
+CLB_DEV uint32_t pack2(float a, float b) {   // a in the low half
+  if constexpr (__is_same(C, __half)) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+}
+// Byte offset of 16-byte chunk c of row r in rows of HD half-precision elements; eight rows' equal chunks in eight bank groups.
+template <int HD>
+CLB_DEV uint32_t chunk_at(int r, int c) { return static_cast<uint32_t>(r * HD * 2 + ((c ^ (r & 7)) << 4)); }
+
+template <typename C, typename O, int HD, int MT>
+__global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kernel(const AttnArgs g) {
+  using S = RowsShape<HD, MT>;
+  constexpr int KK = HD / 16, ROWS = S::ROWS;
+  constexpr bool QREG = MT * KK <= 8;   // the query fragments stay in registers
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ int64_t prefix[ATTN_MAX_SEQ + 1];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
   const clb200_attn &a = g.a;
   const clb200_kv &kv = g.kv;
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (row < kv.q_start[0] || row >= kv.q_start[kv.n_seq]) return;
-  const int s = seq_of_row(kv.q_start, kv.n_seq, row);
-  if (kv.q_start[s + 1] - kv.q_start[s] > a.max_q) {
-    if (threadIdx.x == 0) set_error(g.err, ERR_BAD_ROWS);
-    return;
-  }
-  const int pos = kv.kv_len[s] - kv.q_start[s + 1] + row;
-  const int n = min(pos, kv.kv_len[s] - 1) + 1;
-  const int kh = h / (a.n_head / kv.n_kv);
-  float q[EPL], o[EPL], m = -INFINITY, l = 0.f;
+  const uint32_t q_sm = smem_addr(sm), kv_sm = q_sm + S::Q + warp * S::STAGES * S::STAGE;
+  float *join = reinterpret_cast<float *>(sm + S::Q), *join_m = reinterpret_cast<float *>(sm + S::Q + S::KV), *join_l = join_m + RW * ROWS;
+  const float sc = a.scale * LOG2E;
+  const int gr = lane >> 2, gc = (lane & 3) * 2;   // the lane's row and first column in an accumulator
+  if (tid == 0) g.joins[cta] = make_int4(0, 0, 0, 0);
+  AttnRun<RN> run;
+  run.init(g, prefix, cta);
+  while (run.more()) {
+    const AttnSeq q = run.q;
+    const AttnSpan span = attn_span<RN>(g, q, run.qt);
+    const int i0 = run.i0, n = run.tiles(span), t0 = run.qt * g.tpi, head = run.head, s = run.s;
+    const bool whole = n == span.nt;
+    __syncthreads();   // the last item's queries and joined states have been read
+    for (int i = tid; i < ROWS * (HD / 8); i += RT) {
+      const int r = i / (HD / 8), c = i % (HD / 8), t = t0 + r / g.group, h = head * g.group + r % g.group;
+      const bool live = r < g.tpi * g.group && t < q.nq;
+      const C *src = static_cast<const C *>(a.q) + (live ? (q.row + t) * a.q_stride + h * HD + 8 * c : 0);
+      cp_async16(q_sm + chunk_at<HD>(r, c), src, live);
+    }
+    cp_commit();
+    // this warp's 16 positions of tile i of the item
+    auto issue = [&](int i) {
+      if (i < n) {
+        const int j0 = span.tile(i0 + i) * RN + warp * 16;
+        if (j0 <= span.hi) {
+          const int page = page_of(kv, s, j0, g.err);
+          const int64_t base = (page < 0 ? 0 : page * kv.page_stride + (j0 % kv.page_size) * kv.slot_stride) + head * kv.head_stride;
+          const uint32_t dst = kv_sm + (i % S::STAGES) * S::STAGE;
+          const int left = page < 0 ? 0 : q.kv - j0;   // positions behind the sequence's end come as zeros
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) {
-    q[e] = to_f32(static_cast<const C *>(a.q)[row * a.q_stride + h * HD + lane * EPL + e]);
-    o[e] = 0.f;
-  }
-  for (int j = warp; j < n; j += AW) {
-    if (a.window > 0 && j <= pos - a.window && j >= a.sinks) continue;
-    const int page = page_of(kv, s, j, g.err);
-    if (page < 0) continue;
-    const int64_t at = page * kv.page_stride + (j % kv.page_size) * kv.slot_stride + kh * kv.head_stride + lane * EPL;
-    float d = 0.f;
+          for (int e = lane; e < 16 * (HD / 8); e += 32) {
+            const int r = e / (HD / 8), c = e % (HD / 8);
+            const int64_t at = r < left ? base + r * kv.slot_stride + 8 * c : 0;
+            cp_async16(dst + chunk_at<HD>(r, c), static_cast<const C *>(kv.k) + at, r < left);
+            cp_async16(dst + S::HALF + chunk_at<HD>(r, c), static_cast<const C *>(kv.v) + at, r < left);
+          }
+        }
+      }
+      cp_commit();
+    };
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) d = fmaf(q[e], to_f32(static_cast<const C *>(kv.k)[at + e]), d);
+    for (int i = 0; i < S::STAGES - 1; ++i) issue(i);
+    cp_wait<S::STAGES - 1>();   // the queries
+    __syncthreads();
+    uint32_t qf[QREG ? MT : 1][QREG ? KK : 1][4];
+    auto load_q = [&](int mt, int kk, uint32_t (&f)[4]) {
+      ldsm4(f, q_sm + chunk_at<HD>(16 * mt + (lane & 15), 2 * kk + (lane >> 4)));
+    };
+    if constexpr (QREG)
 #pragma unroll
-    for (int i = 16; i > 0; i >>= 1) d += __shfl_xor_sync(FULL_MASK, d, i);
-    d *= a.scale;
-    const float mn = fmaxf(m, d), f = m == -INFINITY ? 0.f : expf(m - mn), p = mn == -INFINITY ? 0.f : expf(d - mn);
-    l = fmaf(l, f, p);
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) o[e] = fmaf(o[e], f, p * to_f32(static_cast<const C *>(kv.v)[at + e]));
-    m = mn;
-  }
-  if (lane == 0) { sm[warp] = m; sl[warp] = l; }
+        for (int kk = 0; kk < KK; ++kk) load_q(mt, kk, qf[mt][kk]);
+    float o[MT][HD / 8][4], m[MT][2], l[MT][2];
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) so[warp][lane * EPL + e] = o[e];
-  __syncthreads();
-  float mm = -INFINITY, ll = 0.f;
-  for (int w = 0; w < AW; ++w) mm = fmaxf(mm, sm[w]);
-  float f[AW];
-  for (int w = 0; w < AW; ++w) { f[w] = sm[w] == -INFINITY ? 0.f : expf(sm[w] - mm); ll = fmaf(f[w], sl[w], ll); }
-  for (int d = threadIdx.x; d < HD; d += AT) {
-    float v = 0.f;
-    for (int w = 0; w < AW; ++w) v = fmaf(f[w], so[w][d], v);
-    static_cast<O *>(a.out)[row * a.out_stride + h * HD + d] = from_f32<O>(ll > 0.f ? v / ll : 0.f);
+    for (int mt = 0; mt < MT; ++mt) {
+      m[mt][0] = m[mt][1] = -INFINITY;
+      l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[mt][d][e] = 0.f;
+    }
+    for (int i = 0; i < n; ++i) {
+      cp_wait<S::STAGES - 2>();
+      __syncwarp();
+      const int j0 = span.tile(i0 + i) * RN + warp * 16;
+      if (j0 <= span.hi) {
+        const uint32_t ks = kv_sm + (i % S::STAGES) * S::STAGE, vs = ks + S::HALF;
+        float x[MT][2][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[mt][e >> 2][e & 3] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          uint32_t b[4];
+          ldsm4(b, ks + chunk_at<HD>((lane >> 4) * 8 + (lane & 7), 2 * kk + ((lane >> 3) & 1)));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            if constexpr (QREG) {
+              mma16816<C>(x[mt][0], qf[mt][kk], b[0], b[1]);
+              mma16816<C>(x[mt][1], qf[mt][kk], b[2], b[3]);
+            } else {
+              uint32_t f[4];
+              load_q(mt, kk, f);
+              mma16816<C>(x[mt][0], f, b[0], b[1]);
+              mma16816<C>(x[mt][1], f, b[2], b[3]);
+            }
+          }
+        }
+        // some row does not see all 16 positions
+        const bool edge = j0 + 15 > span.lo || (a.window > 0 && j0 <= span.hi - a.window && j0 + 15 >= a.sinks);
+        uint32_t p[MT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[mt][e >> 2][e & 3] *= sc;
+          if (edge) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int r = 16 * mt + gr + ((e & 2) ? 8 : 0), j = j0 + (e >> 2) * 8 + gc + (e & 1);
+              if (!attn_sees(g, span.lo + r / g.group, j)) x[mt][e >> 2][e & 3] = -INFINITY;
+            }
+          }
+          float mx[2] = {m[mt][0], m[mt][1]};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx[(e >> 1) & 1] = fmaxf(mx[(e >> 1) & 1], x[mt][e >> 2][e & 3]);
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            mx[w] = fmaxf(mx[w], __shfl_xor_sync(FULL_MASK, mx[w], 1));
+            mx[w] = fmaxf(mx[w], __shfl_xor_sync(FULL_MASK, mx[w], 2));
+          }
+          if (__any_sync(FULL_MASK, mx[0] > m[mt][0] || mx[1] > m[mt][1])) {
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const float f = m[mt][w] == -INFINITY ? 0.f : exp2_approx(m[mt][w] - mx[w]);
+              l[mt][w] *= f;
+              m[mt][w] = mx[w];
+#pragma unroll
+              for (int d = 0; d < HD / 8; ++d) { o[mt][d][2 * w] *= f; o[mt][d][2 * w + 1] *= f; }
+            }
+          }
+          const float z[2] = {m[mt][0] == -INFINITY ? 0.f : m[mt][0], m[mt][1] == -INFINITY ? 0.f : m[mt][1]};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float &v = x[mt][e >> 2][e & 3];
+            v = exp2_approx(v - z[(e >> 1) & 1]);
+            l[mt][(e >> 1) & 1] += v;
+          }
+          // the probabilities are rounded to the cache's type, the type of the matrix product's operands
+          p[mt][0] = pack2<C>(x[mt][0][0], x[mt][0][1]);
+          p[mt][1] = pack2<C>(x[mt][0][2], x[mt][0][3]);
+          p[mt][2] = pack2<C>(x[mt][1][0], x[mt][1][1]);
+          p[mt][3] = pack2<C>(x[mt][1][2], x[mt][1][3]);
+        }
+#pragma unroll
+        for (int d = 0; d < KK; ++d) {
+          uint32_t b[4];
+          ldsm4t(b, vs + chunk_at<HD>((lane & 7) + ((lane >> 3) & 1) * 8, 2 * d + (lane >> 4)));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16816<C>(o[mt][2 * d], p[mt], b[0], b[1]);
+            mma16816<C>(o[mt][2 * d + 1], p[mt], b[2], b[3]);
+          }
+        }
+      }
+      __syncwarp();   // the stage has been read by every lane
+      issue(i + S::STAGES - 1);
+    }
+    cp_wait<0>();
+    if (!run.more() || run.at + n >= run.end) grid_launch_dependents();
+    // the warps' states: maximum and sum of each row, values in fp32, joined in warp order
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        l[mt][w] += __shfl_xor_sync(FULL_MASK, l[mt][w], 1);
+        l[mt][w] += __shfl_xor_sync(FULL_MASK, l[mt][w], 2);
+        if ((lane & 3) == 0) {
+          join_m[warp * ROWS + 16 * mt + gr + 8 * w] = m[mt][w];
+          join_l[warp * ROWS + 16 * mt + gr + 8 * w] = l[mt][w];
+        }
+      }
+    __syncthreads();   // every warp's stages are free
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+          *reinterpret_cast<float2 *>(join + (warp * ROWS + 16 * mt + gr + 8 * w) * HD + 8 * d + gc) = make_float2(o[mt][d][2 * w], o[mt][d][2 * w + 1]);
+    __syncthreads();
+    const int slot = 2 * cta + (i0 == 0 ? 1 : 0);
+    for (int i = tid; i < ROWS * (HD / 4); i += RT) {
+      const int r = i / (HD / 4), c = 4 * (i % (HD / 4)), t = t0 + r / g.group;
+      if (r >= g.tpi * g.group || t >= q.nq) continue;
+      float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+      for (int w = 0; w < RW; ++w) mm = fmaxf(mm, join_m[w * ROWS + r]);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < RW; ++w) {
+        const float mw = join_m[w * ROWS + r], f = mw == -INFINITY ? 0.f : exp2_approx(mw - mm);
+        const float4 u = *reinterpret_cast<const float4 *>(join + (w * ROWS + r) * HD + c);
+        ll = fmaf(f, join_l[w * ROWS + r], ll);
+        v.x = fmaf(f, u.x, v.x); v.y = fmaf(f, u.y, v.y); v.z = fmaf(f, u.z, v.z); v.w = fmaf(f, u.w, v.w);
+      }
+      if (whole) {
+        const float inv = ll > 0.f ? 1.0f / ll : 0.f;
+        store4<O>(static_cast<O *>(a.out) + (q.row + t) * a.out_stride + (head * g.group + r % g.group) * HD + c, v, inv);
+      } else {
+        *reinterpret_cast<float4 *>(g.piece_o + (static_cast<int64_t>(slot) * g.rows + r) * HD + c) = v;
+        if (c == 0) g.piece_ml[static_cast<int64_t>(slot) * g.rows + r] = make_float2(mm, ll);
+      }
+    }
+    if (!whole && i0 == 0 && tid == 0) g.joins[cta] = make_int4(s, head, run.qt, run.pieces(span.nt - n));
+    run.advance(g, n);
   }
 }
 
-template <typename C, typename O>
-void launch_hd(const AttnArgs &g, cudaStream_t st) {
-  const dim3 grid(g.a.T, g.a.n_head);
-  switch (g.kv.head_dim) {
-    case 64: attn_plain_kernel<C, O, 64><<<grid, AT, 0, st>>>(g); break;
-    case 128: attn_plain_kernel<C, O, 128><<<grid, AT, 0, st>>>(g); break;
-    default: attn_plain_kernel<C, O, 256><<<grid, AT, 0, st>>>(g); break;
+// ---- joining the pieces of items that fell into several runs ---------------------------------------------------------------
+
+constexpr int JT = 128, JW = JT / 32;
+
+// A CTA per row, its warps taking every JW-th piece: the largest of the pieces' maxima first, then their values scaled to it;
+// the warps' sums are added in warp order.
+template <typename O, int HD>
+__global__ void __launch_bounds__(JT) attn_join_kernel(const AttnArgs g) {
+  constexpr int EPL = HD / 32;
+  __shared__ float sum[JW][HD], den[JW];
+  grid_dependency_wait();
+  const int4 j = g.joins[blockIdx.x];
+  if (j.w == 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.y;
+  const AttnSeq q = attn_seq(g, j.x, false);
+  const int t = j.z * g.tpi + r / g.group;
+  if (r >= g.tpi * g.group || t >= q.nq) return;
+  // piece i: slot 1 of this CTA, then slot 0 of the CTAs that follow
+  auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * g.rows + r; };
+  float mm = -INFINITY;
+  for (int i = lane; i <= j.w; i += 32) mm = fmaxf(mm, g.piece_ml[slot(i)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(FULL_MASK, mm, o));
+  float v[EPL], l = 0.f;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) v[e] = 0.f;
+#pragma unroll 4
+  for (int i = warp; i <= j.w; i += JW) {
+    const float2 ml = g.piece_ml[slot(i)];
+    const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - mm);
+    const float *src = g.piece_o + slot(i) * HD;
+    l = fmaf(f, ml.y, l);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) v[e] = fmaf(f, src[lane + 32 * e], v[e]);
   }
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) sum[warp][lane + 32 * e] = v[e];
+  if (lane == 0) den[warp] = l;
+  __syncthreads();
+  l = 0.f;
+  for (int w = 0; w < JW; ++w) l += den[w];
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  O *dst = static_cast<O *>(g.a.out) + (q.row + t) * g.a.out_stride + (j.y * g.group + r % g.group) * HD;
+  for (int d = threadIdx.x; d < HD; d += JT) {
+    float o = 0.f;
+    for (int w = 0; w < JW; ++w) o += sum[w][d];
+    dst[d] = from_f32<O>(o * inv);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------
+
+template <typename F>
+cudaError_t allow_smem(F *fn, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 64 && done[dev]) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done[dev] = true;
+  return e;
+}
+
+template <typename C, typename O, int HD, int MT>
+cudaError_t launch_rows(const AttnArgs &g, cudaStream_t st) {
+  using S = RowsShape<HD, MT>;
+  static bool done[64] = {};
+  const cudaError_t e = allow_smem(attn_rows_kernel<C, O, HD, MT>, S::SMEM, done);
+  if (e != cudaSuccess) return e;
+  attn_rows_kernel<C, O, HD, MT><<<g.nc, RT, S::SMEM, st>>>(g);
+  return cudaGetLastError();
+}
+
+template <typename O, int HD>
+cudaError_t launch_join(const AttnArgs &g, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(g.nc, g.tpi * g.group);
+  cfg.blockDim = dim3(JT);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_join_kernel<O, HD>, g);
+}
+
+template <typename C, typename O, int HD>
+cudaError_t launch_all(const AttnArgs &g, cudaStream_t st) {
+  cudaError_t e;
+  if (g.rows == 16) e = launch_rows<C, O, HD, 1>(g, st);
+  else if constexpr (HD <= 128) e = launch_rows<C, O, HD, 2>(g, st);
+  else e = cudaErrorInvalidValue;
+  return e != cudaSuccess ? e : launch_join<O, HD>(g, st);
+}
+
+template <typename C, typename O>
+cudaError_t launch_hd(const AttnArgs &g, cudaStream_t st) {
+  switch (g.kv.head_dim) {
+    case 64: return launch_all<C, O, 64>(g, st);
+    case 128: return launch_all<C, O, 128>(g, st);
+    default: return launch_all<C, O, 256>(g, st);
+  }
+}
+
+// The kernel's shape for a call, and its workspace: partial values, their maxima and sums, the list of items to join.
+struct AttnPlan {
+  int rows, nc;
+  size_t off_ml, off_joins, total;
+};
+AttnPlan attn_plan(int sms, const clb200_kv &kv, const clb200_attn &a) {
+  AttnPlan p{};
+  const int group = a.n_head / kv.n_kv;
+  p.rows = a.max_q * static_cast<int64_t>(group) <= 16 || kv.head_dim == 256 ? 16 : 32;
+  p.nc = sms * (kv.head_dim == 256 ? 1 : 2);
+  const size_t pieces = static_cast<size_t>(p.nc) * 2 * p.rows;
+  p.off_ml = al(pieces * kv.head_dim * 4);
+  p.off_joins = p.off_ml + al(pieces * 8);
+  p.total = p.off_joins + al(static_cast<size_t>(p.nc) * 16);
+  return p;
 }
 
 int check(const clb200_kv *kv, const clb200_attn *a, char *err, size_t errlen) {
@@ -113,25 +422,48 @@ int check(const clb200_kv *kv, const clb200_attn *a, char *err, size_t errlen) {
 using namespace clb;
 
 extern "C" size_t clb200_attention_work(clb200_ctx *c, const clb200_kv *kv, const clb200_attn *a) {
-  if (!c || !kv || !a) return 0;
-  return 0;
+  char err[8];
+  if (!c || check(kv, a, err, sizeof err)) return 0;
+  return attn_plan(c->sms, *kv, *a).total;
 }
 
 extern "C" int clb200_attention(clb200_ctx *c, const clb200_kv *kv, const clb200_attn *a, void *stream, char *err, size_t errlen) {
   if (check(kv, a, err, errlen)) return 1;
   if (!c) { errf(err, errlen, "no context"); return 1; }
   if (a->T == 0 || kv->n_seq == 0) return 0;
+  const AttnPlan p = attn_plan(c->sms, *kv, *a);
+  if (!a->work || a->work_bytes < p.total || (reinterpret_cast<uintptr_t>(a->work) & 255)) {
+    errf(err, errlen, "the workspace is %zu bytes at %p: it must be %zu bytes (clb200_attention_work) on a 256-byte boundary", a->work ? a->work_bytes : 0,
+         a->work, p.total);
+    return 1;
+  }
   const OnDevice on(c->device);
-  const AttnArgs g{*kv, *a, c->small};
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : c->stream;
   const bool f32 = a->out_type == T_F32;
-  if (kv->type == T_F16) {
-    if (f32) launch_hd<__half, float>(g, st);
-    else launch_hd<__half, __half>(g, st);
-  } else {
-    if (f32) launch_hd<__nv_bfloat16, float>(g, st);
-    else launch_hd<__nv_bfloat16, __nv_bfloat16>(g, st);
+  uint8_t *w = static_cast<uint8_t *>(a->work);
+  for (int s0 = 0; s0 < kv->n_seq; s0 += ATTN_MAX_SEQ) {
+    AttnArgs g{};
+    g.kv = *kv;
+    g.kv.table += static_cast<int64_t>(s0) * kv->table_stride;
+    g.kv.q_start += s0;
+    g.kv.kv_len += s0;
+    g.kv.n_seq = std::min(kv->n_seq - s0, ATTN_MAX_SEQ);
+    g.a = *a;
+    g.a.window = std::min(a->window, 1 << 30);
+    g.a.sinks = std::min(a->sinks, 1 << 30);
+    g.err = c->small;
+    g.group = a->n_head / kv->n_kv;
+    g.rows = p.rows;
+    g.tpi = p.rows / g.group;
+    g.nc = p.nc;
+    g.min_run = 4;
+    g.piece_o = reinterpret_cast<float *>(w);
+    g.piece_ml = reinterpret_cast<float2 *>(w + p.off_ml);
+    g.joins = reinterpret_cast<int4 *>(w + p.off_joins);
+    cudaError_t e;
+    if (kv->type == T_F16) e = f32 ? launch_hd<__half, float>(g, st) : launch_hd<__half, __half>(g, st);
+    else e = f32 ? launch_hd<__nv_bfloat16, float>(g, st) : launch_hd<__nv_bfloat16, __nv_bfloat16>(g, st);
+    CUDA_OR(e, "launching the attention");
   }
-  CUDA_OR(cudaGetLastError(), "launching the attention");
   return 0;
 }

@@ -1,0 +1,185 @@
+// The attention's division of work, shared by its kernels (attn.cu, attn_tc.cu).
+//
+// An item is one sequence, one key/value head and up to `tpi` of the sequence's new tokens, whose tpi x group rows (row = token
+// x group + query head of the group) share every key and value they read. Its keys come in tiles of N positions: those up to
+// the last token's position, without the tiles that a window hides from all of its tokens. Every item has at least one tile (a
+// fully hidden one gives zeros). The tiles of all items, item after item, are dealt to the CTAs in equal runs, so ragged
+// batches and long caches balance by themselves; an item that falls into several runs leaves one partial state (running
+// maximum, sum, unnormalised values per row) per run in the workspace, and a second kernel joins them. A CTA's run holds at
+// most two such pieces: the first item's, when an earlier CTA began it (slot 0), and the last item's, when this CTA begins and
+// does not finish it (slot 1).
+#pragma once
+#include "serve.cuh"
+
+namespace clb {
+
+constexpr int ATTN_MAX_SEQ = 512;   // sequences a launch takes (the host launches once per so many)
+
+struct AttnArgs {
+  clb200_kv kv;
+  clb200_attn a;
+  int *err;
+  int group, tpi;     // query heads per key/value head, new tokens per item
+  int nc, min_run;    // CTAs, tiles a CTA takes at least
+  int rows;           // rows of a piece (>= tpi x group)
+  float *piece_o;     // [nc][2][rows][head_dim]
+  float2 *piece_ml;   // [nc][2][rows] maximum (times log2 e) and sum
+  int4 *joins;        // [nc] the item that begins in this CTA and does not end there: sequence, head, q tile, pieces that
+                      // follow; pieces 0: none
+};
+
+struct AttnSeq {
+  int row, nq, kv;   // first row, new tokens (0: nothing to do), length
+};
+// What the device arrays say of sequence s, made safe: a sequence whose rows or length do not fit is skipped, and reported
+// when `report` is set.
+CLB_DEV AttnSeq attn_seq(const AttnArgs &g, int s, bool report) {
+  const int a = g.kv.q_start[s], z = g.kv.q_start[s + 1], n = max(g.kv.kv_len[s], 0);
+  AttnSeq q{a, z - a, n};
+  if (z <= a) return AttnSeq{a, 0, n};
+  if (a < 0 || z > g.a.T || q.nq > g.a.max_q) {
+    if (report) set_error(g.err, ERR_BAD_ROWS);
+    q.nq = 0;
+  } else if (n > static_cast<int64_t>(g.kv.table_width) * g.kv.page_size) {
+    if (report) set_error(g.err, ERR_BAD_PAGE);
+    q.nq = 0;
+  }
+  return q;
+}
+
+// The tiles of an item: tile i of nt is i for i < sinks, else start + i.
+struct AttnSpan {
+  int lo, hi;        // positions of its first and last token (may be negative: they see nothing)
+  int sinks, start, nt;
+  CLB_DEV int tile(int i) const { return i < sinks ? i : start + i; }
+};
+template <int N>
+CLB_DEV AttnSpan attn_span(const AttnArgs &g, const AttnSeq &q, int qt) {
+  AttnSpan p;
+  const int first = q.kv - q.nq, t0 = qt * g.tpi;
+  p.lo = first + t0;
+  p.hi = first + min(t0 + g.tpi, q.nq) - 1;
+  const int end = p.hi < 0 ? 1 : p.hi / N + 1;
+  p.sinks = 0;
+  p.start = 0;
+  p.nt = end;
+  if (g.a.window > 0) {
+    const int w0 = max(p.lo - g.a.window + 1, 0) / N, ns = g.a.sinks >= w0 * N ? w0 : (g.a.sinks + N - 1) / N;
+    if (ns < w0) {
+      p.sinks = ns;
+      p.start = w0 - ns;
+      p.nt = ns + end - w0;
+    }
+  }
+  return p;
+}
+// Whether row position p sees position j (j below the sequence's length).
+CLB_DEV bool attn_sees(const AttnArgs &g, int p, int j) {
+  return j <= p && (g.a.window <= 0 || j > p - g.a.window || j < g.a.sinks);
+}
+
+// A CTA's run of tiles. Every thread of the CTA makes the same one (init synchronises the CTA; `prefix` is shared memory of
+// ATTN_MAX_SEQ + 1 words).
+template <int N>
+struct AttnRun {
+  int64_t at, end;        // tiles of all items: the next, and the first that is another CTA's
+  int64_t run;            // tiles a CTA takes
+  int s, head, qt, i0;    // the next item, and its first tile that is this CTA's
+  AttnSeq q;
+
+  CLB_DEV void init(const AttnArgs &g, int64_t *prefix, int cta) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5, n_seq = g.kv.n_seq;
+    for (int k = warp; k < n_seq; k += nw) {
+      const AttnSeq t = attn_seq(g, k, cta == 0 && lane == 0);
+      const int nqt = (t.nq + g.tpi - 1) / g.tpi;
+      int64_t sum = 0;
+      for (int i = lane; i < nqt; i += 32) sum += attn_span<N>(g, t, i).nt;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL_MASK, sum, o);
+      if (lane == 0) prefix[k + 1] = sum * g.kv.n_kv;
+    }
+    if (threadIdx.x == 0) prefix[0] = 0;
+    __syncthreads();
+    if (warp == 0) {   // inclusive prefix sums: a lane's share, then the lanes before it
+      const int per = (n_seq + 31) / 32, b = lane * per, e = min(b + per, n_seq);
+      int64_t sum = 0;
+      for (int k = b; k < e; ++k) sum += prefix[k + 1];
+      int64_t before = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(FULL_MASK, before, o);
+        if (lane >= o) before += v;
+      }
+      before -= sum;
+      for (int k = b; k < e; ++k) {
+        before += prefix[k + 1];
+        prefix[k + 1] = before;
+      }
+    }
+    __syncthreads();
+    const int64_t total = prefix[n_seq];
+    run = max((total + g.nc - 1) / g.nc, static_cast<int64_t>(g.min_run));
+    at = min(run * cta, total);
+    end = min(at + run, total);
+    if (at >= end) return;
+    int lo = 0, hi = n_seq - 1;   // the last sequence that begins at or before `at`
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (prefix[mid] <= at) lo = mid;
+      else hi = mid - 1;
+    }
+    s = lo;
+    q = attn_seq(g, s, false);
+    const int64_t per_head = (prefix[s + 1] - prefix[s]) / g.kv.n_kv;
+    int64_t r = at - prefix[s];
+    head = static_cast<int>(r / per_head);
+    r -= head * per_head;
+    for (int base = 0;; base += 32) {   // the q tile, 32 at a time
+      const int nt = (base + lane) * static_cast<int64_t>(g.tpi) < q.nq ? attn_span<N>(g, q, base + lane).nt : 0;
+      int64_t sum = nt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(FULL_MASK, sum, o);
+        if (lane >= o) sum += v;
+      }
+      const unsigned hit = __ballot_sync(FULL_MASK, sum > r);
+      if (hit || base * static_cast<int64_t>(g.tpi) >= q.nq) {
+        const int l = hit ? __ffs(hit) - 1 : 0;
+        qt = base + l;
+        i0 = static_cast<int>(r - __shfl_sync(FULL_MASK, sum - nt, l));
+        break;
+      }
+      r -= __shfl_sync(FULL_MASK, sum, 31);
+    }
+  }
+  // The next item's tiles that are this CTA's; false at the end of the run.
+  CLB_DEV bool more() const { return at < end; }
+  CLB_DEV int tiles(const AttnSpan &p) const { return static_cast<int>(min(static_cast<int64_t>(p.nt - i0), end - at)); }
+  CLB_DEV void advance(const AttnArgs &g, int n) {
+    at += n;
+    i0 = 0;
+    if (at >= end) return;
+    if (++qt * g.tpi < q.nq) return;
+    qt = 0;
+    if (++head < g.kv.n_kv) return;
+    head = 0;
+    do {
+      q = attn_seq(g, ++s, false);
+    } while (q.nq == 0 && s + 1 < g.kv.n_seq);
+  }
+  // For an item that begins in this CTA's run and leaves `rest` tiles: how many CTAs hold them.
+  CLB_DEV int pieces(int rest) const { return static_cast<int>((rest + run - 1) / run); }
+};
+
+CLB_DEV float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+
+// Host: the tensor-core kernel of attn_tc.cu; what it needs of the workspace.
+constexpr int ATTN_TC_ROWS = 256;
+int launch_attn_tc(const AttnArgs &g, cudaStream_t st);
+
+}  // namespace clb

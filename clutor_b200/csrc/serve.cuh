@@ -30,6 +30,19 @@ CLB_DEV __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <>
 CLB_DEV __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Four floats times f, rounded to O (16 or 8 bytes, aligned).
+template <typename O>
+CLB_DEV void store4(O *p, float4 v, float f) {
+  if constexpr (sizeof(O) == 4) {
+    *reinterpret_cast<float4 *>(p) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+  } else {
+    uint2 w;
+    O *h = reinterpret_cast<O *>(&w);
+    h[0] = from_f32<O>(v.x * f); h[1] = from_f32<O>(v.y * f); h[2] = from_f32<O>(v.z * f); h[3] = from_f32<O>(v.w * f);
+    *reinterpret_cast<uint2 *>(p) = w;
+  }
+}
+
 // The last s in [0, n_seq) with q_start[s] <= row, by bisection: the sequence whose rows hold `row` when q_start does not
 // descend and q_start[0] <= row < q_start[n_seq] (sequences without rows are passed over). Reads inside q_start whatever it
 // holds.
