@@ -273,16 +273,17 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
 
 constexpr int JT = 128, JW = JT / 32;
 
-// A CTA per row, its warps taking every JW-th piece: the largest of the pieces' maxima first, then their values scaled to it;
-// the warps' sums are added in warp order.
-template <typename O, int HD>
+// The largest of the pieces' maxima first, then their values scaled to it. BY_ROW: a warp per row, the pieces in run order (many
+// rows in few pieces). Else a CTA per row, its warps taking every JW-th piece and their sums added in warp order (few rows in
+// many pieces).
+template <typename O, int HD, bool BY_ROW>
 __global__ void __launch_bounds__(JT) attn_join_kernel(const AttnArgs g) {
   constexpr int EPL = HD / 32;
   __shared__ float sum[JW][HD], den[JW];
   grid_dependency_wait();
   const int4 j = g.joins[blockIdx.x];
   if (j.w == 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.y;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = BY_ROW ? blockIdx.y * JW + warp : blockIdx.y;
   const AttnSeq q = attn_seq(g, j.x, false);
   const int t = j.z * g.tpi + r / g.group;
   if (r >= g.tpi * g.group || t >= q.nq) return;
@@ -296,13 +297,20 @@ __global__ void __launch_bounds__(JT) attn_join_kernel(const AttnArgs g) {
 #pragma unroll
   for (int e = 0; e < EPL; ++e) v[e] = 0.f;
 #pragma unroll 4
-  for (int i = warp; i <= j.w; i += JW) {
+  for (int i = BY_ROW ? 0 : warp; i <= j.w; i += BY_ROW ? 1 : JW) {
     const float2 ml = g.piece_ml[slot(i)];
     const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - mm);
     const float *src = g.piece_o + slot(i) * HD;
     l = fmaf(f, ml.y, l);
 #pragma unroll
     for (int e = 0; e < EPL; ++e) v[e] = fmaf(f, src[lane + 32 * e], v[e]);
+  }
+  O *dst = static_cast<O *>(g.a.out) + (q.row + t) * g.a.out_stride + (j.y * g.group + r % g.group) * HD;
+  if constexpr (BY_ROW) {
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) dst[lane + 32 * e] = from_f32<O>(v[e] * inv);
+    return;
   }
 #pragma unroll
   for (int e = 0; e < EPL; ++e) sum[warp][lane + 32 * e] = v[e];
@@ -311,7 +319,6 @@ __global__ void __launch_bounds__(JT) attn_join_kernel(const AttnArgs g) {
   l = 0.f;
   for (int w = 0; w < JW; ++w) l += den[w];
   const float inv = l > 0.f ? 1.0f / l : 0.f;
-  O *dst = static_cast<O *>(g.a.out) + (q.row + t) * g.a.out_stride + (j.y * g.group + r % g.group) * HD;
   for (int d = threadIdx.x; d < HD; d += JT) {
     float o = 0.f;
     for (int w = 0; w < JW; ++w) o += sum[w][d];
@@ -320,16 +327,6 @@ __global__ void __launch_bounds__(JT) attn_join_kernel(const AttnArgs g) {
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
-
-template <typename F>
-cudaError_t allow_smem(F *fn, int bytes, bool (&done)[64]) {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 64 && done[dev]) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev < 64) done[dev] = true;
-  return e;
-}
 
 template <typename C, typename O, int HD, int MT>
 cudaError_t launch_rows(const AttnArgs &g, cudaStream_t st) {
@@ -344,7 +341,8 @@ cudaError_t launch_rows(const AttnArgs &g, cudaStream_t st) {
 template <typename O, int HD>
 cudaError_t launch_join(const AttnArgs &g, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(g.nc, g.tpi * g.group);
+  const bool by_row = g.rows > 32;
+  cfg.gridDim = dim3(g.nc, by_row ? (g.tpi * g.group + JW - 1) / JW : g.tpi * g.group);
   cfg.blockDim = dim3(JT);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -352,13 +350,14 @@ cudaError_t launch_join(const AttnArgs &g, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attn_join_kernel<O, HD>, g);
+  return by_row ? cudaLaunchKernelEx(&cfg, attn_join_kernel<O, HD, true>, g) : cudaLaunchKernelEx(&cfg, attn_join_kernel<O, HD, false>, g);
 }
 
 template <typename C, typename O, int HD>
 cudaError_t launch_all(const AttnArgs &g, cudaStream_t st) {
   cudaError_t e;
-  if (g.rows == 16) e = launch_rows<C, O, HD, 1>(g, st);
+  if (g.rows > 32) e = launch_attn_tc(g, st);
+  else if (g.rows == 16) e = launch_rows<C, O, HD, 1>(g, st);
   else if constexpr (HD <= 128) e = launch_rows<C, O, HD, 2>(g, st);
   else e = cudaErrorInvalidValue;
   return e != cudaSuccess ? e : launch_join<O, HD>(g, st);
@@ -375,14 +374,16 @@ cudaError_t launch_hd(const AttnArgs &g, cudaStream_t st) {
 
 // The kernel's shape for a call, and its workspace: partial values, their maxima and sums, the list of items to join.
 struct AttnPlan {
-  int rows, nc;
+  int rows, tpi, nc;
   size_t off_ml, off_joins, total;
 };
 AttnPlan attn_plan(int sms, const clb200_kv &kv, const clb200_attn &a) {
   AttnPlan p{};
   const int group = a.n_head / kv.n_kv;
-  p.rows = a.max_q * static_cast<int64_t>(group) <= 16 || kv.head_dim == 256 ? 16 : 32;
-  p.nc = sms * (kv.head_dim == 256 ? 1 : 2);
+  const int64_t need = a.max_q * static_cast<int64_t>(group);
+  p.rows = need <= 16 ? 16 : need <= 32 && kv.head_dim <= 128 ? 32 : attn_tc_rows(kv.head_dim);
+  p.nc = sms * (p.rows <= 32 && kv.head_dim <= 128 ? 2 : 1);
+  p.tpi = p.rows <= 32 ? p.rows / group : p.rows / 128 * (128 / group);
   const size_t pieces = static_cast<size_t>(p.nc) * 2 * p.rows;
   p.off_ml = al(pieces * kv.head_dim * 4);
   p.off_joins = p.off_ml + al(pieces * 8);
@@ -454,9 +455,9 @@ extern "C" int clb200_attention(clb200_ctx *c, const clb200_kv *kv, const clb200
     g.err = c->small;
     g.group = a->n_head / kv->n_kv;
     g.rows = p.rows;
-    g.tpi = p.rows / g.group;
+    g.tpi = p.tpi;
     g.nc = p.nc;
-    g.min_run = 4;
+    g.min_run = p.rows <= 32 ? 4 : 2;
     g.piece_o = reinterpret_cast<float *>(w);
     g.piece_ml = reinterpret_cast<float2 *>(w + p.off_ml);
     g.joins = reinterpret_cast<int4 *>(w + p.off_joins);

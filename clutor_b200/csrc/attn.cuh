@@ -178,8 +178,19 @@ CLB_DEV float exp2_approx(float x) {
 }
 constexpr float LOG2E = 1.4426950408889634f;
 
-// Host: the tensor-core kernel of attn_tc.cu; what it needs of the workspace.
-constexpr int ATTN_TC_ROWS = 256;
-int launch_attn_tc(const AttnArgs &g, cudaStream_t st);
+// Host: the tcgen05 kernel of attn_tc.cu on an argument block whose rows, tpi and nc are its own (attn_tc_rows(head_dim) rows).
+cudaError_t launch_attn_tc(const AttnArgs &g, cudaStream_t st);
+constexpr int attn_tc_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }
+
+// Host: raises a kernel's shared-memory limit once per device.
+template <typename F>
+cudaError_t allow_smem(F *fn, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 64 && done[dev]) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done[dev] = true;
+  return e;
+}
 
 }  // namespace clb
