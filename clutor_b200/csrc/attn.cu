@@ -23,12 +23,6 @@ struct RowsShape {
   static_assert(RW * ROWS * HD * 4 <= static_cast<int>(KV), "the joined states fit the stages");
 };
 
-CLB_DEV void cp_async16(uint32_t dst, const void *src, bool take) {   // 16 bytes, or zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
-}
-CLB_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int K>
-CLB_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(K) : "memory"); }
 CLB_DEV void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -73,6 +67,7 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
   const float sc = a.scale * LOG2E;
   const int gr = lane >> 2, gc = (lane & 3) * 2;   // the lane's row and first column in an accumulator
   if (tid == 0) g.joins[cta] = make_int4(0, 0, 0, 0);
+  attn_prefix<RN>(g, prefix, cta);
   AttnRun<RN> run;
   run.init(g, prefix, cta);
   while (run.more()) {
@@ -82,7 +77,7 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
     const bool whole = n == span.nt;
     __syncthreads();   // the last item's queries and joined states have been read
     for (int i = tid; i < ROWS * (HD / 8); i += RT) {
-      const int r = i / (HD / 8), c = i % (HD / 8), t = t0 + r / g.group, h = head * g.group + r % g.group;
+      const int r = i / (HD / 8), c = i % (HD / 8), tr = attn_token(g, r), t = t0 + tr, h = head * g.group + r - tr * g.group;
       const bool live = r < g.tpi * g.group && t < q.nq;
       const C *src = static_cast<const C *>(a.q) + (live ? (q.row + t) * a.q_stride + h * HD + 8 * c : 0);
       cp_async16(q_sm + chunk_at<HD>(r, c), src, live);
@@ -93,8 +88,9 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
       if (i < n) {
         const int j0 = span.tile(i0 + i) * RN + warp * 16;
         if (j0 <= span.hi) {
-          const int page = page_of(kv, s, j0, g.err);
-          const int64_t base = (page < 0 ? 0 : page * kv.page_stride + (j0 % kv.page_size) * kv.slot_stride) + head * kv.head_stride;
+          const AttnSlot at0 = attn_slot(g, s, j0);
+          const int page = at0.page;
+          const int64_t base = (page < 0 ? 0 : page * kv.page_stride + at0.slot * kv.slot_stride) + head * kv.head_stride;
           const uint32_t dst = kv_sm + (i % S::STAGES) * S::STAGE;
           const int left = page < 0 ? 0 : q.kv - j0;   // positions behind the sequence's end come as zeros
 #pragma unroll
@@ -170,7 +166,7 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const int r = 16 * mt + gr + ((e & 2) ? 8 : 0), j = j0 + (e >> 2) * 8 + gc + (e & 1);
-              if (!attn_sees(g, span.lo + r / g.group, j)) x[mt][e >> 2][e & 3] = -INFINITY;
+              if (!attn_sees(g, span.lo + attn_token(g, r), j)) x[mt][e >> 2][e & 3] = -INFINITY;
             }
           }
           float mx[2] = {m[mt][0], m[mt][1]};
@@ -243,7 +239,7 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
     __syncthreads();
     const int slot = 2 * cta + (i0 == 0 ? 1 : 0);
     for (int i = tid; i < ROWS * (HD / 4); i += RT) {
-      const int r = i / (HD / 4), c = 4 * (i % (HD / 4)), t = t0 + r / g.group;
+      const int r = i / (HD / 4), c = 4 * (i % (HD / 4)), tr = attn_token(g, r), t = t0 + tr;
       if (r >= g.tpi * g.group || t >= q.nq) continue;
       float mm = -INFINITY, ll = 0.f;
 #pragma unroll
@@ -258,7 +254,7 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
       }
       if (whole) {
         const float inv = ll > 0.f ? 1.0f / ll : 0.f;
-        store4<O>(static_cast<O *>(a.out) + (q.row + t) * a.out_stride + (head * g.group + r % g.group) * HD + c, v, inv);
+        store4<O>(static_cast<O *>(a.out) + (q.row + t) * a.out_stride + (head * g.group + r - tr * g.group) * HD + c, v, inv);
       } else {
         *reinterpret_cast<float4 *>(g.piece_o + (static_cast<int64_t>(slot) * g.rows + r) * HD + c) = v;
         if (c == 0) g.piece_ml[static_cast<int64_t>(slot) * g.rows + r] = make_float2(mm, ll);
@@ -454,6 +450,8 @@ extern "C" int clb200_attention(clb200_ctx *c, const clb200_kv *kv, const clb200
     g.a.sinks = std::min(a->sinks, 1 << 30);
     g.err = c->small;
     g.group = a->n_head / kv->n_kv;
+    g.group_inv = (65536u + g.group - 1) / g.group;
+    g.page_shift = (kv->page_size & (kv->page_size - 1)) ? -1 : __builtin_ctz(kv->page_size);
     g.rows = p.rows;
     g.tpi = p.tpi;
     g.nc = p.nc;

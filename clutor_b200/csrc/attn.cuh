@@ -20,6 +20,8 @@ struct AttnArgs {
   clb200_attn a;
   int *err;
   int group, tpi;     // query heads per key/value head, new tokens per item
+  uint32_t group_inv; // (65536 + group - 1) / group: row / group = row * group_inv >> 16 for rows below 4096
+  int page_shift;     // log2 of the page size where it is a power of two, else -1
   int nc, min_run;    // CTAs, tiles a CTA takes at least
   int rows;           // rows of a piece (>= tpi x group)
   float *piece_o;     // [nc][2][rows][head_dim]
@@ -73,13 +75,65 @@ CLB_DEV AttnSpan attn_span(const AttnArgs &g, const AttnSeq &q, int qt) {
   }
   return p;
 }
+CLB_DEV int attn_token(const AttnArgs &g, int row) { return static_cast<int>((static_cast<uint32_t>(row) * g.group_inv) >> 16); }
+
+// The page and slot of position pos (>= 0) of sequence s; page -1 (and the error word set) when there is none.
+struct AttnSlot {
+  int page, slot;
+};
+CLB_DEV AttnSlot attn_slot(const AttnArgs &g, int s, int pos) {
+  const clb200_kv &kv = g.kv;
+  const int i = g.page_shift >= 0 ? pos >> g.page_shift : static_cast<int>(static_cast<uint32_t>(pos) / static_cast<uint32_t>(kv.page_size));
+  AttnSlot r{-1, pos - i * kv.page_size};
+  if (i < kv.table_width) r.page = __ldg(kv.table + static_cast<int64_t>(s) * kv.table_stride + i);
+  if (r.page < 0 || r.page >= kv.n_pages) {
+    set_error(g.err, ERR_BAD_PAGE);
+    r.page = -1;
+  }
+  return r;
+}
+
 // Whether row position p sees position j (j below the sequence's length).
 CLB_DEV bool attn_sees(const AttnArgs &g, int p, int j) {
   return j <= p && (g.a.window <= 0 || j > p - g.a.window || j < g.a.sinks);
 }
 
-// A CTA's run of tiles. Every thread of the CTA makes the same one (init synchronises the CTA; `prefix` is shared memory of
-// ATTN_MAX_SEQ + 1 words).
+// The tiles of the sequences before each sequence (prefix [n_seq + 1], shared memory). Every thread of the CTA calls it; it
+// synchronises the CTA.
+template <int N>
+CLB_DEV void attn_prefix(const AttnArgs &g, int64_t *prefix, int cta) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5, n_seq = g.kv.n_seq;
+  for (int k = warp; k < n_seq; k += nw) {
+    const AttnSeq t = attn_seq(g, k, cta == 0 && lane == 0);
+    const int nqt = (t.nq + g.tpi - 1) / g.tpi;
+    int64_t sum = 0;
+    for (int i = lane; i < nqt; i += 32) sum += attn_span<N>(g, t, i).nt;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL_MASK, sum, o);
+    if (lane == 0) prefix[k + 1] = sum * g.kv.n_kv;
+  }
+  if (threadIdx.x == 0) prefix[0] = 0;
+  __syncthreads();
+  if (warp == 0) {   // inclusive prefix sums: a lane's share, then the lanes before it
+    const int per = (n_seq + 31) / 32, b = lane * per, e = min(b + per, n_seq);
+    int64_t sum = 0;
+    for (int k = b; k < e; ++k) sum += prefix[k + 1];
+    int64_t before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(FULL_MASK, before, o);
+      if (lane >= o) before += v;
+    }
+    before -= sum;
+    for (int k = b; k < e; ++k) {
+      before += prefix[k + 1];
+      prefix[k + 1] = before;
+    }
+  }
+  __syncthreads();
+}
+
+// A CTA's run of tiles, walked by whole warps (every lane holds the same state).
 template <int N>
 struct AttnRun {
   int64_t at, end;        // tiles of all items: the next, and the first that is another CTA's
@@ -87,36 +141,8 @@ struct AttnRun {
   int s, head, qt, i0;    // the next item, and its first tile that is this CTA's
   AttnSeq q;
 
-  CLB_DEV void init(const AttnArgs &g, int64_t *prefix, int cta) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5, n_seq = g.kv.n_seq;
-    for (int k = warp; k < n_seq; k += nw) {
-      const AttnSeq t = attn_seq(g, k, cta == 0 && lane == 0);
-      const int nqt = (t.nq + g.tpi - 1) / g.tpi;
-      int64_t sum = 0;
-      for (int i = lane; i < nqt; i += 32) sum += attn_span<N>(g, t, i).nt;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL_MASK, sum, o);
-      if (lane == 0) prefix[k + 1] = sum * g.kv.n_kv;
-    }
-    if (threadIdx.x == 0) prefix[0] = 0;
-    __syncthreads();
-    if (warp == 0) {   // inclusive prefix sums: a lane's share, then the lanes before it
-      const int per = (n_seq + 31) / 32, b = lane * per, e = min(b + per, n_seq);
-      int64_t sum = 0;
-      for (int k = b; k < e; ++k) sum += prefix[k + 1];
-      int64_t before = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(FULL_MASK, before, o);
-        if (lane >= o) before += v;
-      }
-      before -= sum;
-      for (int k = b; k < e; ++k) {
-        before += prefix[k + 1];
-        prefix[k + 1] = before;
-      }
-    }
-    __syncthreads();
+  CLB_DEV void init(const AttnArgs &g, const int64_t *prefix, int cta) {
+    const int lane = threadIdx.x & 31, n_seq = g.kv.n_seq;
     const int64_t total = prefix[n_seq];
     run = max((total + g.nc - 1) / g.nc, static_cast<int64_t>(g.min_run));
     at = min(run * cta, total);
@@ -171,6 +197,18 @@ struct AttnRun {
   CLB_DEV int pieces(int rest) const { return static_cast<int>((rest + run - 1) / run); }
 };
 
+CLB_DEV void cp_async16(uint32_t dst, const void *src, bool take) {   // 16 bytes, or zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+CLB_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int K>
+CLB_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(K) : "memory"); }
+
+CLB_DEV float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 CLB_DEV float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -2,13 +2,16 @@
 //
 // An item's rows (new tokens x the group's query heads) fill up to two tiles of 128 rows, the streams; both use every key and
 // value tile of N positions that is loaded. A CTA per SM walks its run of tiles (attn.cuh) with
-//   warps of softmax group w (128 threads, a row each): load the stream's queries into shared memory; per tile read their row
-//           of the scores S_w from TMEM, mask, take the exponentials against the row's running maximum, keep its sum, and
-//           write the probabilities back over S_w as the operand P_w; at the end of the item read O_w and store it;
-//   one warp (TMA): the item's key and value tiles through a ring of stages, a box per page piece; positions at or past the
+//   softmax group w (128 threads, a row each): per tile read their row of the scores S_w from TMEM, mask, take the exponentials
+//           against the row's running maximum, keep its sum, and write the probabilities back over S_w as the operand P_w; at
+//           the end of the item read O_w and store it;
+//   items   (one warp): walks the run and puts each item's numbers into shared memory for the others;
+//   queries (one warp): a stream's queries by TMA (a box of tokens x the group's heads x 64 elements is 128-byte-swizzled rows
+//           in order) once the item before has no product left that reads them;
+//   keys    (one warp): the item's key and value tiles through a ring of stages, a box per page piece; positions at or past the
 //           sequence's end come from outside the tensor, as zeros, except inside the last box;
-//   one warp (MMA): S_w = Q_w K^T (both operands in shared memory), O_w += P_w V (P_w from TMEM). While group 0 works on its
-//           scores the tensor cores run the other stream's products.
+//   MMA     (one warp): S_w = Q_w K^T (both operands in shared memory), O_w += P_w V (P_w from TMEM). While group 0 works on
+//           its scores the tensor cores run the other stream's products.
 // The maximum that scales a row's sums is only moved when the row's maximum has grown by more than 2^8 (the probabilities then
 // reach 2^8 at most, far inside fp16 and fp32), so rescaling O_w, a round trip through the registers, is rare.
 // The values of positions past the sequence's end inside the last box may be anything, and 0 x NaN is NaN: the MMA warp zeroes
@@ -32,7 +35,7 @@ struct TcAttn {
   static constexpr int THREADS = 128 * (STREAMS + 1);
   static constexpr uint32_t Q_TILE = 128 * HD * 2, STAGE = N * HD * 2;
   static constexpr int STAGES = HD == 64 ? 10 : 5;
-  static constexpr int N_BARS = 2 * STAGES + 4 * STREAMS + 1;
+  static constexpr int N_BARS = 2 * STAGES + 6 * STREAMS + 2 * 4 + 1;
   static constexpr uint32_t SMEM = 1024 + STREAMS * Q_TILE + STAGES * STAGE + 8 * N_BARS + 16;
   static constexpr uint32_t S_COL = 0, O_COL = 256;          // S_w at 128 w (P_w over its first half), O_w at 256 + HD w
   static_assert(SMEM <= 232448, "shared memory budget");
@@ -42,6 +45,14 @@ struct TcAttn {
 CLB_DEV void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(dst)),
                "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
+               : "memory");
+}
+
+CLB_DEV uint32_t upto(int i) { return i < 0 ? 0u : i >= 31 ? ~0u : (2u << i) - 1u; }   // bits 0 .. i
+
+CLB_DEV void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_addr(dst)),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
                : "memory");
 }
 
@@ -56,29 +67,51 @@ CLB_DEV uint32_t pack_pair(float a, float b) {   // a in the low half
   }
 }
 
+// What the roles need to know of an item; n 0: the run has ended.
+struct __align__(16) TcItem {
+  int n, i0, sinks, start;     // this CTA's tiles [i0, i0 + n) of the item; tile i is i below sinks, else start + i
+  int s, head, kv, row;        // sequence, key/value head, length, first token's row
+  int tokens, lo, hi, whole;   // tokens, positions of the first and last, whether all of its tiles are here
+  int qt, pieces, pad[2];      // q tile, CTAs that hold the rest of an item that begins here
+  CLB_DEV int tile(int i) const { return i0 + i + (i0 + i < sinks ? 0 : start); }
+};
+constexpr int ITEMS = 4;       // items in shared memory at once
+
 template <typename C, typename O, int HD>
 __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
-    attn_tc_kernel(const AttnArgs g, const int box, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    attn_tc_kernel(const AttnArgs g, const int box, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v) {
   using S = TcAttn<HD>;
   constexpr int N = S::N, ST = S::STREAMS;
   constexpr bool BF16 = __is_same(C, __nv_bfloat16);
   extern __shared__ uint8_t raw[];
+  __shared__ TcItem items[ITEMS];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t *ring = sm + ST * S::Q_TILE;
   uint64_t *kv_full = reinterpret_cast<uint64_t *>(ring + S::STAGES * S::STAGE), *kv_free = kv_full + S::STAGES;
-  uint64_t *q_full = kv_free + S::STAGES, *s_full = q_full + ST, *p_full = s_full + ST, *o_full = p_full + ST, *mma_done = o_full + ST;
+  uint64_t *q_full = kv_free + S::STAGES, *q_free = q_full + ST, *s_full = q_free + ST, *p_half = s_full + ST, *o_full = p_half + 2 * ST;
+  uint64_t *item_full = o_full + ST, *item_free = item_full + ITEMS, *mma_done = item_free + ITEMS;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
   const clb200_attn &a = g.a;
-  const clb200_kv &kv = g.kv;
   const int tps = 128 / g.group;   // new tokens per stream
 
+  int64_t *prefix = reinterpret_cast<int64_t *>(ring);
+  attn_prefix<N>(g, prefix, cta);
   AttnRun<N> run;
-  run.init(g, reinterpret_cast<int64_t *>(ring), cta);
+  if (warp == 4 * ST + 2) run.init(g, prefix, cta);
   if (tid == 0) {
     g.joins[cta] = make_int4(0, 0, 0, 0);
     for (int i = 0; i < S::STAGES; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_free[i], 1); }
-    for (int w = 0; w < ST; ++w) { mbar_init(&q_full[w], 4); mbar_init(&s_full[w], 1); mbar_init(&p_full[w], 4); mbar_init(&o_full[w], 1); }
+    for (int w = 0; w < ST; ++w) {
+      mbar_init(&q_full[w], 1);
+      mbar_init(&q_free[w], 1);
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_half[2 * w], 4);
+      mbar_init(&p_half[2 * w + 1], 4);
+      mbar_init(&o_full[w], 1);
+    }
+    for (int i = 0; i < ITEMS; ++i) { mbar_init(&item_full[i], 1); mbar_init(&item_free[i], 4 * ST + 3); }   // warps that read items
     mbar_init(mma_done, 1);
     fence_barrier_init();
   }
@@ -89,78 +122,135 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
+  uint32_t it = 0;   // items taken
+  // The next item, by a whole warp; n 0 at the end of the run, and when the wait runs out (ok false).
+  auto next_item = [&](TcItem &x) {
+    const uint32_t k = it % ITEMS;
+    if (!mbar_wait_bounded(&item_full[k], (it / ITEMS) & 1)) { ok = false; x.n = 0; return; }
+    x = items[k];
+    ++it;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_free[k]);
+  };
 
   if (warp >= 4 * ST) {
     if constexpr (ST == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 4 * ST) {   // ---- TMA
+    if (warp == 4 * ST + 2) {   // ---- items
+      for (;; ++it) {
+        const uint32_t k = it % ITEMS;
+        if (it >= ITEMS && !mbar_wait_bounded(&item_free[k], (it / ITEMS - 1) & 1)) { ok = false; break; }
+        TcItem x{};
+        if (run.more()) {
+          const AttnSpan p = attn_span<N>(g, run.q, run.qt);
+          x.n = run.tiles(p);
+          x.i0 = run.i0; x.sinks = p.sinks; x.start = p.start;
+          x.s = run.s; x.head = run.head; x.kv = run.q.kv; x.row = run.q.row + run.qt * g.tpi;
+          x.tokens = min(g.tpi, run.q.nq - run.qt * g.tpi); x.lo = p.lo; x.hi = p.hi; x.whole = x.n == p.nt;
+          x.qt = run.qt; x.pieces = run.i0 == 0 && !x.whole ? run.pieces(p.nt - x.n) : 0;
+          run.advance(g, x.n);
+        }
+        if (lane == 0) {
+          items[k] = x;
+          mbar_arrive(&item_full[k]);
+        }
+        if (x.n == 0) break;
+      }
+    } else if (warp == 4 * ST + 3) {   // ---- queries
+      TcItem x;
+      uint32_t q_cnt[2] = {0, 0};
+      for (next_item(x); ok && x.n; next_item(x)) {
+#pragma unroll
+        for (int w = 0; w < ST; ++w) {
+          if (x.tokens <= w * tps) continue;
+          if (q_cnt[w] && !mbar_wait_bounded(&q_free[w], (q_cnt[w] - 1) & 1)) { ok = false; break; }
+          ++q_cnt[w];
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&q_full[w], static_cast<uint32_t>(tps * g.group) * HD * 2);
+#pragma unroll
+            for (int cb = 0; cb < HD / 64; ++cb) tma_load_3d(sm + w * S::Q_TILE + cb * (128 * 128), &map_q, 64 * cb, x.head * g.group, x.row + w * tps, &q_full[w]);
+          }
+          __syncwarp();
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < ST; ++w)   // every copy issued has landed before the CTA exits
+        if (q_cnt[w] && !mbar_wait_bounded(&q_full[w], (q_cnt[w] - 1) & 1)) ok = false;
+    } else if (warp == 4 * ST) {   // ---- keys and values
       uint32_t cnt = 0;
       const int boxes = N / box;
-      auto load = [&](const CUtensorMap &map, const AttnSeq &q, int s, int head, int tile) -> bool {
+      const AttnSlot outside{g.kv.n_pages, 0};   // a page past the tensor: zeros
+      TcItem x{};
+      auto where = [&](int tile) {   // this lane's box of a tile
+        const int pos = tile * N + lane * box;
+        if (lane >= boxes || pos >= x.kv) return outside;
+        const AttnSlot at = attn_slot(g, x.s, pos);
+        return at.page < 0 ? outside : at;
+      };
+      auto load = [&](const CUtensorMap &map, const AttnSlot &at) -> bool {
         const uint32_t st = cnt % S::STAGES;
         if (cnt >= S::STAGES && !mbar_wait_bounded(&kv_free[st], (cnt / S::STAGES - 1) & 1)) return false;
         if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], S::STAGE);
         __syncwarp();
         if (lane < boxes) {
-          const int pos = tile * N + lane * box;
-          int page = kv.n_pages, slot = 0;   // outside the tensor: zeros
-          if (pos < q.kv) {
-            page = page_of(kv, s, pos, g.err);
-            if (page < 0) page = kv.n_pages;
-            slot = pos % kv.page_size;
-          }
           uint8_t *dst = ring + st * S::STAGE + lane * box * 128;
 #pragma unroll
-          for (int cb = 0; cb < HD / 64; ++cb) tma_load_4d(dst + cb * N * 128, &map, 64 * cb, head, slot, page, &kv_full[st]);
+          for (int cb = 0; cb < HD / 64; ++cb) tma_load_4d(dst + cb * N * 128, &map, 64 * cb, x.head, at.slot, at.page, &kv_full[st]);
         }
         ++cnt;
         return true;
       };
-      while (ok && run.more()) {
-        const AttnSpan span = attn_span<N>(g, run.q, run.qt);
-        const int n = run.tiles(span), i0 = run.i0;
-        ok = load(map_k, run.q, run.s, run.head, span.tile(i0));
-        for (int j = 0; ok && j < n; ++j) {
-          if (j + 1 < n) ok = load(map_k, run.q, run.s, run.head, span.tile(i0 + j + 1));
-          if (ok) ok = load(map_v, run.q, run.s, run.head, span.tile(i0 + j));
+      for (next_item(x); ok && x.n; next_item(x)) {   // in the order the products take them; pages are looked up two tiles ahead
+        AttnSlot at = where(x.tile(0)), next = x.n > 1 ? where(x.tile(1)) : outside;
+        ok = load(map_k, at);
+        for (int j = 0; ok && j < x.n; ++j) {
+          const AttnSlot ahead = j + 2 < x.n ? where(x.tile(j + 2)) : outside;
+          if (j + 1 < x.n) ok = load(map_k, next);
+          if (ok) ok = load(map_v, at);
+          at = next;
+          next = ahead;
         }
-        run.advance(g, n);
+        if (!ok) break;
       }
       // every copy issued has landed before the CTA exits (already so unless a wait gave up)
       for (uint32_t v = cnt > S::STAGES ? cnt - S::STAGES : 0; v < cnt; ++v)
         if (!mbar_wait_bounded(&kv_full[v % S::STAGES], (v / S::STAGES) & 1)) ok = false;
-    } else if (warp == 4 * ST + 1) {   // ---- MMA
+    } else {   // ---- MMA
       constexpr uint32_t ID_S = tc::idesc_half(BF16, false, 128, N), ID_O = tc::idesc_half(BF16, true, 128, HD);
-      uint32_t cnt = 0, items[ST] = {}, tiles[ST] = {};   // stages, items and tiles consumed
-      auto scores = [&](int w, uint32_t st) {             // S_w = Q_w K^T; lane 0
+      uint32_t cnt = 0, q_cnt[2] = {0, 0}, p_cnt[2] = {0, 0};   // stages, items and tiles consumed
+      auto scores = [&](int w, uint32_t st) {                   // S_w = Q_w K^T; lane 0
         const uint64_t qd = tc::sw128_desc(smem_addr(sm + w * S::Q_TILE)), kd = tc::sw128_desc(smem_addr(ring + st * S::STAGE));
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
           tc::mma_f16(tmem + S::S_COL + 128 * w, qd + (kk / 4) * (128 * 128 / 16) + 2 * (kk % 4), kd + (kk / 4) * (N * 128 / 16) + 2 * (kk % 4), ID_S, kk != 0);
         tc::commit(&s_full[w]);
       };
-      while (ok && run.more()) {
-        const AttnSeq q = run.q;
-        const AttnSpan span = attn_span<N>(g, q, run.qt);
-        const int n = run.tiles(span), i0 = run.i0;
-        const int live = ST == 2 && q.nq - run.qt * g.tpi > tps ? 2 : 1;   // streams that have rows
-        const uint32_t k0 = cnt++ % S::STAGES;
-        if (!mbar_wait_bounded(&kv_full[k0], ((cnt - 1) / S::STAGES) & 1)) { ok = false; break; }
-        for (int w = 0; ok && w < live; ++w) {
-          if (!mbar_wait_bounded(&q_full[w], items[w]++ & 1)) ok = false;
-          tc::fence_after_sync();
-          if (ok && lane == 0) scores(w, k0);
+      auto stage = [&](uint32_t &st) {   // the next stage, once it is full
+        st = cnt % S::STAGES;
+        const bool got = mbar_wait_bounded(&kv_full[st], (cnt / S::STAGES) & 1);
+        ++cnt;
+        return got;
+      };
+      TcItem x;
+      for (next_item(x); ok && x.n; next_item(x)) {
+        uint32_t ks, vs;
+        ok = stage(ks);
+#pragma unroll
+        for (int w = 0; w < ST; ++w) {
+          if (!ok || x.tokens <= w * tps) continue;
+          ok = mbar_wait_bounded(&q_full[w], q_cnt[w]++ & 1);
+          if (ok && lane == 0) {
+            scores(w, ks);
+            if (x.n == 1) tc::commit(&q_free[w]);
+          }
         }
         if (!ok) break;
-        if (lane == 0) tc::commit(&kv_free[k0]);
-        for (int j = 0; j < n; ++j) {
-          uint32_t ks = 0;
-          if (j + 1 < n) {
-            ks = cnt++ % S::STAGES;
-            if (!mbar_wait_bounded(&kv_full[ks], ((cnt - 1) / S::STAGES) & 1)) { ok = false; break; }
-          }
-          const uint32_t vs = cnt++ % S::STAGES;
-          if (!mbar_wait_bounded(&kv_full[vs], ((cnt - 1) / S::STAGES) & 1)) { ok = false; break; }
-          const int left = q.kv - span.tile(i0 + j) * N;   // rows of the tile that are the sequence's
+        if (lane == 0) tc::commit(&kv_free[ks]);
+        for (int j = 0; j < x.n; ++j) {
+          const bool more = j + 1 < x.n;
+          if (more) ok = stage(ks);
+          if (ok) ok = stage(vs);
+          if (!ok) break;
+          const int left = x.kv - x.tile(j) * N;   // rows of the tile that are the sequence's
           if (left < N) {
             for (int i = lane; i < (N - max(left, 0)) * 8 * (HD / 64); i += 32) {
               const int c = i & 7, cb = (i >> 3) % (HD / 64), r = max(left, 0) + (i >> 3) / (HD / 64);
@@ -170,24 +260,34 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
             __syncwarp();
           }
           const uint64_t vd = tc::sw128_desc_mn(smem_addr(ring + vs * S::STAGE), N * 128);
-          for (int w = 0; w < live; ++w) {
-            if (!mbar_wait_bounded(&p_full[w], tiles[w]++ & 1)) { ok = false; break; }
-            tc::fence_after_sync();
-            if (lane == 0) {
 #pragma unroll
-              for (int kk = 0; kk < N / 16; ++kk)
-                tc::mma_f16_ts(tmem + S::O_COL + HD * w, tmem + S::S_COL + 128 * w + 8 * kk, vd + 128 * kk, ID_O, j != 0 || kk != 0);
-              if (j + 1 < n) scores(w, ks);
+          for (int w = 0; w < ST; ++w) {
+            if (!ok || x.tokens <= w * tps) continue;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (ok) ok = mbar_wait_bounded(&p_half[2 * w + h], p_cnt[w] & 1);
+              tc::fence_after_sync();
+              if (ok && lane == 0) {
+#pragma unroll
+                for (int kk = 0; kk < N / 32; ++kk)
+                  tc::mma_f16_ts(tmem + S::O_COL + HD * w, tmem + S::S_COL + 128 * w + 8 * (N / 32 * h + kk), vd + 128 * (N / 32 * h + kk), ID_O,
+                                 j != 0 || h != 0 || kk != 0);
+              }
+            }
+            ++p_cnt[w];
+            if (ok && lane == 0) {
+              if (more) scores(w, ks);
               else tc::commit(&o_full[w]);
+              if (j + 2 == x.n) tc::commit(&q_free[w]);
             }
           }
           if (!ok) break;
           if (lane == 0) {
             tc::commit(&kv_free[vs]);
-            if (j + 1 < n) tc::commit(&kv_free[ks]);
+            if (more) tc::commit(&kv_free[ks]);
           }
         }
-        run.advance(g, n);
+        if (!ok) break;
       }
       if (lane == 0) {
         tc::commit(mma_done);   // the TMEM is released only after every MMA issued has completed
@@ -196,64 +296,53 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
     }
   } else {   // ---- softmax group w, a row per thread
     if constexpr (ST == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int w = warp >> 2, r = tid & 127;
+    const int w = warp >> 2, r = tid & 127, tr = attn_token(g, r);
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t s_col = tmem + lanes + S::S_COL + 128 * w, o_col = tmem + lanes + S::O_COL + HD * w;
     const float sc = a.scale * LOG2E;
-    uint8_t *qt_sm = sm + w * S::Q_TILE;
-    uint32_t items = 0, tiles = 0;
-    auto mine = [&]() { return w == 0 || run.q.nq - run.qt * g.tpi > tps; };   // whether the item has rows in this stream
-    auto load_q = [&]() {
-      const int t0 = run.qt * g.tpi + w * tps;
-      for (int i = r; i < 128 * (HD / 8); i += 128) {
-        const int row = i / (HD / 8), c = i % (HD / 8), t = t0 + row / g.group;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < tps * g.group && t < run.q.nq)
-          v = *reinterpret_cast<const uint4 *>(static_cast<const C *>(a.q) + (run.q.row + t) * a.q_stride + (run.head * g.group + row % g.group) * HD + 8 * c);
-        *reinterpret_cast<uint4 *>(qt_sm + (c >> 3) * (128 * 128) + tc::sw128_chunk(row, c & 7)) = v;
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[w]);
-    };
-    while (run.more() && !mine()) run.advance(g, run.tiles(attn_span<N>(g, run.q, run.qt)));
-    if (run.more()) load_q();
-    while (ok && run.more()) {
-      const AttnSeq q = run.q;
-      const AttnSpan span = attn_span<N>(g, q, run.qt);
-      const int n = run.tiles(span), i0 = run.i0, head = run.head, t0 = run.qt * g.tpi + w * tps, t = t0 + r / g.group;
-      const bool whole = n == span.nt, row_live = r < tps * g.group && t < q.nq;
-      const int first = span.lo + w * tps;            // position of the stream's first token
-      const int pos = first + r / g.group;
+    uint32_t o_cnt = 0, s_cnt = 0;
+    TcItem x_;
+    for (next_item(x_); ok && x_.n; next_item(x_)) {
+      const TcItem x = x_;
+      if (x.tokens <= w * tps) continue;
+      const int pos = x.lo + w * tps + tr;
       float m = -INFINITY;
       float2 l0 = make_float2(0.f, 0.f), l1 = l0;
-      for (int j = 0; j < n; ++j) {
-        if (!mbar_wait_bounded(&s_full[w], tiles++ & 1)) { ok = false; break; }
+      for (int j = 0; j < x.n; ++j) {
+        if (!mbar_wait_bounded(&s_full[w], s_cnt++ & 1)) { ok = false; break; }
         tc::fence_after_sync();
         uint32_t xr[N];
+        float *v = reinterpret_cast<float *>(xr);
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        tc::ld_x32_async(s_col, xr);
 #pragma unroll
-        for (int c = 0; c < N / 32; ++c) tc::ld_x32_async(s_col + 32 * c, xr + 32 * c);
+        for (int c = 0; c < N / 32; ++c) {   // the next columns are on their way while these are compared
+          tc::wait_ld_x32(xr + 32 * c);
+          if (c + 1 < N / 32) tc::ld_x32_async(s_col + 32 * (c + 1), xr + 32 * (c + 1));
 #pragma unroll
-        for (int c = 0; c < N / 32; ++c) tc::wait_ld_x32(xr + 32 * c);
-        float *x = reinterpret_cast<float *>(xr);
-        const int p0 = span.tile(i0 + j) * N;
-        // some row of the stream does not see the whole tile
-        if (p0 + N - 1 > first || (a.window > 0 && p0 <= span.hi - a.window && p0 + N - 1 >= a.sinks)) {
-          const int hi = pos - p0, lo = a.window > 0 ? pos - a.window - p0 : -1, sk = a.window > 0 ? a.sinks - p0 : 0;
-#pragma unroll
-          for (int i = 0; i < N; ++i)
-            if (i > hi || (i <= lo && i >= sk)) x[i] = -INFINITY;
+          for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], v[32 * c + i], v[32 * c + i + 1]);
         }
-        float mx[4] = {x[0], x[1], x[2], x[3]};
+        const int p0 = x.tile(j) * N;
+        // some row of the stream does not see the whole tile
+        if (p0 + N - 1 > x.lo + w * tps || (a.window > 0 && p0 <= x.hi - a.window && p0 + N - 1 >= a.sinks)) {
+          const int hi = pos - p0, lo = a.window > 0 ? pos - a.window - p0 : -1, sk = a.window > 0 ? a.sinks - p0 : 0;
+          mx[0] = mx[1] = mx[2] = mx[3] = -INFINITY;
 #pragma unroll
-        for (int i = 4; i < N; ++i) mx[i & 3] = fmaxf(mx[i & 3], x[i]);
+          for (int c = 0; c < N / 32; ++c) {
+            const uint32_t seen = upto(hi - 32 * c) & ~(upto(lo - 32 * c) & ~upto(sk - 1 - 32 * c));
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[32 * c + i] = seen & (1u << i) ? v[32 * c + i] : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], v[32 * c + i], v[32 * c + i + 1]);
+          }
+        }
         const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
         if (__any_sync(FULL_MASK, mn > m + 8.0f)) {   // also where m is still -infinity
           const float mb = fmaxf(m, mn), f = m == -INFINITY ? 0.f : exp2_approx(m - mb);
           m = mb;
           l0.x *= f; l0.y *= f; l1.x *= f; l1.y *= f;
           if (j > 0) {   // the products before this tile's scores are complete: O_w is at rest
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {
               uint32_t o[32];
               tc::ld_x32_async(o_col + 32 * c, o);
@@ -268,54 +357,60 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
         const float2 sc2 = make_float2(sc, sc), nz = make_float2(-z, -z);
         // the probabilities go into the product in the cache's type (its operands share a type); their sum stays fp32
 #pragma unroll
-        for (int h = 0; h < N / 64; ++h) {
-          uint32_t p[32];
+        for (int h = 0; h < 2; ++h) {   // in halves: the product starts on the first while the second is computed
+          uint32_t p[N / 4];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float2 v = ffma2(make_float2(x[64 * h + 2 * i], x[64 * h + 2 * i + 1]), sc2, nz);
-            v.x = exp2_approx(v.x);
-            v.y = exp2_approx(v.y);
-            if (i & 1) l1 = fadd2(l1, v);
-            else l0 = fadd2(l0, v);
-            p[i] = pack_pair<C>(v.x, v.y);
+          for (int i = 0; i < N / 4; ++i) {
+            float2 e = ffma2(make_float2(v[N / 2 * h + 2 * i], v[N / 2 * h + 2 * i + 1]), sc2, nz);
+            e.x = exp2_approx(e.x);
+            e.y = exp2_approx(e.y);
+            if (i & 1) l1 = fadd2(l1, e);
+            else l0 = fadd2(l0, e);
+            p[i] = pack_pair<C>(e.x, e.y);
           }
-          tc::st_x32(s_col + 32 * h, p);
+          if constexpr (N == 128) tc::st_x32(s_col + 32 * h, p);
+          else tc::st_x16(s_col + 16 * h, reinterpret_cast<const uint32_t(&)[16]>(p));
+          tc::wait_st();
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_half[2 * w + h]);
         }
-        tc::wait_st();
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[w]);
       }
       if (!ok) break;
-      if (i0 == 0 && !whole && tid == 0) g.joins[cta] = make_int4(run.s, head, run.qt, run.pieces(span.nt - n));
-      // the next item's queries: every product that reads this item's is complete (its last scores have been read)
-      run.advance(g, n);
-      while (run.more() && !mine()) run.advance(g, run.tiles(attn_span<N>(g, run.q, run.qt)));
-      if (run.more()) load_q();
-      else grid_launch_dependents();
-      if (!mbar_wait_bounded(&o_full[w], items++ & 1)) { ok = false; break; }
+      if (x.pieces && tid == 0) g.joins[cta] = make_int4(x.s, x.head, x.qt, x.pieces);
+      if (!mbar_wait_bounded(&o_full[w], o_cnt++ & 1)) { ok = false; break; }
       tc::fence_after_sync();
+      const int t = w * tps + tr;
+      const bool row_live = r < tps * g.group && t < x.tokens;
       const float l = (l0.x + l0.y) + (l1.x + l1.y), inv = l > 0.f ? 1.0f / l : 0.f;
-      const int64_t piece = static_cast<int64_t>(2 * cta + (i0 == 0 ? 1 : 0)) * g.rows + w * tps * g.group + r;
-      O *dst = static_cast<O *>(a.out) + (row_live ? (q.row + t) * a.out_stride + (head * g.group + r % g.group) * HD : 0);
+      const int64_t piece = static_cast<int64_t>(2 * cta + (x.i0 == 0 ? 1 : 0)) * g.rows + w * tps * g.group + r;
+      O *dst = static_cast<O *>(a.out) + (row_live ? (x.row + t) * a.out_stride + (x.head * g.group + r - tr * g.group) * HD : 0);
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t o[32];
         tc::ld_x32_async(o_col + 32 * c, o);
         tc::wait_ld_x32(o);
         if (!row_live) continue;
-        const float *v = reinterpret_cast<const float *>(o);
-        if (whole) {
+        const float *f = reinterpret_cast<const float *>(o);
+        if (x.whole) {
+          if constexpr (sizeof(O) == 2) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) store4<O>(dst + 32 * c + i, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]), inv);
+            for (int i = 0; i < 32; i += 8)
+              *reinterpret_cast<uint4 *>(dst + 32 * c + i) = make_uint4(pack_pair<O>(f[i] * inv, f[i + 1] * inv), pack_pair<O>(f[i + 2] * inv, f[i + 3] * inv),
+                                                                        pack_pair<O>(f[i + 4] * inv, f[i + 5] * inv), pack_pair<O>(f[i + 6] * inv, f[i + 7] * inv));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) store4<O>(dst + 32 * c + i, make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]), inv);
+          }
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(g.piece_o + piece * HD + 32 * c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(g.piece_o + piece * HD + 32 * c + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
         }
       }
-      if (!whole && row_live) g.piece_ml[piece] = make_float2(m, l);
+      if (!x.whole && row_live) g.piece_ml[piece] = make_float2(m, l);
       tc::fence_before_sync();
     }
+    grid_launch_dependents();
   }
   if (!ok) set_error(g.err, ERR_WAIT_COPY);
   tc::fence_before_sync();
@@ -352,6 +447,18 @@ bool encode_pages(CUtensorMap *m, const clb200_kv &kv, const void *base, int box
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The queries as a tensor (element, head, row): boxes of 64 elements of a group's heads by the tokens of a stream.
+bool encode_queries(CUtensorMap *m, const AttnArgs &g) {
+  const EncodeTiled fn = encoder();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(g.kv.head_dim), static_cast<cuuint64_t>(g.a.n_head), static_cast<cuuint64_t>(g.a.T)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(g.kv.head_dim) * 2, static_cast<cuuint64_t>(g.a.q_stride) * 2};
+  const cuuint32_t boxes[3] = {64, static_cast<cuuint32_t>(g.group), static_cast<cuuint32_t>(128 / g.group)}, estr[3] = {1, 1, 1};
+  return fn(m, g.kv.type == T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(g.a.q), dims, strides, boxes,
+            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename C, typename O, int HD>
 cudaError_t launch(const AttnArgs &g, cudaStream_t st) {
   using S = TcAttn<HD>;
@@ -359,9 +466,9 @@ cudaError_t launch(const AttnArgs &g, cudaStream_t st) {
   const cudaError_t e = allow_smem(attn_tc_kernel<C, O, HD>, S::SMEM, done);
   if (e != cudaSuccess) return e;
   const int box = std::gcd(g.kv.page_size, S::N);
-  CUtensorMap mk, mv;
-  if (!encode_pages(&mk, g.kv, g.kv.k, box) || !encode_pages(&mv, g.kv, g.kv.v, box)) return cudaErrorInvalidValue;
-  attn_tc_kernel<C, O, HD><<<g.nc, S::THREADS, S::SMEM, st>>>(g, box, mk, mv);
+  CUtensorMap mq, mk, mv;
+  if (!encode_queries(&mq, g) || !encode_pages(&mk, g.kv, g.kv.k, box) || !encode_pages(&mv, g.kv, g.kv.v, box)) return cudaErrorInvalidValue;
+  attn_tc_kernel<C, O, HD><<<g.nc, S::THREADS, S::SMEM, st>>>(g, box, mq, mk, mv);
   return cudaGetLastError();
 }
 
