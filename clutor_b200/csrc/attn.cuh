@@ -197,6 +197,18 @@ struct AttnRun {
   CLB_DEV int pieces(int rest) const { return static_cast<int>((rest + run - 1) / run); }
 };
 
+// Waits for an mbarrier phase, for two seconds at most; false when they ran out.
+CLB_DEV bool wait_bar(uint64_t *bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = global_ns();
+  do {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+  } while (global_ns() - t0 < 2000000000ull);
+  return false;
+}
+
 CLB_DEV void cp_async16(uint32_t dst, const void *src, bool take) {   // 16 bytes, or zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }

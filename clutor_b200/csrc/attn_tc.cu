@@ -14,7 +14,7 @@
 //           its scores the tensor cores run the other stream's products.
 // The maximum that scales a row's sums is only moved when the row's maximum has grown by more than 2^8 (the probabilities then
 // reach 2^8 at most, far inside fp16 and fp32), so rescaling O_w, a round trip through the registers, is rare.
-// The values of positions past the sequence's end inside the last box may be anything, and 0 x NaN is NaN: the MMA warp zeroes
+// The values of positions past the sequence's end inside the last box may be anything, and 0 x NaN is NaN: the keys' warp zeroes
 // their rows in shared memory. Every wait is bounded; one that runs out sets the error word.
 #include <cuda.h>
 
@@ -34,9 +34,10 @@ struct TcAttn {
   static constexpr int N = HD == 256 ? 64 : 128;             // positions per tile
   static constexpr int THREADS = 128 * (STREAMS + 1);
   static constexpr uint32_t Q_TILE = 128 * HD * 2, STAGE = N * HD * 2;
-  static constexpr int STAGES = HD == 64 ? 10 : 5;
-  static constexpr int N_BARS = 2 * STAGES + 6 * STREAMS + 2 * 4 + 1;
-  static constexpr uint32_t SMEM = 1024 + STREAMS * Q_TILE + STAGES * STAGE + 8 * N_BARS + 16;
+  static constexpr int STAGES = HD == 64 ? 8 : 4;
+  static constexpr uint32_t OUT = 4096;                      // a softmax warp's buffer for 32 rows on their way out, 128 bytes each
+  static constexpr int N_BARS = 3 * STAGES + 6 * STREAMS + 2 * 4 + 1;
+  static constexpr uint32_t SMEM = 1024 + STREAMS * Q_TILE + STAGES * STAGE + 4 * STREAMS * OUT + 8 * N_BARS + 16;
   static constexpr uint32_t S_COL = 0, O_COL = 256;          // S_w at 128 w (P_w over its first half), O_w at 256 + HD w
   static_assert(SMEM <= 232448, "shared memory budget");
   static_assert((ATTN_MAX_SEQ + 1) * 8 <= STAGES * STAGE, "the prefix sums fit the ring");
@@ -56,11 +57,30 @@ CLB_DEV void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z,
                : "memory");
 }
 
+// 2^x for x up to 127, two at a time on the FMA pipes: x = n + f with n the nearest integer (by adding 1.5 * 2^23) and f in
+// [-0.5, 0.5]; 2^f by a polynomial of degree 5 with constant term 1, fitted to the least relative error (1.6e-7 in fp32); n
+// goes into the exponent. Below -127, -infinity included, the result is exactly 0 (n = -127, f = 0).
+CLB_DEV float2 exp2_poly(float2 x) {
+  x = make_float2(fmaxf(x.x, -127.f), fmaxf(x.y, -127.f));
+  const float2 magic = make_float2(12582912.f, 12582912.f);
+  const float2 t = fadd2(x, magic), f = fsub2(x, fsub2(t, magic));
+  float2 p = make_float2(0.0013264707522466779f, 0.0013264707522466779f);
+  p = ffma2(p, f, make_float2(0.00967151764780283f, 0.00967151764780283f));
+  p = ffma2(p, f, make_float2(0.05550733953714371f, 0.05550733953714371f));
+  p = ffma2(p, f, make_float2(0.24022242426872253f, 0.24022242426872253f));
+  p = ffma2(p, f, make_float2(0.6931470036506653f, 0.6931470036506653f));
+  p = ffma2(p, f, make_float2(1.f, 1.f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
 template <typename C>
 CLB_DEV uint32_t pack_pair(float a, float b) {   // a in the low half
   if constexpr (__is_same(C, __half)) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
+  } else if constexpr (__is_same(C, float)) {
+    return 0;
   } else {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -88,9 +108,10 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
   __shared__ TcItem items[ITEMS];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t *ring = sm + ST * S::Q_TILE;
-  uint64_t *kv_full = reinterpret_cast<uint64_t *>(ring + S::STAGES * S::STAGE), *kv_free = kv_full + S::STAGES;
+  uint8_t *out_sm = ring + S::STAGES * S::STAGE;
+  uint64_t *kv_full = reinterpret_cast<uint64_t *>(out_sm + 4 * ST * S::OUT), *kv_free = kv_full + S::STAGES;
   uint64_t *q_full = kv_free + S::STAGES, *q_free = q_full + ST, *s_full = q_free + ST, *p_half = s_full + ST, *o_full = p_half + 2 * ST;
-  uint64_t *item_full = o_full + ST, *item_free = item_full + ITEMS, *mma_done = item_free + ITEMS;
+  uint64_t *item_full = o_full + ST, *item_free = item_full + ITEMS, *v_whole = item_free + ITEMS, *mma_done = v_whole + S::STAGES;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
   const clb200_attn &a = g.a;
@@ -102,7 +123,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
   if (warp == 4 * ST + 2) run.init(g, prefix, cta);
   if (tid == 0) {
     g.joins[cta] = make_int4(0, 0, 0, 0);
-    for (int i = 0; i < S::STAGES; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_free[i], 1); }
+    for (int i = 0; i < S::STAGES; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_free[i], 1); mbar_init(&v_whole[i], 1); }
     for (int w = 0; w < ST; ++w) {
       mbar_init(&q_full[w], 1);
       mbar_init(&q_free[w], 1);
@@ -126,7 +147,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
   // The next item, by a whole warp; n 0 at the end of the run, and when the wait runs out (ok false).
   auto next_item = [&](TcItem &x) {
     const uint32_t k = it % ITEMS;
-    if (!mbar_wait_bounded(&item_full[k], (it / ITEMS) & 1)) { ok = false; x.n = 0; return; }
+    if (!wait_bar(&item_full[k], (it / ITEMS) & 1)) { ok = false; x.n = 0; return; }
     x = items[k];
     ++it;
     __syncwarp();
@@ -138,7 +159,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
     if (warp == 4 * ST + 2) {   // ---- items
       for (;; ++it) {
         const uint32_t k = it % ITEMS;
-        if (it >= ITEMS && !mbar_wait_bounded(&item_free[k], (it / ITEMS - 1) & 1)) { ok = false; break; }
+        if (it >= ITEMS && !wait_bar(&item_free[k], (it / ITEMS - 1) & 1)) { ok = false; break; }
         TcItem x{};
         if (run.more()) {
           const AttnSpan p = attn_span<N>(g, run.q, run.qt);
@@ -162,7 +183,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
 #pragma unroll
         for (int w = 0; w < ST; ++w) {
           if (x.tokens <= w * tps) continue;
-          if (q_cnt[w] && !mbar_wait_bounded(&q_free[w], (q_cnt[w] - 1) & 1)) { ok = false; break; }
+          if (q_cnt[w] && !wait_bar(&q_free[w], (q_cnt[w] - 1) & 1)) { ok = false; break; }
           ++q_cnt[w];
           if (lane == 0) {
             mbar_arrive_expect_tx(&q_full[w], static_cast<uint32_t>(tps * g.group) * HD * 2);
@@ -174,7 +195,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
       }
 #pragma unroll
       for (int w = 0; w < ST; ++w)   // every copy issued has landed before the CTA exits
-        if (q_cnt[w] && !mbar_wait_bounded(&q_full[w], (q_cnt[w] - 1) & 1)) ok = false;
+        if (q_cnt[w] && !wait_bar(&q_full[w], (q_cnt[w] - 1) & 1)) ok = false;
     } else if (warp == 4 * ST) {   // ---- keys and values
       uint32_t cnt = 0;
       const int boxes = N / box;
@@ -188,7 +209,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
       };
       auto load = [&](const CUtensorMap &map, const AttnSlot &at) -> bool {
         const uint32_t st = cnt % S::STAGES;
-        if (cnt >= S::STAGES && !mbar_wait_bounded(&kv_free[st], (cnt / S::STAGES - 1) & 1)) return false;
+        if (cnt >= S::STAGES && !wait_bar(&kv_free[st], (cnt / S::STAGES - 1) & 1)) return false;
         if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], S::STAGE);
         __syncwarp();
         if (lane < boxes) {
@@ -209,90 +230,96 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
           at = next;
           next = ahead;
         }
+        const int left = x.kv - x.tile(x.n - 1) * N;
+        if (ok && left < N) {   // values past the sequence's end in the item's last tile: zeros, since 0 x NaN is NaN
+          const uint32_t vs = (cnt - 1) % S::STAGES;
+          if (!wait_bar(&kv_full[vs], ((cnt - 1) / S::STAGES) & 1)) { ok = false; break; }
+          for (int i = lane; i < (N - max(left, 0)) * 8 * (HD / 64); i += 32) {
+            const int c = i & 7, cb = (i >> 3) % (HD / 64), row = max(left, 0) + (i >> 3) / (HD / 64);
+            *reinterpret_cast<uint4 *>(ring + vs * S::STAGE + cb * N * 128 + row * 128 + 16 * c) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_whole[vs]);
+        }
         if (!ok) break;
       }
       // every copy issued has landed before the CTA exits (already so unless a wait gave up)
       for (uint32_t v = cnt > S::STAGES ? cnt - S::STAGES : 0; v < cnt; ++v)
-        if (!mbar_wait_bounded(&kv_full[v % S::STAGES], (v / S::STAGES) & 1)) ok = false;
-    } else {   // ---- MMA
+        if (!wait_bar(&kv_full[v % S::STAGES], (v / S::STAGES) & 1)) ok = false;
+    } else if (tc::elect_one()) {   // ---- MMA: one thread, whose every instruction is on the path of both streams
       constexpr uint32_t ID_S = tc::idesc_half(BF16, false, 128, N), ID_O = tc::idesc_half(BF16, true, 128, HD);
-      uint32_t cnt = 0, q_cnt[2] = {0, 0}, p_cnt[2] = {0, 0};   // stages, items and tiles consumed
-      auto scores = [&](int w, uint32_t st) {                   // S_w = Q_w K^T; lane 0
-        const uint64_t qd = tc::sw128_desc(smem_addr(sm + w * S::Q_TILE)), kd = tc::sw128_desc(smem_addr(ring + st * S::STAGE));
+      const uint32_t q_lo = tc::sw128_lo(smem_addr(sm)), k_lo = tc::sw128_lo(smem_addr(ring)), v_lo = tc::sw128_lo(smem_addr(ring), N * 128);
+      uint32_t st = 0, round = 0, q_cnt[2] = {0, 0}, p_cnt[2] = {0, 0};   // the next stage and its phase; items and tiles consumed
+      uint32_t tails = 0;                                                   // the phase of each stage's v_whole
+      auto scores = [&](int w, uint32_t k) {   // S_w = Q_w K^T
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
-          tc::mma_f16(tmem + S::S_COL + 128 * w, qd + (kk / 4) * (128 * 128 / 16) + 2 * (kk % 4), kd + (kk / 4) * (N * 128 / 16) + 2 * (kk % 4), ID_S, kk != 0);
+          tc::mma_ss(tmem + S::S_COL + 128 * w, q_lo + w * (S::Q_TILE / 16) + (kk / 4) * (128 * 128 / 16) + 2 * (kk % 4), k + (kk / 4) * (N * 128 / 16) + 2 * (kk % 4), ID_S, kk != 0);
         tc::commit(&s_full[w]);
       };
-      auto stage = [&](uint32_t &st) {   // the next stage, once it is full
-        st = cnt % S::STAGES;
-        const bool got = mbar_wait_bounded(&kv_full[st], (cnt / S::STAGES) & 1);
-        ++cnt;
-        return got;
+      auto stage = [&]() {   // the next stage, once it is full
+        const uint32_t k = st;
+        if (!wait_bar(&kv_full[k], round)) ok = false;
+        if (++st == S::STAGES) { st = 0; round ^= 1; }
+        return k;
       };
-      TcItem x;
-      for (next_item(x); ok && x.n; next_item(x)) {
-        uint32_t ks, vs;
-        ok = stage(ks);
+      for (;; ++it) {
+        const uint32_t slot = it % ITEMS;
+        if (!wait_bar(&item_full[slot], (it / ITEMS) & 1)) { ok = false; break; }
+        const int n = items[slot].n;
+        const bool two = ST == 2 && items[slot].tokens > tps;                                  // whether the second stream has rows
+        const bool tail = n > 0 && items[slot].kv - items[slot].tile(n - 1) * N < N;           // whether the last values are mended
+        mbar_arrive(&item_free[slot]);
+        if (n == 0) break;
+        uint32_t ks = stage(), vs;
 #pragma unroll
         for (int w = 0; w < ST; ++w) {
-          if (!ok || x.tokens <= w * tps) continue;
-          ok = mbar_wait_bounded(&q_full[w], q_cnt[w]++ & 1);
-          if (ok && lane == 0) {
-            scores(w, ks);
-            if (x.n == 1) tc::commit(&q_free[w]);
-          }
+          if (w == 1 && !two) break;
+          if (!wait_bar(&q_full[w], q_cnt[w]++ & 1)) ok = false;
+          if (!ok) break;
+          scores(w, k_lo + ks * (S::STAGE / 16));
+          if (n == 1) tc::commit(&q_free[w]);
         }
         if (!ok) break;
-        if (lane == 0) tc::commit(&kv_free[ks]);
-        for (int j = 0; j < x.n; ++j) {
-          const bool more = j + 1 < x.n;
-          if (more) ok = stage(ks);
-          if (ok) ok = stage(vs);
-          if (!ok) break;
-          const int left = x.kv - x.tile(j) * N;   // rows of the tile that are the sequence's
-          if (left < N) {
-            for (int i = lane; i < (N - max(left, 0)) * 8 * (HD / 64); i += 32) {
-              const int c = i & 7, cb = (i >> 3) % (HD / 64), r = max(left, 0) + (i >> 3) / (HD / 64);
-              *reinterpret_cast<uint4 *>(ring + vs * S::STAGE + cb * N * 128 + r * 128 + 16 * c) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async();
-            __syncwarp();
+        tc::commit(&kv_free[ks]);
+        for (int j = 0; j < n; ++j) {
+          const bool more = j + 1 < n;
+          if (more) ks = stage();
+          vs = stage();
+          if (tail && !more) {
+            if (!wait_bar(&v_whole[vs], (tails >> vs) & 1)) ok = false;
+            tails ^= 1u << vs;
           }
-          const uint64_t vd = tc::sw128_desc_mn(smem_addr(ring + vs * S::STAGE), N * 128);
+          if (!ok) break;
+          const uint32_t v = v_lo + vs * (S::STAGE / 16), k = k_lo + ks * (S::STAGE / 16);
 #pragma unroll
           for (int w = 0; w < ST; ++w) {
-            if (!ok || x.tokens <= w * tps) continue;
+            if (w == 1 && !two) break;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (ok) ok = mbar_wait_bounded(&p_half[2 * w + h], p_cnt[w] & 1);
+              if (!wait_bar(&p_half[2 * w + h], p_cnt[w] & 1)) ok = false;
+              if (!ok) break;
               tc::fence_after_sync();
-              if (ok && lane == 0) {
 #pragma unroll
-                for (int kk = 0; kk < N / 32; ++kk)
-                  tc::mma_f16_ts(tmem + S::O_COL + HD * w, tmem + S::S_COL + 128 * w + 8 * (N / 32 * h + kk), vd + 128 * (N / 32 * h + kk), ID_O,
-                                 j != 0 || h != 0 || kk != 0);
-              }
+              for (int kk = 0; kk < N / 32; ++kk)
+                tc::mma_ts(tmem + S::O_COL + HD * w, tmem + S::S_COL + 128 * w + 8 * (N / 32 * h + kk), v + 128 * (N / 32 * h + kk), ID_O,
+                           (h != 0 || kk != 0) ? true : j != 0);
             }
             ++p_cnt[w];
-            if (ok && lane == 0) {
-              if (more) scores(w, ks);
-              else tc::commit(&o_full[w]);
-              if (j + 2 == x.n) tc::commit(&q_free[w]);
-            }
+            if (!ok) break;
+            if (more) scores(w, k);
+            else tc::commit(&o_full[w]);
+            if (j + 2 == n) tc::commit(&q_free[w]);
           }
           if (!ok) break;
-          if (lane == 0) {
-            tc::commit(&kv_free[vs]);
-            if (more) tc::commit(&kv_free[ks]);
-          }
+          tc::commit(&kv_free[vs]);
+          if (more) tc::commit(&kv_free[ks]);
         }
         if (!ok) break;
       }
-      if (lane == 0) {
-        tc::commit(mma_done);   // the TMEM is released only after every MMA issued has completed
-        if (!mbar_wait_bounded(mma_done, 0)) ok = false;
-      }
+      tc::commit(mma_done);   // the TMEM is released only after every MMA issued has completed
+      if (!wait_bar(mma_done, 0)) ok = false;
     }
   } else {   // ---- softmax group w, a row per thread
     if constexpr (ST == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -309,19 +336,17 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
       float m = -INFINITY;
       float2 l0 = make_float2(0.f, 0.f), l1 = l0;
       for (int j = 0; j < x.n; ++j) {
-        if (!mbar_wait_bounded(&s_full[w], s_cnt++ & 1)) { ok = false; break; }
+        if (!wait_bar(&s_full[w], s_cnt++ & 1)) { ok = false; break; }
         tc::fence_after_sync();
         uint32_t xr[N];
         float *v = reinterpret_cast<float *>(xr);
+#pragma unroll
+        for (int c = 0; c < N / 32; ++c) tc::ld_x32_async(s_col + 32 * c, xr + 32 * c);
+#pragma unroll
+        for (int c = 0; c < N / 32; ++c) tc::wait_ld_x32(xr + 32 * c);
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        tc::ld_x32_async(s_col, xr);
 #pragma unroll
-        for (int c = 0; c < N / 32; ++c) {   // the next columns are on their way while these are compared
-          tc::wait_ld_x32(xr + 32 * c);
-          if (c + 1 < N / 32) tc::ld_x32_async(s_col + 32 * (c + 1), xr + 32 * (c + 1));
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], v[32 * c + i], v[32 * c + i + 1]);
-        }
+        for (int i = 0; i < N; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], v[i], v[i + 1]);
         const int p0 = x.tile(j) * N;
         // some row of the stream does not see the whole tile
         if (p0 + N - 1 > x.lo + w * tps || (a.window > 0 && p0 <= x.hi - a.window && p0 + N - 1 >= a.sinks)) {
@@ -362,8 +387,12 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
 #pragma unroll
           for (int i = 0; i < N / 4; ++i) {
             float2 e = ffma2(make_float2(v[N / 2 * h + 2 * i], v[N / 2 * h + 2 * i + 1]), sc2, nz);
-            e.x = exp2_approx(e.x);
-            e.y = exp2_approx(e.y);
+            if (i % 4 == 3) {   // one pair in four on the FMA pipes: the special-function unit alone would be the limit
+              e = exp2_poly(e);
+            } else {
+              e.x = exp2_approx(e.x);
+              e.y = exp2_approx(e.y);
+            }
             if (i & 1) l1 = fadd2(l1, e);
             else l0 = fadd2(l0, e);
             p[i] = pack_pair<C>(e.x, e.y);
@@ -378,36 +407,53 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
       }
       if (!ok) break;
       if (x.pieces && tid == 0) g.joins[cta] = make_int4(x.s, x.head, x.qt, x.pieces);
-      if (!mbar_wait_bounded(&o_full[w], o_cnt++ & 1)) { ok = false; break; }
+      if (!wait_bar(&o_full[w], o_cnt++ & 1)) { ok = false; break; }
       tc::fence_after_sync();
-      const int t = w * tps + tr;
-      const bool row_live = r < tps * g.group && t < x.tokens;
-      const float l = (l0.x + l0.y) + (l1.x + l1.y), inv = l > 0.f ? 1.0f / l : 0.f;
-      const int64_t piece = static_cast<int64_t>(2 * cta + (x.i0 == 0 ? 1 : 0)) * g.rows + w * tps * g.group + r;
-      O *dst = static_cast<O *>(a.out) + (row_live ? (x.row + t) * a.out_stride + (x.head * g.group + r - tr * g.group) * HD : 0);
+      const float l = (l0.x + l0.y) + (l1.x + l1.y), inv = x.whole ? (l > 0.f ? 1.0f / l : 0.f) : 1.0f;
+      const int64_t piece = static_cast<int64_t>(2 * cta + (x.i0 == 0 ? 1 : 0)) * g.rows + w * tps * g.group;
+      if (!x.whole && r < tps * g.group) g.piece_ml[piece + r] = make_float2(m, l);
+      // 128 bytes of every row at a time through shared memory, so that eight lanes store a row's and not each lane its own
+      uint8_t *buf = out_sm + warp * S::OUT;
+      const int k = lane & 7;
+      auto pass = [&](const uint32_t (&u)[32], int c, bool to_piece) {   // u: this lane's row; c: the chunk of 128 bytes
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<uint4 *>(buf + lane * 128 + ((e ^ (lane & 7)) << 4)) = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int row = 4 * e + (lane >> 3), rr = 32 * (warp & 3) + row, tt = attn_token(g, rr), t = w * tps + tt;
+          const uint4 q = *reinterpret_cast<const uint4 *>(buf + row * 128 + ((k ^ (row & 7)) << 4));
+          if (rr >= tps * g.group || t >= x.tokens) continue;
+          uint8_t *dst = to_piece ? reinterpret_cast<uint8_t *>(g.piece_o + (piece + rr) * HD)
+                                  : reinterpret_cast<uint8_t *>(static_cast<O *>(a.out) + (x.row + t) * a.out_stride + (x.head * g.group + rr - tt * g.group) * HD);
+          reinterpret_cast<uint4 *>(dst + 128 * c)[k] = q;
+        }
+        __syncwarp();
+      };
+      if (x.whole && sizeof(O) == 2) {
 #pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t o[32];
-        tc::ld_x32_async(o_col + 32 * c, o);
-        tc::wait_ld_x32(o);
-        if (!row_live) continue;
-        const float *f = reinterpret_cast<const float *>(o);
-        if (x.whole) {
-          if constexpr (sizeof(O) == 2) {
+        for (int c = 0; c < HD / 64; ++c) {
+          uint32_t o[64], u[32];
+          tc::ld_x32_async(o_col + 64 * c, o);
+          tc::ld_x32_async(o_col + 64 * c + 32, o + 32);
+          tc::wait_ld_x32(o);
+          tc::wait_ld_x32(o + 32);
 #pragma unroll
-            for (int i = 0; i < 32; i += 8)
-              *reinterpret_cast<uint4 *>(dst + 32 * c + i) = make_uint4(pack_pair<O>(f[i] * inv, f[i + 1] * inv), pack_pair<O>(f[i + 2] * inv, f[i + 3] * inv),
-                                                                        pack_pair<O>(f[i + 4] * inv, f[i + 5] * inv), pack_pair<O>(f[i + 6] * inv, f[i + 7] * inv));
-          } else {
+          for (int i = 0; i < 32; ++i) u[i] = pack_pair<O>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+          pass(u, c, false);
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          tc::ld_x32_async(o_col + 32 * c, o);
+          tc::wait_ld_x32(o);
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) store4<O>(dst + 32 * c + i, make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]), inv);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(g.piece_o + piece * HD + 32 * c + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+          pass(o, c, !x.whole);
         }
       }
-      if (!x.whole && row_live) g.piece_ml[piece] = make_float2(m, l);
       tc::fence_before_sync();
     }
     grid_launch_dependents();

@@ -34,12 +34,35 @@ __host__ __device__ constexpr uint32_t idesc_half(bool bf16, bool b_mn, int M, i
   return idesc_f16_f32(M, N) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
 }
 
-// Shared-memory descriptor of an N-major operand in 128-byte-swizzled blocks: a block is 64 elements of N by any number of
-// rows of K, 128 bytes a row (row k's 16-byte chunk j at chunk position j ^ (k % 8)), and blocks `block_bytes` apart follow
-// one another along N. One MMA reads 16 rows: successive K steps advance the start address by 2048 bytes.
-CLB_DEV uint64_t sw128_desc_mn(uint32_t smem_byte_addr, uint32_t block_bytes) {
-  return (static_cast<uint64_t>((smem_byte_addr >> 4) & 0x3FFFu)) | (static_cast<uint64_t>(block_bytes >> 4) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+// An N-major operand lies in 128-byte-swizzled blocks: a block is 64 elements of N by any number of rows of K, 128 bytes a row
+// (row k's 16-byte chunk j at chunk position j ^ (k % 8)), and blocks follow one another along N at a fixed distance, which
+// its descriptor holds in place of LBO. One MMA reads 16 rows: successive K steps advance the start address by 2048 bytes.
+//
+// The two words of those descriptors: the high one is the same for both layouts, the low one holds the start address (16-byte
+// units, bits 0-13; adding to it advances the address) and the distance of blocks (bits 16-29).
+constexpr uint32_t SW128_HI = (1024 >> 4) | (1u << 14) | (2u << 29);
+CLB_DEV uint32_t sw128_lo(uint32_t smem_byte_addr, uint32_t block_bytes = 16) { return ((smem_byte_addr >> 4) & 0x3FFFu) | ((block_bytes >> 4) << 16); }
+
+// kind::f16 products with the descriptors given by their low words: A and B in shared memory, and A in TMEM.
+CLB_DEV void mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %5, 0;\n mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(SW128_HI), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+CLB_DEV void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n mov.b64 b, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(SW128_HI), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+// True in one lane of a converged warp.
+CLB_DEV bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0;
 }
 
 CLB_DEV void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate) {
