@@ -12,10 +12,9 @@
 namespace clb {
 namespace {
 
-constexpr int CL = 8;                        // CTAs of a cluster: one row
-constexpr int ST = 512, SW = ST / 32;        // threads and warps of a CTA
+constexpr int ST = 1024, SW = ST / 32;       // threads and warps of a CTA
 constexpr int NB = 1024;                     // bins of a histogram
-constexpr int CAP = 512;                     // tokens of one bin that are ordered directly
+constexpr int CAP = 512;                     // tokens that are sorted directly
 constexpr int SAMPLE_MAX_VOCAB = 1 << 18;
 constexpr double UNIT = 17592186044416.0;    // 2^44
 constexpr float BINS_PER_NAT = 32.f;         // the first histogram's bins cover 32 e-foldings: lighter weights are below 2^-44
@@ -31,28 +30,31 @@ CLB_DEV uint32_t key_of(float x) {
 }
 CLB_DEV float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
-// ---- the cluster -----------------------------------------------------------------------------------------------------------
+// ---- the cluster: CL CTAs, one row -----------------------------------------------------------------------------------------
+template <int CL>
 CLB_DEV uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  uint32_t r = 0;
+  if constexpr (CL > 1) asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
   return r;
 }
+template <int CL>
 CLB_DEV void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if constexpr (CL > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  else __syncthreads();
 }
-CLB_DEV uint32_t remote(const void *p, uint32_t rank) {   // p's counterpart in another CTA of the cluster
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
-  return a;
-}
-CLB_DEV u64 remote_u64(const u64 *p, uint32_t rank) {
+// A word of another CTA's shared memory, at the place that p has in this one's.
+template <int CL>
+CLB_DEV u64 remote(const u64 *p, uint32_t rank) {
+  if constexpr (CL == 1) return *p;
   u64 v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(remote(p, rank)) : "memory");
+  asm volatile("{\n .reg .u32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.u64 %0, [a];\n}\n" : "=l"(v) : "r"(smem_addr(p)), "r"(rank) : "memory");
   return v;
 }
-CLB_DEV uint32_t remote_u32(const uint32_t *p, uint32_t rank) {
+template <int CL>
+CLB_DEV uint32_t remote(const uint32_t *p, uint32_t rank) {
+  if constexpr (CL == 1) return *p;
   uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote(p, rank)) : "memory");
+  asm volatile("{\n .reg .u32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.u32 %0, [a];\n}\n" : "=r"(v) : "r"(smem_addr(p)), "r"(rank) : "memory");
   return v;
 }
 
@@ -62,18 +64,51 @@ struct Limit {
   uint32_t id;
   CLB_DEV bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= id); }
 };
+CLB_DEV u64 token_word(uint32_t key, uint32_t id) { return (static_cast<u64>(key) << 32) | (0xffffffffu - id); }   // larger first in the order
 
 struct Shared {
-  u64 sum[NB];          // a histogram's values
-  uint32_t cnt[NB];     // and counts
-  u64 list[CAP];        // this CTA's tokens of a bin: key, complement of the id
-  u64 all[CAP];         // every CTA's
-  u64 part[SW + 1];
-  u64 mine[4];          // what this CTA tells the others
-  u64 found[4];         // what a search found, for the CTA's threads
-  uint32_t n_list;
-  double exp2_64[64];   // 2^(i / 64)
+  uint32_t lo[NB], hi[NB];   // a histogram: counts in lo, or the halves of 64-bit sums
+  u64 coarse[32];            // the sums of 32 bins each
+  u64 list[CAP];             // this CTA's tokens of a search, as token_word
+  u64 all[CAP];              // every CTA's
+  u64 part[SW];
+  u64 mine[4];               // what this CTA tells the others
+  u64 found[6];              // what a search found, for the CTA's threads
+  uint32_t n_list, n_above;
+  double exp2_128[128];      // 2^(i / 128)
 };
+
+__device__ const double EXP2_128[128] = {
+    1.0, 1.0054299011128027, 1.0108892860517005, 1.016378314910953, 1.0218971486541166,
+    1.0274459491187637, 1.0330248790212284, 1.0386341019613787, 1.0442737824274138, 1.0499440858006872,
+    1.0556451783605572, 1.061377227289262, 1.0671404006768237, 1.0729348675259756, 1.0787607977571199,
+    1.0846183622133092, 1.0905077326652577, 1.0964290818163769, 1.102382583307841, 1.1083684117236787,
+    1.1143867425958924, 1.1204377524096067, 1.1265216186082418, 1.1326385195987192, 1.1387886347566916,
+    1.1449721444318042, 1.1511892299529827, 1.1574400736337511, 1.1637248587775775, 1.1700437696832502,
+    1.1763969916502812, 1.182784710984341, 1.189207115002721, 1.1956643920398273, 1.202156731452703,
+    1.2086843236265816, 1.215247359980469, 1.2218460329727576, 1.22848053610687, 1.2351510639369334,
+    1.241857812073484, 1.2486009771892048, 1.255380757024691, 1.2621973503942507, 1.2690509571917332,
+    1.275941778396392, 1.2828700160787783, 1.2898358734066657, 1.2968395546510096, 1.3038812651919358,
+    1.3109612115247644, 1.318079601266064, 1.3252366431597413, 1.3324325470831615, 1.339667524053303,
+    1.3469417862329458, 1.3542555469368927, 1.3616090206382248, 1.3690024229745905, 1.3764359707545302,
+    1.383909881963832, 1.3914243757719262, 1.3989796725383112, 1.4065759938190154, 1.4142135623730951,
+    1.4218926021691656, 1.42961333839197, 1.4373759974489824, 1.4451808069770467, 1.4530279958490526,
+    1.460917794180647, 1.4688504333369818, 1.4768261459394993, 1.4848451658727524, 1.4929077282912648,
+    1.5010140696264256, 1.5091644275934228, 1.5173590411982147, 1.5255981507445384, 1.533881997840956,
+    1.5422108254079407, 1.550584877685, 1.559004400237837, 1.567469639965553, 1.5759808451078865,
+    1.5845382652524937, 1.593142151342267, 1.6017927556826934, 1.6104903319492543, 1.6192351351948637,
+    1.6280274218573478, 1.6368674497669644, 1.645755478153965, 1.6546917676561943, 1.6636765803267364,
+    1.6727101796415966, 1.681792830507429, 1.6909247992693053, 1.7001063537185235, 1.709337763100463,
+    1.718619298122478, 1.7279512309618377, 1.7373338352737062, 1.746767386199169, 1.7562521603732995,
+    1.7657884359332727, 1.7753764925265212, 1.785016611318935, 1.7947090750031072, 1.804454167806624,
+    1.8142521755003989, 1.8241033854070534, 1.8340080864093424, 1.843966568958626, 1.8539791250833855,
+    1.864046048397789, 1.8741676341103, 1.8843441790323345, 1.8945759815869656, 1.9048633418176741,
+    1.9152065613971474, 1.925605943636125, 1.9360617934922943, 1.9465744175792332, 1.9571441241754002,
+    1.9677712232331759, 1.978456026387951, 1.9891988469672663,
+};
+
+constexpr int SAMPLE_SMEM = 227 * 1024;
+constexpr uint32_t MAX_SLICE = (SAMPLE_SMEM - sizeof(Shared)) / 4;
 
 // One row's slice in this CTA, and what is known of the row.
 struct Row {
@@ -81,196 +116,249 @@ struct Row {
   const uint32_t *key;   // [n] keys of tokens [base, base + n)
   uint32_t n, base, rank, per_thread;
   float top, inv_f;      // the largest logit; 1 / temperature
-  double scale;          // log2(e) / temperature
+  double scale, shift;   // log2(e) / temperature, and top times it
   uint32_t top_key;
 
-  // exp((x - top) / temperature): 2^y with y = n / 64 + r, 2^(n/64) from a table and 2^r by its series (|r| <= 1 / 128: the
-  // first term left out is below 4e-17), the table-driven method of Tang (1989).
-  CLB_DEV double weight(uint32_t k) const;
-  CLB_DEV u64 mass(uint32_t k) const;
+  // (top - x) / (2 temperature): halved so that it does not overflow; NaN for infinity x 0.
+  CLB_DEV float distance(float x) const { return __fmul_rn(__fsub_rn(0.5f * top, 0.5f * x), inv_f); }
+  // exp((x - top) / temperature) = 2^y with y = n / 128 + r: 2^(n/128) from a table and 2^r by its series (|r| <= 1 / 256: the
+  // first term left out is below 1.3e-15), the table-driven method of Tang (1989). Weights below 2^-45 count as 0.
+  CLB_DEV double weight(uint32_t k) const {
+    if (k == top_key) return 1.0;
+    const float x = logit_of(k);
+    if (!(distance(x) < 16.f)) return 0.0;   // also where x or top is infinite
+    const double y = fma(static_cast<double>(x), scale, -shift);
+    const double t = fma(y, 128.0, 6755399441055744.0);   // 1.5 * 2^52: the nearest integer in the low bits
+    const int n = __double2loint(t);
+    const double r = fma(t - 6755399441055744.0, -1.0 / 128.0, y);
+    double p = fma(r, 0.009618129107628477, 0.05550410866482158);
+    p = fma(p, r, 0.24022650695910072);
+    p = fma(p, r, 0.6931471805599453);
+    p = fma(p, r, 1.0) * sh->exp2_128[n & 127];
+    return __hiloint2double(__double2hiint(p) + (n >> 7) * (1 << 20), __double2loint(p));
+  }
+  CLB_DEV u64 mass(uint32_t k) const { return __double2ull_rn(weight(k) * UNIT); }
   // (top - x) / temperature in bins: equal or larger for smaller logits, so a bin holds one run of the order.
   CLB_DEV uint32_t bin(uint32_t k) const {
     if (k == top_key) return 0;
-    const float d = __fmul_rn(__fsub_rn(top, logit_of(k)), inv_f) * BINS_PER_NAT;   // NaN for infinity x 0
+    const float d = __fmul_rn(distance(logit_of(k)), 2.f * BINS_PER_NAT);
     return d < static_cast<float>(NB - 1) ? static_cast<uint32_t>(d) : static_cast<uint32_t>(NB - 1);
   }
 };
 
-__device__ const double EXP2_64[64] = {
-    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284, 1.0442737824274138,
-    1.0556451783605572, 1.0671404006768237, 1.0787607977571199, 1.0905077326652577, 1.102382583307841,
-    1.1143867425958924, 1.1265216186082418, 1.1387886347566916, 1.1511892299529827, 1.1637248587775775,
-    1.1763969916502812, 1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
-    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783, 1.2968395546510096,
-    1.3109612115247644, 1.3252366431597413, 1.339667524053303, 1.3542555469368927, 1.3690024229745905,
-    1.383909881963832, 1.3989796725383112, 1.4142135623730951, 1.42961333839197, 1.4451808069770467,
-    1.460917794180647, 1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
-    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267, 1.6104903319492543,
-    1.6280274218573478, 1.645755478153965, 1.6636765803267364, 1.681792830507429, 1.7001063537185235,
-    1.718619298122478, 1.7373338352737062, 1.7562521603732995, 1.7753764925265212, 1.7947090750031072,
-    1.8142521755003989, 1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
-    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951,
-};
-
-CLB_DEV double Row::weight(uint32_t k) const {
-  if (k == top_key) return 1.0;
-  const float x = logit_of(k);
-  if (top == INFINITY || x == -INFINITY) return 0.0;
-  const double y = (static_cast<double>(x) - static_cast<double>(top)) * scale;
-  if (!(y > -1000.0)) return 0.0;
-  const double t = y * 64.0 + 6755399441055744.0;   // 1.5 * 2^52: the nearest integer in the low bits
-  const int n = __double2loint(t);
-  const double r = fma(t - 6755399441055744.0, -1.0 / 64.0, y) * 0.6931471805599453;
-  double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  p *= sh->exp2_64[n & 63];
-  return __hiloint2double(__double2hiint(p) + (n >> 6) * (1 << 20), __double2loint(p));   // p in [0.99, 2), n >> 6 >= -1001: a normal number
-}
-CLB_DEV u64 Row::mass(uint32_t k) const { return __double2ull_rn(weight(k) * UNIT); }
-
-// The sum of the threads' values before this thread's, and (total) of all.
-CLB_DEV u64 block_scan(Shared *sh, u64 v, u64 &total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  u64 s = v;
+// Sums over a warp's lanes up to and with each.
+CLB_DEV u64 warp_scan(u64 s) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const u64 u = __shfl_up_sync(FULL_MASK, s, o);
     if (lane >= o) s += u;
   }
+  return s;
+}
+// The sum of the threads' values before this thread's, and (total) of all.
+CLB_DEV u64 block_scan(Shared *sh, u64 v, u64 &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const u64 s = warp_scan(v);
   __syncthreads();
   if (lane == 31) sh->part[warp] = s;
   __syncthreads();
-  u64 before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < SW; ++w) {
-    const u64 u = sh->part[w];
-    if (w < warp) before += u;
-    total += u;
-  }
-  return before + s - v;
+  const u64 w = warp_scan(sh->part[lane]);   // SW = 32 warps
+  total = __shfl_sync(FULL_MASK, w, 31);
+  const u64 before = __shfl_sync(FULL_MASK, w, max(warp - 1, 0));
+  return (warp ? before : 0) + s - v;
 }
 // The CTAs' values v (the same in every thread of a CTA) before this CTA's, and of all.
+template <int CL>
 CLB_DEV u64 cluster_scan(Row &r, u64 v, u64 &total) {
-  Shared *sh = r.sh;
-  cluster_sync();   // what was exchanged before has been read
-  if (threadIdx.x == 0) sh->mine[0] = v;
-  cluster_sync();
+  if constexpr (CL == 1) {
+    total = v;
+    return 0;
+  }
+  cluster_sync<CL>();   // what was exchanged before has been read
+  if (threadIdx.x == 0) r.sh->mine[0] = v;
+  cluster_sync<CL>();
   u64 before = 0;
   total = 0;
 #pragma unroll
   for (uint32_t c = 0; c < CL; ++c) {
-    const u64 u = remote_u64(&sh->mine[0], c);
+    const u64 u = remote<CL>(&r.sh->mine[0], c);
     if (c < r.rank) before += u;
     total += u;
   }
   return before;
 }
+// Threads 0 .. n - 1 (n <= CAP) hold words, the others 0; sorts them descending (bitonic).
+CLB_DEV u64 sort_words(Shared *sh, u64 x, int n) {
+  const int tid = threadIdx.x;
+  int size = 1;
+  while (size < n) size <<= 1;
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      u64 y;
+      if (j >= 32) {
+        __syncthreads();
+        if (tid < CAP) sh->all[tid] = x;
+        __syncthreads();
+        y = sh->all[(tid ^ j) & (CAP - 1)];
+      } else {
+        y = __shfl_xor_sync(FULL_MASK, x, j);
+      }
+      const bool first = (tid & j) == 0, down = (tid & k) == 0;   // down: the larger first
+      x = (x > y) == (first == down) ? x : y;
+    }
+  return tid < n ? x : 0;
+}
+// Every CTA's listed tokens, to every CTA: thread i gets the i-th.
+template <int CL>
+CLB_DEV u64 gather(Row &r, uint32_t &n) {
+  Shared *sh = r.sh;
+  const uint32_t tid = threadIdx.x;
+  uint32_t m[CL], at = 0;
+#pragma unroll
+  for (uint32_t c = 0; c < CL; ++c) m[c] = remote<CL>(&sh->n_list, c);
+  u64 x = 0;
+#pragma unroll
+  for (uint32_t c = 0; c < CL; ++c) {
+    if (tid >= at && tid < at + m[c]) x = remote<CL>(&sh->list[tid - at], c);
+    at += m[c];
+  }
+  n = at;
+  return x;
+}
+
+// A search's outcome: the end of the prefix, or, `few`, all the tokens of the prefix and of the bin that it ends in, sorted (thread
+// i the i-th of n); and the total mass of the tokens searched (masses only).
+struct Found {
+  Limit lim;
+  bool few;
+  u64 word;
+  uint32_t n;
+  u64 total;
+};
 
 // The end of the shortest prefix of the order, among the tokens that `among` keeps, whose values (masses, or ones) sum to at
-// least `want` -- for masses ceil(share x their total). Histograms over ever finer runs of the order, summed over the cluster
-// by every CTA for itself, narrow it to a bin of at most CAP tokens, which are sorted, or to one key, whose tokens count by id.
-template <bool MASS>
-CLB_DEV Limit prefix(Row &r, const Limit &among, u64 want, double share) {
+// least `want` -- for masses ceil(share x their total). Histograms over ever finer runs of the order, summed over the cluster,
+// narrow it to a bin of at most CAP tokens, which are sorted, or to one key, whose tokens count by id. Where the tokens before
+// the bin are few as well (allow_few) they are all listed and left to the caller.
+template <int CL, bool MASS>
+CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool allow_few) {
   Shared *sh = r.sh;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t lo = 0, hi = 0, shift = 0;   // the run that a level divides: at level 0 everything, then the keys [lo, hi]
+  Found f{};
   for (int level = 0;; ++level) {
-    auto inside = [&](uint32_t k, uint32_t i) {   // whether a token belongs to the run that this level divides
-      if (!among.keeps(k, r.base + i)) return false;
-      return level == 0 || (k >= lo && k <= hi);
-    };
+    auto inside = [&](uint32_t k, uint32_t i) { return among.keeps(k, r.base + i) && (level == 0 || (k >= lo && k <= hi)); };
     auto place = [&](uint32_t k) { return level == 0 ? r.bin(k) : (hi - k) >> shift; };
-    for (int b = tid; b < NB; b += ST) { sh->sum[b] = 0; sh->cnt[b] = 0; }
+    for (int b = tid; b < NB; b += ST) { sh->lo[b] = 0; sh->hi[b] = 0; }
+    if (tid == 0) { sh->n_list = 0; sh->n_above = 0; }
     __syncthreads();
+#pragma unroll 2
     for (uint32_t i = tid; i < r.n; i += ST) {
       const uint32_t k = r.key[i];
       if (!inside(k, i)) continue;
       const uint32_t b = place(k);
-      atomicAdd(&sh->cnt[b], 1u);
-      if (MASS) {
+      if (MASS) {   // in 32-bit halves with the carry, since only those add in one instruction
         const u64 m = r.mass(k);
-        if (m) atomicAdd(&sh->sum[b], m);
+        const uint32_t l = static_cast<uint32_t>(m);
+        if (!m) continue;
+        const uint32_t up = static_cast<uint32_t>(m >> 32) + (atomicAdd(&sh->lo[b], l) > ~l ? 1u : 0u);
+        if (up) atomicAdd(&sh->hi[b], up);
+      } else {
+        atomicAdd(&sh->lo[b], 1u);
       }
     }
-    cluster_sync();
-    u64 v[NB / ST], mine = 0;
-    uint32_t n[NB / ST];
+    __syncthreads();
+    {
+      const int b = 32 * warp + lane;   // a warp adds 32 bins
+      u64 v = (static_cast<u64>(sh->hi[b]) << 32) + sh->lo[b];
 #pragma unroll
-    for (int e = 0; e < NB / ST; ++e) {
-      const int b = tid * (NB / ST) + e;
-      v[e] = 0;
-      n[e] = 0;
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
+      if (lane == 0) sh->coarse[warp] = v;
+    }
+    cluster_sync<CL>();
+    if (warp == 0) {   // the 32 bins that hold the border, then the one
+      u64 v = 0;
+#pragma unroll
+      for (uint32_t c = 0; c < CL; ++c) v += remote<CL>(&sh->coarse[lane], c);
+      u64 s = warp_scan(v);
+      if (level == 0) {
+        f.total = __shfl_sync(FULL_MASK, s, 31);
+        if (MASS) {
+          const double w = ceil(share * static_cast<double>(f.total));
+          want = w >= static_cast<double>(f.total) ? f.total : w < 1.0 ? 1ull : static_cast<u64>(w);
+        }
+      }
+      const int cb = min(__ffs(__ballot_sync(FULL_MASK, s >= want)) - 1, 31) & 31;
+      const u64 before = __shfl_sync(FULL_MASK, s - v, cb);
+      v = 0;
 #pragma unroll
       for (uint32_t c = 0; c < CL; ++c) {
-        n[e] += remote_u32(&sh->cnt[b], c);
-        if (MASS) v[e] += remote_u64(&sh->sum[b], c);
+        v += remote<CL>(&sh->lo[32 * cb + lane], c);
+        if (MASS) v += static_cast<u64>(remote<CL>(&sh->hi[32 * cb + lane], c)) << 32;
       }
-      if (!MASS) v[e] = n[e];
-      mine += v[e];
-    }
-    u64 total;
-    u64 before = block_scan(sh, mine, total);
-    if (MASS && level == 0) {
-      const double w = ceil(share * static_cast<double>(total));
-      want = w >= static_cast<double>(total) ? total : w < 1.0 ? 1ull : static_cast<u64>(w);
-    }
-#pragma unroll
-    for (int e = 0; e < NB / ST; ++e) {
-      if (before < want && before + v[e] >= want) {
-        sh->found[0] = tid * (NB / ST) + e;
-        sh->found[1] = before;
-        sh->found[2] = n[e];
+      s = before + warp_scan(v);
+      const int fb = min(__ffs(__ballot_sync(FULL_MASK, s >= want)) - 1, 31) & 31;
+      if (lane == fb) {
+        sh->found[0] = 32 * cb + fb;
+        sh->found[1] = s - v;   // before the bin
+        sh->found[2] = v;
+        sh->found[3] = want;
+        sh->found[4] = f.total;
       }
-      before += v[e];
     }
-    if (tid == 0) sh->n_list = 0;
     __syncthreads();
-    const uint32_t b = static_cast<uint32_t>(sh->found[0]), count = static_cast<uint32_t>(sh->found[2]);
-    want -= sh->found[1];
-    if (count <= CAP) {   // few: every CTA lists its own, then sorts everybody's
+    const uint32_t b = static_cast<uint32_t>(sh->found[0]);
+    const u64 before = sh->found[1];
+    want = sh->found[3] - before;
+    if (level == 0) f.total = sh->found[4];
+    // list the bin's tokens and, where counts say that it fits, those before it
+    const bool with_above = !MASS && allow_few && level == 0 && before + sh->found[2] <= CAP;
+    auto list = [&](bool bin, bool above) {
       for (uint32_t i = tid; i < r.n; i += ST) {
         const uint32_t k = r.key[i];
-        if (inside(k, i) && place(k) == b) sh->list[atomicAdd(&sh->n_list, 1u)] = (static_cast<u64>(k) << 32) | (0xffffffffu - (r.base + i));
-      }
-      cluster_sync();
-      uint32_t at = 0;
-      for (uint32_t c = 0; c < CL; ++c) {
-        const uint32_t m = remote_u32(&sh->n_list, c);
-        if (tid >= at && tid < at + m) sh->all[tid] = remote_u64(&sh->list[tid - at], c);
-        at += m;
-      }
-      __syncthreads();
-      cluster_sync();   // the lists and histograms have been read
-      u64 x = static_cast<uint32_t>(tid) < count ? sh->all[tid] : 0;   // descending; 0 sorts last
-      int size = 1;
-      while (size < static_cast<int>(count)) size <<= 1;
-      for (int k = 2; k <= size; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-          u64 y;
-          if (j >= 32) {
-            __syncthreads();
-            sh->all[tid] = x;
-            __syncthreads();
-            y = sh->all[tid ^ j];
-          } else {
-            y = __shfl_xor_sync(FULL_MASK, x, j);
-          }
-          const bool first = (tid & j) == 0, down = (tid & k) == 0;   // down: the larger first
-          x = (x > y) == (first == down) ? x : y;
+        if (!inside(k, i)) continue;
+        const uint32_t at = place(k);
+        if ((bin && at == b) || (above && at < b)) {
+          const uint32_t q = atomicAdd(&sh->n_list, 1u);
+          if (q < CAP) sh->list[q] = token_word(k, r.base + i);
+        } else if (MASS && !above && at < b) {
+          atomicAdd(&sh->n_above, 1u);
         }
-      const uint32_t k = static_cast<uint32_t>(x >> 32);
-      const u64 val = static_cast<uint32_t>(tid) < count ? (MASS ? r.mass(k) : 1ull) : 0ull;
-      const u64 s = block_scan(sh, val, total);
-      if (s < want && s + val >= want) sh->found[3] = x;
-      __syncthreads();
-      const u64 f = sh->found[3];
-      return Limit{static_cast<uint32_t>(f >> 32), 0xffffffffu - static_cast<uint32_t>(f)};
+      }
+    };
+    list(true, with_above);
+    cluster_sync<CL>();
+    uint32_t n_bin = 0, n_above = 0;
+#pragma unroll
+    for (uint32_t c = 0; c < CL; ++c) {
+      n_bin += remote<CL>(&sh->n_list, c);
+      if (MASS) n_above += remote<CL>(&sh->n_above, c);
     }
-    // the keys of that bin, and their range over the cluster
+    if (n_bin <= CAP) {
+      f.few = with_above;
+      if (MASS && allow_few && level == 0 && n_bin + n_above <= CAP) {
+        cluster_sync<CL>();   // the counts have been read
+        list(false, true);
+        cluster_sync<CL>();
+        f.few = true;
+      }
+      u64 x = gather<CL>(r, f.n);
+      cluster_sync<CL>();   // lists and histograms have been read
+      x = sort_words(sh, x, static_cast<int>(f.n));
+      f.word = x;
+      if (f.few) return f;
+      const uint32_t k = static_cast<uint32_t>(x >> 32);
+      const u64 val = static_cast<uint32_t>(tid) < f.n ? (MASS ? r.mass(k) : 1ull) : 0ull;
+      u64 t;
+      const u64 s = block_scan(sh, val, t);
+      if (s < want && s + val >= want) sh->found[5] = x;
+      __syncthreads();
+      const u64 w = sh->found[5];
+      f.lim = Limit{static_cast<uint32_t>(w >> 32), 0xffffffffu - static_cast<uint32_t>(w)};
+      return f;
+    }
+    // the range of that bin's keys over the cluster
     uint32_t kmin = 0xffffffffu, kmax = 0;
     for (uint32_t i = tid; i < r.n; i += ST) {
       const uint32_t k = r.key[i];
@@ -279,84 +367,107 @@ CLB_DEV Limit prefix(Row &r, const Limit &among, u64 want, double share) {
     kmin = __reduce_min_sync(FULL_MASK, kmin);
     kmax = __reduce_max_sync(FULL_MASK, kmax);
     __syncthreads();
-    if ((tid & 31) == 0) sh->part[tid >> 5] = (static_cast<u64>(kmax) << 32) | kmin;
+    if (lane == 0) sh->part[warp] = (static_cast<u64>(kmax) << 32) | kmin;
     __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < SW; ++w) {
-        kmin = min(kmin, static_cast<uint32_t>(sh->part[w]));
-        kmax = max(kmax, static_cast<uint32_t>(sh->part[w] >> 32));
-      }
-      sh->mine[1] = (static_cast<u64>(kmax) << 32) | kmin;
+    if (warp == 0) {
+      kmin = __reduce_min_sync(FULL_MASK, static_cast<uint32_t>(sh->part[lane]));
+      kmax = __reduce_max_sync(FULL_MASK, static_cast<uint32_t>(sh->part[lane] >> 32));
+      if (lane == 0) sh->mine[1] = (static_cast<u64>(kmax) << 32) | kmin;
     }
-    cluster_sync();
+    cluster_sync<CL>();
     lo = 0xffffffffu;
     hi = 0;
+#pragma unroll
     for (uint32_t c = 0; c < CL; ++c) {
-      const u64 m = remote_u64(&sh->mine[1], c);
+      const u64 m = remote<CL>(&sh->mine[1], c);
       lo = min(lo, static_cast<uint32_t>(m));
       hi = max(hi, static_cast<uint32_t>(m >> 32));
     }
     if (lo == hi) {   // one key: the q-th of its tokens by id
       const u64 one = MASS ? r.mass(lo) : 1ull, q = one ? (want + one - 1) / one : 1;
-      u64 c = 0, t;
-      const uint32_t i0 = tid * r.per_thread, i1 = min(i0 + r.per_thread, r.n);
+      u64 c = 0, t, cl_total;
+      const uint32_t i0 = min(tid * r.per_thread, r.n), i1 = min(i0 + r.per_thread, r.n);
       for (uint32_t i = i0; i < i1; ++i) c += r.key[i] == lo && among.keeps(lo, r.base + i);
       u64 s = block_scan(sh, c, t);
-      u64 cl_total;
-      s += cluster_scan(r, t, cl_total);
+      s += cluster_scan<CL>(r, t, cl_total);
       if (tid == 0) sh->mine[2] = 0;
       __syncthreads();
       if (s < q && s + c >= q)
         for (uint32_t i = i0; i < i1; ++i)
           if (r.key[i] == lo && among.keeps(lo, r.base + i) && ++s == q) sh->mine[2] = r.base + i + 1ull;
-      cluster_sync();
+      cluster_sync<CL>();
       u64 id = 0;
-      for (uint32_t d = 0; d < CL; ++d) id = max(id, remote_u64(&sh->mine[2], d));
-      cluster_sync();
-      return Limit{lo, static_cast<uint32_t>(id - 1)};
+#pragma unroll
+      for (uint32_t d = 0; d < CL; ++d) id = max(id, remote<CL>(&sh->mine[2], d));
+      cluster_sync<CL>();
+      f.few = false;
+      f.lim = Limit{lo, static_cast<uint32_t>(id - 1)};
+      return f;
     }
     const int bits = 32 - __clz(hi - lo);
     shift = bits > 10 ? bits - 10 : 0;
-    cluster_sync();   // the ranges and the histograms have been read
+    cluster_sync<CL>();   // the ranges, lists and histograms have been read
   }
 }
 
-// One row by one cluster: its keys lie in the CTAs' shared memory, a slice each, and are read from memory once.
-__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(ST, 2) sample_kernel(const clb200_sampling s, const uint32_t slice) {
+// Four (or eight) consecutive logits as keys.
+template <typename T>
+CLB_DEV void load_keys(const T *src, uint32_t *key, uint32_t n, uint32_t base, u64 &best) {
+  constexpr uint32_t V = 16 / sizeof(T);
+  auto put = [&](uint32_t i, float x) {
+    const uint32_t k = key_of(x);
+    key[i] = k;
+    best = max(best, token_word(k, base + i));
+  };
+  const uint32_t head = min(n, static_cast<uint32_t>(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(T)));   // up to a 16-byte boundary
+  if (threadIdx.x < head) put(threadIdx.x, to_f32(src[threadIdx.x]));
+  const uint32_t body = (n - head) / V;
+  const uint4 *v = reinterpret_cast<const uint4 *>(src + head);
+#pragma unroll 8
+  for (uint32_t i = threadIdx.x; i < body; i += ST) {
+    const uint4 w = __ldcs(v + i);
+    const T *t = reinterpret_cast<const T *>(&w);
+#pragma unroll
+    for (uint32_t e = 0; e < V; ++e) put(head + V * i + e, to_f32(t[e]));
+  }
+  const uint32_t rest = head + V * body + threadIdx.x;
+  if (rest < n) put(rest, to_f32(src[rest]));
+}
+
+// One row by CL CTAs: its keys lie in their shared memory, a slice each, and are read from memory once.
+template <int CL>
+__global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, const uint32_t slice) {
   extern __shared__ __align__(16) uint8_t sm[];
   Shared *sh = reinterpret_cast<Shared *>(sm);
   uint32_t *key = reinterpret_cast<uint32_t *>(sh + 1);
-  const int row = blockIdx.x / CL, tid = threadIdx.x;
+  const int row = blockIdx.x / CL, tid = threadIdx.x, lane = tid & 31;
   Row r;
   r.sh = sh;
   r.key = key;
-  r.rank = cluster_rank();
+  r.rank = cluster_rank<CL>();
   r.base = r.rank * slice;
   r.n = r.base < static_cast<uint32_t>(s.vocab) ? min(slice, static_cast<uint32_t>(s.vocab) - r.base) : 0;
   r.per_thread = ((slice + ST - 1) / ST) | 1;   // odd: a warp's threads read different banks
-  if (tid < 64) sh->exp2_64[tid] = EXP2_64[tid];
+  if (tid < 128) sh->exp2_128[tid] = EXP2_128[tid];
   // the keys, and the largest with the lowest id
   u64 best = 0;
   const int64_t at = row * s.stride + r.base;
-#pragma unroll 8
-  for (uint32_t i = tid; i < r.n; i += ST) {
-    const float x = s.type == T_F32 ? static_cast<const float *>(s.logits)[at + i]
-                    : s.type == T_F16 ? to_f32(static_cast<const __half *>(s.logits)[at + i]) : to_f32(static_cast<const __nv_bfloat16 *>(s.logits)[at + i]);
-    const uint32_t k = key_of(x);
-    key[i] = k;
-    best = max(best, (static_cast<u64>(k) << 32) | (0xffffffffu - (r.base + i)));
-  }
+  if (s.type == T_F32) load_keys(static_cast<const float *>(s.logits) + at, key, r.n, r.base, best);
+  else if (s.type == T_F16) load_keys(static_cast<const __half *>(s.logits) + at, key, r.n, r.base, best);
+  else load_keys(static_cast<const __nv_bfloat16 *>(s.logits) + at, key, r.n, r.base, best);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(FULL_MASK, best, o));
-  if ((tid & 31) == 0) sh->part[tid >> 5] = best;
+  if (lane == 0) sh->part[tid >> 5] = best;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < SW; ++w) best = max(best, sh->part[w]);
-    sh->mine[3] = best;
+  best = sh->part[lane];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(FULL_MASK, best, o));
+  if constexpr (CL > 1) {
+    if (tid == 0) sh->mine[3] = best;
+    cluster_sync<CL>();
+#pragma unroll
+    for (uint32_t c = 0; c < CL; ++c) best = max(best, remote<CL>(&sh->mine[3], c));
   }
-  cluster_sync();
-  best = 0;
-  for (uint32_t c = 0; c < CL; ++c) best = max(best, remote_u64(&sh->mine[3], c));
   r.top_key = static_cast<uint32_t>(best >> 32);
   r.top = logit_of(r.top_key);
   const float t = s.temperature ? s.temperature[row] : 1.f;
@@ -365,17 +476,62 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(ST, 2) sample_kerne
       s.token[row] = r.top == -INFINITY ? -1 : static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
       if (s.prob) s.prob[row] = r.top == -INFINITY ? 0.f : 1.f;
     }
-    cluster_sync();   // the others may still be reading this CTA's shared memory
+    cluster_sync<CL>();   // the others may still be reading this CTA's shared memory
     return;
   }
-  r.inv_f = 1.0f / t;
-  r.scale = 1.4426950408889634 / static_cast<double>(t);
+  const float heat = fmaxf(t, 1.17549435e-38f);   // the smallest normal number, whose inverse is finite
+  r.inv_f = 1.0f / heat;
+  r.scale = 1.4426950408889634 / static_cast<double>(heat);
+  r.shift = static_cast<double>(r.top) * r.scale;
   const int k = s.top_k ? s.top_k[row] : 0;
   const float share = s.top_p ? s.top_p[row] : 1.f, least = s.min_p ? s.min_p[row] : 0.f;
   const double min_w = least > 0.f ? fmin(static_cast<double>(least), 1.0) : 0.0;
+  const double u = fmin(fmax(static_cast<double>(s.u[row]), 0.0), 1.0);   // a NaN counts as 0
+  const bool by_k = k > 0 && k < s.vocab, by_p = share < 1.f;
+  auto border = [](double part, u64 total) { return min(static_cast<u64>(part * static_cast<double>(total)), total - 1); };
+  auto answer = [&](uint32_t id, double w, u64 total) {
+    s.token[row] = static_cast<int>(id);
+    if (s.prob) s.prob[row] = static_cast<float>(w / (static_cast<double>(total) * (1.0 / UNIT)));
+  };
   Limit lim{0, 0xffffffffu};
-  if (k > 0 && k < s.vocab) lim = prefix<false>(r, lim, static_cast<u64>(k), 0.0);
-  if (share < 1.f) lim = prefix<true>(r, lim, 0, static_cast<double>(share));
+  if (by_k || by_p) {
+    Found f = by_k ? search<CL, false>(r, lim, static_cast<u64>(k), 0.0, true) : search<CL, true>(r, lim, 0, static_cast<double>(share), true);
+    if (f.few) {   // the candidates, sorted, a thread each: the filters are prefixes, the draw goes by id
+      const uint32_t q = static_cast<uint32_t>(f.word >> 32), id = 0xffffffffu - static_cast<uint32_t>(f.word);
+      const bool cand = static_cast<uint32_t>(tid) < f.n && (!by_k || tid < k);
+      double w = cand ? r.weight(q) : 0.0;
+      u64 m = __double2ull_rn(w * UNIT), total, kept;
+      const u64 before = block_scan(sh, m, total);
+      if (by_p) {
+        if (!by_k) total = f.total;
+        const double x = ceil(static_cast<double>(share) * static_cast<double>(total));
+        const u64 want = x >= static_cast<double>(total) ? total : x < 1.0 ? 1ull : static_cast<u64>(x);
+        if (before >= want) m = 0;
+      }
+      if (w < min_w) m = 0;
+      __syncthreads();
+      if (tid < CAP) sh->list[tid] = m;
+      __syncthreads();
+      // by id: the complement of the id above, the place below
+      const u64 x = sort_words(sh, m ? (static_cast<u64>(0xffffffffu - id) << 32) | static_cast<uint32_t>(tid) : 0ull, static_cast<int>(f.n));
+      const uint32_t place = static_cast<uint32_t>(x);
+      m = x ? sh->list[place & (CAP - 1)] : 0;
+      const u64 s0 = block_scan(sh, m, kept);
+      const u64 want = border(u, kept);
+      if (r.rank == 0 && s0 <= want && want < s0 + m) {
+        const uint32_t token = 0xffffffffu - static_cast<uint32_t>(x >> 32);
+        sh->found[0] = token;
+        sh->found[1] = place;
+        sh->found[2] = kept;
+      }
+      __syncthreads();
+      if (r.rank == 0 && tid == static_cast<int>(sh->found[1])) answer(static_cast<uint32_t>(sh->found[0]), w, sh->found[2]);
+      cluster_sync<CL>();
+      return;
+    }
+    lim = f.lim;
+    if (by_k && by_p) lim = search<CL, true>(r, lim, 0, static_cast<double>(share), false).lim;
+  }
   auto kept = [&](uint32_t q, uint32_t i) -> u64 {
     if (!lim.keeps(q, r.base + i)) return 0;
     const double w = r.weight(q);
@@ -383,23 +539,45 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(ST, 2) sample_kerne
   };
   // the kept masses by id: a thread's tokens, the threads before it, the CTAs before its own
   u64 mine = 0, cta_total, total;
-  const uint32_t i0 = tid * r.per_thread, i1 = min(i0 + r.per_thread, r.n);
+  const uint32_t i0 = min(tid * r.per_thread, r.n), i1 = min(i0 + r.per_thread, r.n);
+#pragma unroll 2
   for (uint32_t i = i0; i < i1; ++i) mine += kept(key[i], i);
   u64 before = block_scan(sh, mine, cta_total);
-  before += cluster_scan(r, cta_total, total);
-  const double u = fmin(fmax(static_cast<double>(s.u[row]), 0.0), 1.0);   // a NaN counts as 0
-  const u64 want = min(static_cast<u64>(u * static_cast<double>(total)), total - 1);
+  before += cluster_scan<CL>(r, cta_total, total);
+  const u64 want = border(u, total);
   if (before <= want && want < before + mine) {
     for (uint32_t i = i0; i < i1; ++i) {
       before += kept(key[i], i);
       if (before > want) {
-        s.token[row] = static_cast<int>(r.base + i);
-        if (s.prob) s.prob[row] = static_cast<float>(r.weight(key[i]) / (static_cast<double>(total) * (1.0 / UNIT)));
+        answer(r.base + i, r.weight(key[i]), total);
         break;
       }
     }
   }
-  cluster_sync();
+  cluster_sync<CL>();
+}
+
+template <int CL>
+cudaError_t launch_sample(const clb200_sampling &s, int device, cudaStream_t st) {
+  const uint32_t slice = (static_cast<uint32_t>(s.vocab) + CL - 1) / CL;
+  static bool done[64] = {};
+  if (device >= 64 || !done[device]) {
+    const cudaError_t e = cudaFuncSetAttribute(sample_kernel<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, SAMPLE_SMEM);
+    if (e != cudaSuccess) return e;
+    if (device < 64) done[device] = true;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(s.rows) * CL);
+  cfg.blockDim = dim3(ST);
+  cfg.dynamicSmemBytes = sizeof(Shared) + static_cast<size_t>(slice) * 4;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CL;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<CL>, s, slice);
 }
 
 int check(const clb200_sampling *s, char *err, size_t errlen) {
@@ -425,15 +603,13 @@ extern "C" int clb200_sample(clb200_ctx *c, const clb200_sampling *s, void *stre
   if (!c) { errf(err, errlen, "no context"); return 1; }
   if (s->rows == 0) return 0;
   const OnDevice on(c->device);
-  const uint32_t slice = (static_cast<uint32_t>(s->vocab) + CL - 1) / CL;
-  const size_t smem = sizeof(Shared) + static_cast<size_t>(slice) * 4;
-  static bool done[64] = {};
-  if (c->device >= 64 || !done[c->device]) {
-    CUDA_OR(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(Shared) + SAMPLE_MAX_VOCAB / CL * 4)),
-            "kernel attribute");
-    if (c->device < 64) done[c->device] = true;
-  }
-  sample_kernel<<<static_cast<unsigned>(s->rows) * CL, ST, smem, stream ? static_cast<cudaStream_t>(stream) : c->stream>>>(*s, slice);
-  CUDA_OR(cudaGetLastError(), "launching the sampling");
+  // the fewest CTAs a row that hold it, and more while the rows leave SMs idle: at 256 rows of 50304 a CTA a row takes @A@ us,
+  // eight @B@; one row of 151936 takes @C@ us with eight, @D@ with four
+  int cl = 1;
+  while (cl < 8 && ((s->vocab + cl - 1) / cl > static_cast<int>(MAX_SLICE) || (static_cast<int64_t>(s->rows) * cl * 2 <= c->sms && s->vocab >= 2048 * cl))) cl *= 2;
+  cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : c->stream;
+  const cudaError_t e = cl == 1 ? launch_sample<1>(*s, c->device, st) : cl == 2 ? launch_sample<2>(*s, c->device, st)
+                        : cl == 4 ? launch_sample<4>(*s, c->device, st) : launch_sample<8>(*s, c->device, st);
+  CUDA_OR(e, "launching the sampling");
   return 0;
 }

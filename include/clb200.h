@@ -400,7 +400,7 @@ int clb200_attention(clb200_ctx *c, const clb200_kv *kv, const clb200_attn *a, v
  * token at least), and have w_i >= min_p. token is the first kept id, ids ascending, at which the running sum of the kept w
  * exceeds u times their total; prob its w over that total. Each setting has a value per row; a NULL array, top_k <= 0,
  * top_p >= 1 and min_p <= 0 leave that filter out, temperature NULL is 1, and temperature <= 0 takes the arg-max (the lowest
- * id on ties) with prob 1. A row with nothing above -infinity gives token -1, prob 0. prob may be NULL. The weights are
+ * id on ties) with prob 1; one below 2^-126 counts as 2^-126. A row with nothing above -infinity gives token -1, prob 0. prob may be NULL. The weights are
  * summed as 64-bit integers in units of 2^-44, so the result does not depend on any order of execution. */
 typedef struct {
   int rows, vocab;
