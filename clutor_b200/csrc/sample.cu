@@ -1,7 +1,7 @@
 // clb200_sample: the choice of a token from logits by temperature, top-k, top-p and min-p, from given random numbers.
 //
 // Every filter keeps a prefix of the tokens ordered by (logit descending, id ascending), so a filter is a pair (key, id): a
-// token is kept when its key is larger, or equal with an id at most that one. Keys are the logits' bits made monotone.
+// token is kept when its key is larger, or equal with an id at most that one. A key is a logit's bits made monotone.
 // Weights are 64-bit integers, w = round(exp((x - M) / temperature) * 2^44): at most 2^18 of at most 2^44 fit 62 bits, and
 // integer sums do not depend on their order.
 #include <algorithm>
@@ -13,22 +13,22 @@ namespace clb {
 namespace {
 
 constexpr int ST = 1024, SW = ST / 32;       // threads and warps of a CTA
-constexpr int NB = 1024;                     // bins of a histogram
+constexpr int NB = 2048;                     // bins of a histogram
 constexpr int CAP = 512;                     // tokens that are sorted directly
+constexpr int E = 4;                         // tokens a thread weighs at once
 constexpr int SAMPLE_MAX_VOCAB = 1 << 18;
 constexpr double UNIT = 17592186044416.0;    // 2^44
-constexpr float BINS_PER_NAT = 32.f;         // the first histogram's bins cover 32 e-foldings: lighter weights are below 2^-44
+constexpr float BINS_PER_NAT = 64.f;         // the first histogram's bins cover 32 e-foldings: lighter weights are below 2^-44
 
 using u64 = unsigned long long;
 
-// A logit as an unsigned integer in the same order; NaN as -infinity.
+// A logit (not NaN, not -0) as an unsigned integer in the same order.
 CLB_DEV uint32_t key_of(float x) {
-  if (x != x) x = -INFINITY;
-  if (x == 0.f) x = 0.f;   // -0 is 0
   const uint32_t b = __float_as_uint(x);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  return b ^ (static_cast<uint32_t>(static_cast<int>(b) >> 31) | 0x80000000u);
 }
 CLB_DEV float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+constexpr uint32_t KEY_LOWEST = 0x007fffffu;   // of -infinity
 
 // ---- the cluster: CL CTAs, one row -----------------------------------------------------------------------------------------
 template <int CL>
@@ -63,20 +63,22 @@ struct Limit {
   uint32_t key;
   uint32_t id;
   CLB_DEV bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= id); }
+  CLB_DEV bool all() const { return key <= KEY_LOWEST && id == 0xffffffffu; }
 };
 CLB_DEV u64 token_word(uint32_t key, uint32_t id) { return (static_cast<u64>(key) << 32) | (0xffffffffu - id); }   // larger first in the order
 
 struct Shared {
   uint32_t lo[NB], hi[NB];   // a histogram: counts in lo, or the halves of 64-bit sums
-  u64 coarse[32];            // the sums of 32 bins each
+  u64 coarse[32];            // the sums of NB / 32 bins each
   u64 list[CAP];             // this CTA's tokens of a search, as token_word
   u64 all[CAP];              // every CTA's
   u64 part[SW];
   u64 mine[4];               // what this CTA tells the others
-  u64 found[6];              // what a search found, for the CTA's threads
+  u64 found[7];              // what a search found, for the CTA's threads
   uint32_t n_list, n_above;
   double exp2_128[128];      // 2^(i / 128)
 };
+static_assert(sizeof(Shared) % 16 == 0, "the logits follow on a 16-byte boundary");
 
 __device__ const double EXP2_128[128] = {
     1.0, 1.0054299011128027, 1.0108892860517005, 1.016378314910953, 1.0218971486541166,
@@ -108,40 +110,57 @@ __device__ const double EXP2_128[128] = {
 };
 
 constexpr int SAMPLE_SMEM = 227 * 1024;
-constexpr uint32_t MAX_SLICE = (SAMPLE_SMEM - sizeof(Shared)) / 4;
+constexpr uint32_t MAX_SLICE = (SAMPLE_SMEM - sizeof(Shared)) / 4 - 3;
 
 // One row's slice in this CTA, and what is known of the row.
+// w (at most 1) in units of 2^-44, rounded to the nearest: the sum with 2^52 has it in its low bits.
+CLB_DEV u64 units(double w) { return static_cast<u64>(__double_as_longlong(fma(w, UNIT, 4503599627370496.0))) & 0xfffffffffffffull; }
+
 struct Row {
   Shared *sh;
-  const uint32_t *key;   // [n] keys of tokens [base, base + n)
+  float *x;              // [n] logits of tokens [base, base + n): NaN as -infinity, no -0
   uint32_t n, base, rank, per_thread;
-  float top, inv_f;      // the largest logit; 1 / temperature
-  double scale, shift;   // log2(e) / temperature, and top times it
-  uint32_t top_key;
+  float top, half_top, inv_f;   // the largest logit (finite), half of it; 1 / temperature
+  double top_d, scale;   // log2(e) / temperature
 
   // (top - x) / (2 temperature): halved so that it does not overflow; NaN for infinity x 0.
-  CLB_DEV float distance(float x) const { return __fmul_rn(__fsub_rn(0.5f * top, 0.5f * x), inv_f); }
+  CLB_DEV float distance(float v) const { return __fmul_rn(fmaf(v, -0.5f, half_top), inv_f); }
   // exp((x - top) / temperature) = 2^y with y = n / 128 + r: 2^(n/128) from a table and 2^r by its series (|r| <= 1 / 256: the
-  // first term left out is below 1.3e-15), the table-driven method of Tang (1989). Weights below 2^-45 count as 0.
-  CLB_DEV double weight(uint32_t k) const {
-    if (k == top_key) return 1.0;
-    const float x = logit_of(k);
-    if (!(distance(x) < 16.f)) return 0.0;   // also where x or top is infinite
-    const double y = fma(static_cast<double>(x), scale, -shift);
-    const double t = fma(y, 128.0, 6755399441055744.0);   // 1.5 * 2^52: the nearest integer in the low bits
-    const int n = __double2loint(t);
-    const double r = fma(t - 6755399441055744.0, -1.0 / 128.0, y);
-    double p = fma(r, 0.009618129107628477, 0.05550410866482158);
-    p = fma(p, r, 0.24022650695910072);
-    p = fma(p, r, 0.6931471805599453);
-    p = fma(p, r, 1.0) * sh->exp2_128[n & 127];
-    return __hiloint2double(__double2hiint(p) + (n >> 7) * (1 << 20), __double2loint(p));
+  // first term left out is below 1.3e-15), the table-driven method of Tang (1989). Weights below 2^-45 count as 0. COUNT at once
+  // and without branches: one alone is a chain of a dozen dependent double-precision operations.
+  template <int COUNT>
+  CLB_DEV void weights(const float (&v)[COUNT], double (&w)[COUNT]) const {
+    double y[COUNT], t[COUNT];
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) y[e] = (static_cast<double>(v[e]) - top_d) * scale;
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) t[e] = fma(y[e], 128.0, 6755399441055744.0);   // 1.5 * 2^52: the nearest integer in the low bits
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) y[e] = fma(t[e] - 6755399441055744.0, -1.0 / 128.0, y[e]);
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) w[e] = fma(y[e], 0.009618129107628477, 0.05550410866482158);   // ln(2)^4 / 24, ln(2)^3 / 6
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) w[e] = fma(w[e], y[e], 0.2402265069591007);
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) w[e] = fma(w[e], y[e], 0.6931471805599453);
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) w[e] = fma(w[e], y[e], 1.0) * sh->exp2_128[__double2loint(t[e]) & 127];
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) {
+      const double u = __hiloint2double(__double2hiint(w[e]) + (__double2loint(t[e]) >> 7) * (1 << 20), __double2loint(w[e]));
+      w[e] = distance(v[e]) < 16.f ? u : 0.0;
+    }
   }
-  CLB_DEV u64 mass(uint32_t k) const { return __double2ull_rn(weight(k) * UNIT); }
+  CLB_DEV double weight(float v) const {
+    const float q[1] = {v};
+    double w[1];
+    weights(q, w);
+    return w[0];
+  }
+  CLB_DEV u64 mass(uint32_t k) const { return units(weight(logit_of(k))); }
   // (top - x) / temperature in bins: equal or larger for smaller logits, so a bin holds one run of the order.
-  CLB_DEV uint32_t bin(uint32_t k) const {
-    if (k == top_key) return 0;
-    const float d = __fmul_rn(distance(logit_of(k)), 2.f * BINS_PER_NAT);
+  CLB_DEV uint32_t bin(float v) const {
+    const float d = __fmul_rn(distance(v), 2.f * BINS_PER_NAT);
     return d < static_cast<float>(NB - 1) ? static_cast<uint32_t>(d) : static_cast<uint32_t>(NB - 1);
   }
 };
@@ -197,10 +216,14 @@ CLB_DEV u64 sort_words(Shared *sh, u64 x, int n) {
     for (int j = k >> 1; j > 0; j >>= 1) {
       u64 y;
       if (j >= 32) {
-        __syncthreads();
-        if (tid < CAP) sh->all[tid] = x;
-        __syncthreads();
-        y = sh->all[(tid ^ j) & (CAP - 1)];
+        if (tid < CAP) {   // whole warps
+          asm volatile("bar.sync 1, %0;" ::"n"(CAP) : "memory");
+          sh->all[tid] = x;
+          asm volatile("bar.sync 1, %0;" ::"n"(CAP) : "memory");
+          y = sh->all[tid ^ j];
+        } else {
+          y = 0;
+        }
       } else {
         y = __shfl_xor_sync(FULL_MASK, x, j);
       }
@@ -248,36 +271,54 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
   uint32_t lo = 0, hi = 0, shift = 0;   // the run that a level divides: at level 0 everything, then the keys [lo, hi]
   Found f{};
   for (int level = 0;; ++level) {
-    auto inside = [&](uint32_t k, uint32_t i) { return among.keeps(k, r.base + i) && (level == 0 || (k >= lo && k <= hi)); };
-    auto place = [&](uint32_t k) { return level == 0 ? r.bin(k) : (hi - k) >> shift; };
+    const bool whole = level == 0 && among.all();
+    auto inside = [&](float x, uint32_t i) {
+      if (whole) return true;
+      const uint32_t k = key_of(x);
+      return among.keeps(k, r.base + i) && (level == 0 || (k >= lo && k <= hi));
+    };
+    auto place = [&](float x) { return level == 0 ? r.bin(x) : (hi - key_of(x)) >> shift; };
     for (int b = tid; b < NB; b += ST) { sh->lo[b] = 0; sh->hi[b] = 0; }
     if (tid == 0) { sh->n_list = 0; sh->n_above = 0; }
     __syncthreads();
-#pragma unroll 2
-    for (uint32_t i = tid; i < r.n; i += ST) {
-      const uint32_t k = r.key[i];
-      if (!inside(k, i)) continue;
-      const uint32_t b = place(k);
-      if (MASS) {   // in 32-bit halves with the carry, since only those add in one instruction
-        const u64 m = r.mass(k);
-        const uint32_t l = static_cast<uint32_t>(m);
-        if (!m) continue;
-        const uint32_t up = static_cast<uint32_t>(m >> 32) + (atomicAdd(&sh->lo[b], l) > ~l ? 1u : 0u);
-        if (up) atomicAdd(&sh->hi[b], up);
-      } else {
-        atomicAdd(&sh->lo[b], 1u);
+    if (MASS) {
+      for (uint32_t i = tid; i < r.n; i += E * ST) {
+        float x[E];
+        double w[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {   // what does not belong here weighs nothing
+          const uint32_t q = i + e * ST;
+          x[e] = q < r.n ? r.x[q] : -INFINITY;
+          if (!inside(x[e], q)) x[e] = -INFINITY;
+        }
+        r.weights(x, w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {   // in 32-bit halves with the carry, since only those add in one instruction
+          const u64 m = units(w[e]);
+          if (!m) continue;
+          const uint32_t b = place(x[e]), l = static_cast<uint32_t>(m);
+          const uint32_t up = static_cast<uint32_t>(m >> 32) + (atomicAdd(&sh->lo[b], l) > ~l ? 1u : 0u);
+          if (up) atomicAdd(&sh->hi[b], up);
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (uint32_t i = tid; i < r.n; i += ST) {
+        const float x = r.x[i];
+        if (inside(x, i)) atomicAdd(&sh->lo[place(x)], 1u);
       }
     }
     __syncthreads();
-    {
-      const int b = 32 * warp + lane;   // a warp adds 32 bins
-      u64 v = (static_cast<u64>(sh->hi[b]) << 32) + sh->lo[b];
+    {   // a warp adds NB / 32 bins
+      u64 v = 0;
+#pragma unroll
+      for (int b = 0; b < NB / 32; b += 32) v += (static_cast<u64>(sh->hi[NB / 32 * warp + b + lane]) << 32) + sh->lo[NB / 32 * warp + b + lane];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
       if (lane == 0) sh->coarse[warp] = v;
     }
     cluster_sync<CL>();
-    if (warp == 0) {   // the 32 bins that hold the border, then the one
+    if (warp == 0) {   // the NB / 32 bins that hold the border, then the one, then its keys
       u64 v = 0;
 #pragma unroll
       for (uint32_t c = 0; c < CL; ++c) v += remote<CL>(&sh->coarse[lane], c);
@@ -291,40 +332,79 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
       }
       const int cb = min(__ffs(__ballot_sync(FULL_MASK, s >= want)) - 1, 31) & 31;
       const u64 before = __shfl_sync(FULL_MASK, s - v, cb);
-      v = 0;
+      constexpr int PER = NB / 32 / 32;   // a lane's bins
+      u64 bv[PER], mine = 0;
 #pragma unroll
-      for (uint32_t c = 0; c < CL; ++c) {
-        v += remote<CL>(&sh->lo[32 * cb + lane], c);
-        if (MASS) v += static_cast<u64>(remote<CL>(&sh->hi[32 * cb + lane], c)) << 32;
+      for (int e = 0; e < PER; ++e) {
+        const int at = NB / 32 * cb + PER * lane + e;
+        bv[e] = 0;
+#pragma unroll
+        for (uint32_t c = 0; c < CL; ++c) {
+          bv[e] += remote<CL>(&sh->lo[at], c);
+          if (MASS) bv[e] += static_cast<u64>(remote<CL>(&sh->hi[at], c)) << 32;
+        }
+        mine += bv[e];
       }
-      s = before + warp_scan(v);
-      const int fb = min(__ffs(__ballot_sync(FULL_MASK, s >= want)) - 1, 31) & 31;
-      if (lane == fb) {
-        sh->found[0] = 32 * cb + fb;
-        sh->found[1] = s - v;   // before the bin
-        sh->found[2] = v;
+      s = before + warp_scan(mine);
+      const int fl = min(__ffs(__ballot_sync(FULL_MASK, s >= want)) - 1, 31) & 31;
+      u64 at = s - mine, value = bv[0];
+      uint32_t b = NB / 32 * cb + PER * lane;
+#pragma unroll
+      for (int e = 1; e < PER; ++e)
+        if (at + value < want) { at += value; value = bv[e]; ++b; }
+      b = __shfl_sync(FULL_MASK, b, fl);
+      // the bin's keys: bins do not grow with the key, so its ends are found by halving, 32 ways at a time
+      uint32_t first, after;
+      const uint32_t top_key = key_of(r.top);
+      if (level == 0) {
+        auto least = [&](uint32_t most) {   // the smallest key whose bin is at most `most`
+          uint32_t base = 0;
+#pragma unroll 1
+          for (int sh5 = 27; sh5 > -5; sh5 -= 5) {   // 5 bits a round, the last of 2
+            const int sft = max(sh5, 0), ways = sh5 < 0 ? 4 : 32;
+            const uint32_t probe = base + ((static_cast<uint32_t>(lane) + 1) << sft) - 1;   // the last key of the lane's part
+            const bool reach = lane < ways && (probe >= top_key || (probe >= KEY_LOWEST && r.bin(logit_of(probe)) <= most));
+            base += static_cast<uint32_t>(__ffs(__ballot_sync(FULL_MASK, reach)) - 1) << sft;
+          }
+          return base;
+        };
+        first = b < NB - 1 ? least(b) : KEY_LOWEST;
+        after = b ? least(b - 1) : top_key + 1;
+      } else {
+        after = hi - (b << shift) + 1;
+        first = after - (1u << shift) < lo || after < (1u << shift) ? lo : after - (1u << shift);
+      }
+      if (lane == fl) {
+        sh->found[0] = (static_cast<u64>(after) << 32) | first;
+        sh->found[1] = at;   // before the bin
+        sh->found[2] = value;
         sh->found[3] = want;
         sh->found[4] = f.total;
       }
     }
     __syncthreads();
-    const uint32_t b = static_cast<uint32_t>(sh->found[0]);
+    const uint32_t k0 = static_cast<uint32_t>(sh->found[0]), k1 = static_cast<uint32_t>(sh->found[0] >> 32) - 1;   // the bin's keys: k0 .. k1
     const u64 before = sh->found[1];
     want = sh->found[3] - before;
     if (level == 0) f.total = sh->found[4];
     // list the bin's tokens and, where counts say that it fits, those before it
     const bool with_above = !MASS && allow_few && level == 0 && before + sh->found[2] <= CAP;
     auto list = [&](bool bin, bool above) {
+      uint32_t seen = 0;
+#pragma unroll 4
       for (uint32_t i = tid; i < r.n; i += ST) {
-        const uint32_t k = r.key[i];
-        if (!inside(k, i)) continue;
-        const uint32_t at = place(k);
-        if ((bin && at == b) || (above && at < b)) {
+        const uint32_t k = key_of(r.x[i]);
+        if (k < k0 || !among.keeps(k, r.base + i)) continue;
+        if (k <= k1 ? bin : above) {
           const uint32_t q = atomicAdd(&sh->n_list, 1u);
           if (q < CAP) sh->list[q] = token_word(k, r.base + i);
-        } else if (MASS && !above && at < b) {
-          atomicAdd(&sh->n_above, 1u);
+        } else {
+          ++seen;
         }
+      }
+      if (MASS && !above) {   // how many come before the bin
+        seen = __reduce_add_sync(FULL_MASK, seen);
+        if (lane == 0 && seen) atomicAdd(&sh->n_above, seen);
       }
     };
     list(true, with_above);
@@ -361,8 +441,8 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
     // the range of that bin's keys over the cluster
     uint32_t kmin = 0xffffffffu, kmax = 0;
     for (uint32_t i = tid; i < r.n; i += ST) {
-      const uint32_t k = r.key[i];
-      if (inside(k, i) && place(k) == b) { kmin = min(kmin, k); kmax = max(kmax, k); }
+      const uint32_t k = key_of(r.x[i]);
+      if (k >= k0 && k <= k1 && among.keeps(k, r.base + i)) { kmin = min(kmin, k); kmax = max(kmax, k); }
     }
     kmin = __reduce_min_sync(FULL_MASK, kmin);
     kmax = __reduce_max_sync(FULL_MASK, kmax);
@@ -387,14 +467,14 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
       const u64 one = MASS ? r.mass(lo) : 1ull, q = one ? (want + one - 1) / one : 1;
       u64 c = 0, t, cl_total;
       const uint32_t i0 = min(tid * r.per_thread, r.n), i1 = min(i0 + r.per_thread, r.n);
-      for (uint32_t i = i0; i < i1; ++i) c += r.key[i] == lo && among.keeps(lo, r.base + i);
+      for (uint32_t i = i0; i < i1; ++i) c += key_of(r.x[i]) == lo && among.keeps(lo, r.base + i);
       u64 s = block_scan(sh, c, t);
       s += cluster_scan<CL>(r, t, cl_total);
       if (tid == 0) sh->mine[2] = 0;
       __syncthreads();
       if (s < q && s + c >= q)
         for (uint32_t i = i0; i < i1; ++i)
-          if (r.key[i] == lo && among.keeps(lo, r.base + i) && ++s == q) sh->mine[2] = r.base + i + 1ull;
+          if (key_of(r.x[i]) == lo && among.keeps(lo, r.base + i) && ++s == q) sh->mine[2] = r.base + i + 1ull;
       cluster_sync<CL>();
       u64 id = 0;
 #pragma unroll
@@ -405,22 +485,24 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
       return f;
     }
     const int bits = 32 - __clz(hi - lo);
-    shift = bits > 10 ? bits - 10 : 0;
+    shift = bits > 11 ? bits - 11 : 0;   // NB = 2^11 bins
     cluster_sync<CL>();   // the ranges, lists and histograms have been read
   }
 }
 
-// Four (or eight) consecutive logits as keys.
+// n logits from src into shared memory, which starts where the first 16-byte boundary of src falls on one there too; returns the
+// first's place. best: the thread's largest.
 template <typename T>
-CLB_DEV void load_keys(const T *src, uint32_t *key, uint32_t n, uint32_t base, u64 &best) {
+CLB_DEV float *load_logits(const T *src, float *dst, uint32_t n, float &best) {
   constexpr uint32_t V = 16 / sizeof(T);
-  auto put = [&](uint32_t i, float x) {
-    const uint32_t k = key_of(x);
-    key[i] = k;
-    best = max(best, token_word(k, base + i));
+  auto clean = [&](float v) {   // NaN as -infinity, -0 as 0
+    v = fmaxf(v, -INFINITY) + 0.f;
+    best = fmaxf(best, v);
+    return v;
   };
-  const uint32_t head = min(n, static_cast<uint32_t>(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(T)));   // up to a 16-byte boundary
-  if (threadIdx.x < head) put(threadIdx.x, to_f32(src[threadIdx.x]));
+  const uint32_t head = min(n, static_cast<uint32_t>(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(T)));
+  dst += (4 - (head & 3)) & 3;
+  if (threadIdx.x < head) dst[threadIdx.x] = clean(to_f32(src[threadIdx.x]));
   const uint32_t body = (n - head) / V;
   const uint4 *v = reinterpret_cast<const uint4 *>(src + head);
 #pragma unroll 8
@@ -428,61 +510,75 @@ CLB_DEV void load_keys(const T *src, uint32_t *key, uint32_t n, uint32_t base, u
     const uint4 w = __ldcs(v + i);
     const T *t = reinterpret_cast<const T *>(&w);
 #pragma unroll
-    for (uint32_t e = 0; e < V; ++e) put(head + V * i + e, to_f32(t[e]));
+    for (uint32_t e = 0; e < V; e += 4)
+      *reinterpret_cast<float4 *>(dst + head + V * i + e) = make_float4(clean(to_f32(t[e])), clean(to_f32(t[e + 1])), clean(to_f32(t[e + 2])), clean(to_f32(t[e + 3])));
   }
   const uint32_t rest = head + V * body + threadIdx.x;
-  if (rest < n) put(rest, to_f32(src[rest]));
+  if (rest < n) dst[rest] = clean(to_f32(src[rest]));
+  return dst;
 }
 
-// One row by CL CTAs: its keys lie in their shared memory, a slice each, and are read from memory once.
+// One row by CL CTAs: its logits lie in their shared memory, a slice each, and are read from memory once.
 template <int CL>
 __global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, const uint32_t slice) {
   extern __shared__ __align__(16) uint8_t sm[];
   Shared *sh = reinterpret_cast<Shared *>(sm);
-  uint32_t *key = reinterpret_cast<uint32_t *>(sh + 1);
+  float *room = reinterpret_cast<float *>(sh + 1);   // slice + 3
   const int row = blockIdx.x / CL, tid = threadIdx.x, lane = tid & 31;
   Row r;
   r.sh = sh;
-  r.key = key;
   r.rank = cluster_rank<CL>();
   r.base = r.rank * slice;
   r.n = r.base < static_cast<uint32_t>(s.vocab) ? min(slice, static_cast<uint32_t>(s.vocab) - r.base) : 0;
   r.per_thread = ((slice + ST - 1) / ST) | 1;   // odd: a warp's threads read different banks
   if (tid < 128) sh->exp2_128[tid] = EXP2_128[tid];
-  // the keys, and the largest with the lowest id
-  u64 best = 0;
+  float best = -INFINITY;
   const int64_t at = row * s.stride + r.base;
-  if (s.type == T_F32) load_keys(static_cast<const float *>(s.logits) + at, key, r.n, r.base, best);
-  else if (s.type == T_F16) load_keys(static_cast<const __half *>(s.logits) + at, key, r.n, r.base, best);
-  else load_keys(static_cast<const __nv_bfloat16 *>(s.logits) + at, key, r.n, r.base, best);
+  if (s.type == T_F32) r.x = load_logits(static_cast<const float *>(s.logits) + at, room, r.n, best);
+  else if (s.type == T_F16) r.x = load_logits(static_cast<const __half *>(s.logits) + at, room, r.n, best);
+  else r.x = load_logits(static_cast<const __nv_bfloat16 *>(s.logits) + at, room, r.n, best);
+  auto largest = [&](u64 v) {   // of the row's threads
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(FULL_MASK, best, o));
-  if (lane == 0) sh->part[tid >> 5] = best;
-  __syncthreads();
-  best = sh->part[lane];
+    for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(FULL_MASK, v, o));
+    __syncthreads();
+    if (lane == 0) sh->part[tid >> 5] = v;
+    __syncthreads();
+    v = sh->part[lane];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(FULL_MASK, best, o));
-  if constexpr (CL > 1) {
-    if (tid == 0) sh->mine[3] = best;
-    cluster_sync<CL>();
+    for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(FULL_MASK, v, o));
+    if constexpr (CL > 1) {
+      cluster_sync<CL>();   // what was exchanged before has been read
+      if (tid == 0) sh->mine[3] = v;
+      cluster_sync<CL>();
 #pragma unroll
-    for (uint32_t c = 0; c < CL; ++c) best = max(best, remote<CL>(&sh->mine[3], c));
-  }
-  r.top_key = static_cast<uint32_t>(best >> 32);
-  r.top = logit_of(r.top_key);
+      for (uint32_t c = 0; c < CL; ++c) v = max(v, remote<CL>(&sh->mine[3], c));
+    }
+    return v;
+  };
+  r.top = logit_of(static_cast<uint32_t>(largest(key_of(best))));
   const float t = s.temperature ? s.temperature[row] : 1.f;
   if (r.top == -INFINITY || !(t > 0.f)) {
+    u64 first = 0;   // the lowest id among the largest
+    for (uint32_t i = tid; i < r.n; i += ST)
+      if (r.x[i] == r.top) { first = 0xffffffffu - (r.base + i); break; }
+    first = largest(first);
     if (r.rank == 0 && tid == 0) {
-      s.token[row] = r.top == -INFINITY ? -1 : static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
+      s.token[row] = r.top == -INFINITY ? -1 : static_cast<int>(0xffffffffu - static_cast<uint32_t>(first));
       if (s.prob) s.prob[row] = r.top == -INFINITY ? 0.f : 1.f;
     }
     cluster_sync<CL>();   // the others may still be reading this CTA's shared memory
     return;
   }
+  if (r.top == INFINITY) {   // those at infinity share everything
+    for (uint32_t i = tid; i < r.n; i += ST) r.x[i] = r.x[i] == INFINITY ? 0.f : -INFINITY;
+    r.top = 0.f;
+    __syncthreads();
+  }
+  r.half_top = 0.5f * r.top;
+  r.top_d = static_cast<double>(r.top);
   const float heat = fmaxf(t, 1.17549435e-38f);   // the smallest normal number, whose inverse is finite
   r.inv_f = 1.0f / heat;
   r.scale = 1.4426950408889634 / static_cast<double>(heat);
-  r.shift = static_cast<double>(r.top) * r.scale;
   const int k = s.top_k ? s.top_k[row] : 0;
   const float share = s.top_p ? s.top_p[row] : 1.f, least = s.min_p ? s.min_p[row] : 0.f;
   const double min_w = least > 0.f ? fmin(static_cast<double>(least), 1.0) : 0.0;
@@ -493,14 +589,14 @@ __global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, 
     s.token[row] = static_cast<int>(id);
     if (s.prob) s.prob[row] = static_cast<float>(w / (static_cast<double>(total) * (1.0 / UNIT)));
   };
-  Limit lim{0, 0xffffffffu};
+  Limit lim{KEY_LOWEST, 0xffffffffu};
   if (by_k || by_p) {
     Found f = by_k ? search<CL, false>(r, lim, static_cast<u64>(k), 0.0, true) : search<CL, true>(r, lim, 0, static_cast<double>(share), true);
     if (f.few) {   // the candidates, sorted, a thread each: the filters are prefixes, the draw goes by id
       const uint32_t q = static_cast<uint32_t>(f.word >> 32), id = 0xffffffffu - static_cast<uint32_t>(f.word);
       const bool cand = static_cast<uint32_t>(tid) < f.n && (!by_k || tid < k);
-      double w = cand ? r.weight(q) : 0.0;
-      u64 m = __double2ull_rn(w * UNIT), total, kept;
+      double w = cand ? r.weight(logit_of(q)) : 0.0;
+      u64 m = units(w), total, kept;
       const u64 before = block_scan(sh, m, total);
       if (by_p) {
         if (!by_k) total = f.total;
@@ -513,7 +609,7 @@ __global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, 
       if (tid < CAP) sh->list[tid] = m;
       __syncthreads();
       // by id: the complement of the id above, the place below
-      const u64 x = sort_words(sh, m ? (static_cast<u64>(0xffffffffu - id) << 32) | static_cast<uint32_t>(tid) : 0ull, static_cast<int>(f.n));
+      const u64 x = sort_words(sh, m ? (static_cast<u64>(0xffffffffu - id) << 32) | static_cast<uint32_t>(tid) : 0ull, by_k ? min(static_cast<int>(f.n), k) : static_cast<int>(f.n));
       const uint32_t place = static_cast<uint32_t>(x);
       m = x ? sh->list[place & (CAP - 1)] : 0;
       const u64 s0 = block_scan(sh, m, kept);
@@ -532,24 +628,38 @@ __global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, 
     lim = f.lim;
     if (by_k && by_p) lim = search<CL, true>(r, lim, 0, static_cast<double>(share), false).lim;
   }
-  auto kept = [&](uint32_t q, uint32_t i) -> u64 {
-    if (!lim.keeps(q, r.base + i)) return 0;
-    const double w = r.weight(q);
-    return w >= min_w ? __double2ull_rn(w * UNIT) : 0ull;
+  const bool every = lim.all();
+  auto kept = [&](float x, uint32_t i) -> u64 {
+    if (!every && !lim.keeps(key_of(x), r.base + i)) return 0;
+    const double w = r.weight(x);
+    return w >= min_w ? units(w) : 0ull;
   };
   // the kept masses by id: a thread's tokens, the threads before it, the CTAs before its own
   u64 mine = 0, cta_total, total;
   const uint32_t i0 = min(tid * r.per_thread, r.n), i1 = min(i0 + r.per_thread, r.n);
-#pragma unroll 2
-  for (uint32_t i = i0; i < i1; ++i) mine += kept(key[i], i);
+  for (uint32_t i = i0; i < i1; i += E) {
+    float x[E];
+    double w[E];
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      x[e] = i + e < i1 ? r.x[i + e] : -INFINITY;
+      if (!every && !lim.keeps(key_of(x[e]), r.base + i + e)) x[e] = -INFINITY;
+      any = any || x[e] != -INFINITY;
+    }
+    if (!any) continue;
+    r.weights(x, w);
+#pragma unroll
+    for (int e = 0; e < E; ++e) mine += w[e] >= min_w ? units(w[e]) : 0ull;
+  }
   u64 before = block_scan(sh, mine, cta_total);
   before += cluster_scan<CL>(r, cta_total, total);
   const u64 want = border(u, total);
   if (before <= want && want < before + mine) {
     for (uint32_t i = i0; i < i1; ++i) {
-      before += kept(key[i], i);
+      before += kept(r.x[i], i);
       if (before > want) {
-        answer(r.base + i, r.weight(key[i]), total);
+        answer(r.base + i, r.weight(r.x[i]), total);
         break;
       }
     }
@@ -569,7 +679,7 @@ cudaError_t launch_sample(const clb200_sampling &s, int device, cudaStream_t st)
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(s.rows) * CL);
   cfg.blockDim = dim3(ST);
-  cfg.dynamicSmemBytes = sizeof(Shared) + static_cast<size_t>(slice) * 4;
+  cfg.dynamicSmemBytes = sizeof(Shared) + static_cast<size_t>(slice + 3) * 4;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
