@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import re
+import struct
 
 import numpy as np
 
@@ -284,6 +285,11 @@ class Context:
             raise ClutorError(self._err.value.decode())
         self.device = device
         self._keep: list = []
+        # the serving calls' argument structs, written anew for every call
+        self._kv, self._args = C.create_string_buffer(_KV.size), C.create_string_buffer(max(_QK.size, _ATTN.size, _SAMPLING.size))
+        self._kv_at, self._args_at = C.addressof(self._kv), C.addressof(self._args)
+        self._c_qk, self._c_attention, self._c_sample = lib().clb200_qk_rope, lib().clb200_attention, lib().clb200_sample
+        self._work_bytes: dict = {}
 
     def close(self) -> None:
         if self.handle:
@@ -409,28 +415,32 @@ class Context:
         type; rows any stride apart) are normalised, turned by position and, k and v, stored into `pages`; q_start [n_seq + 1]
         and kv_len [n_seq] int32; rope [n_pos, head_dim] float32 (cosines, then sines). Returns the turned q, [T, n_head,
         head_dim] of the cache's type (`out`, or a new tensor); asynchronous."""
-        import torch
-        st = _torch_stream(stream, self.device)
-        self._tensors(pages=pages.k, q=q, k=k, v=v, rope=rope, q_start=q_start, kv_len=kv_len, q_norm=q_norm, k_norm=k_norm, out=out)
         T, H, D = q.shape
-        if k.shape != (T, pages.n_kv, D) or v.shape != k.shape or D != pages.head_dim:
+        KV, dt = pages.n_kv, q.dtype
+        if k.shape != (T, KV, D) or v.shape != (T, KV, D) or D != pages.head_dim:
             raise ClutorError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit a cache of "
-                              f"{pages.n_kv} heads of {pages.head_dim}")
-        if k.dtype != q.dtype or v.dtype != q.dtype:
+                              f"{KV} heads of {pages.head_dim}")
+        if k.dtype != dt or v.dtype != dt:
             raise ClutorError("q, k and v must have one type")
-        if rope.dtype != torch.float32 or rope.dim() != 2 or rope.shape[1] != D or not rope.is_contiguous():
+        self._on_device(pages.k, q, k, v, rope, q_start, kv_len, q_norm, k_norm, out)
+        if rope.dtype != _torch().float32 or rope.dim() != 2 or rope.shape[1] != D or not rope.is_contiguous():
             raise ClutorError("rope must be a contiguous float32 [n_pos, head_dim] tensor")
         if norm:
-            nq, nk = (D, D) if norm == QK_NORM_HEAD else (H * D, pages.n_kv * D)
-            for w, n in ((q_norm, nq), (k_norm, nk)):
-                if w is None or w.dtype != torch.float32 or w.numel() != n or not w.is_contiguous():
-                    raise ClutorError(f"the norm's weights must be contiguous float32 tensors of {nq} and {nk} elements")
-        out = _out(out, (T, H, D), pages.k.dtype, q.device, st, stream)
-        kv = pages.struct(q_start, kv_len)
-        a = QkStruct(T, H, _dtype(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), _rows(q), _rows(k), _rows(v), int(norm),
-                     _ptr(q_norm), _ptr(k_norm), eps, rope.data_ptr(), rope.shape[0], int(pairs), out.data_ptr(), _rows(out))
-        self._check(lib().clb200_qk_rope(self.handle, C.byref(kv), C.byref(a), st.cuda_stream or CUDA_STREAM_LEGACY,
-                                         self._err, 512))
+            for w, n in ((q_norm, D if norm == QK_NORM_HEAD else H * D), (k_norm, D if norm == QK_NORM_HEAD else KV * D)):
+                if w is None or w.dtype != _torch().float32 or w.numel() != n or not w.is_contiguous():
+                    raise ClutorError("the norm's weights must be contiguous float32 tensors of head_dim elements, or for the "
+                                      "whole row of its heads' elements")
+        st = self._raw_stream(stream)
+        if out is None:
+            out = _empty((T, H, D), pages.k.dtype, q.device, stream)
+        elif out.shape != (T, H, D) or out.dtype != pages.k.dtype:
+            raise ClutorError(f"out must be {[T, H, D]} of {pages.k.dtype}")
+        pages.pack(self._kv, q_start, kv_len)
+        _QK.pack_into(self._args, 0, T, H, _dtype(dt), q.data_ptr(), k.data_ptr(), v.data_ptr(), _rows(q), _rows(k), _rows(v), norm,
+                      q_norm.data_ptr() if q_norm is not None else 0, k_norm.data_ptr() if k_norm is not None else 0, eps,
+                      rope.data_ptr(), rope.shape[0], 1 if pairs else 0, out.data_ptr(), _rows(out))
+        if self._c_qk(self.handle, self._kv_at, self._args_at, st, self._err, 512):
+            raise ClutorError(self._err.value.decode())
         return out
 
     def attention(self, q, pages: "KvPages", q_start, kv_len, *, max_q: int | None = None, scale: float | None = None,
@@ -439,128 +449,156 @@ class Context:
         keys and values (the new ones included) are in `pages`; max_q bounds the new rows of a sequence (default: T); scale
         defaults to head_dim ** -0.5. Returns [T, n_head, head_dim] (`out`, or a new tensor of out_dtype, by default q's type);
         asynchronous. The call's workspace is allocated for the stream, so calls may overlap."""
-        import torch
-        st = _torch_stream(stream, self.device)
-        self._tensors(pages=pages.k, q=q, q_start=q_start, kv_len=kv_len, out=out)
         T, H, D = q.shape
         if D != pages.head_dim or q.dtype != pages.k.dtype:
             raise ClutorError(f"q {tuple(q.shape)} of {q.dtype} does not fit a {pages.k.dtype} cache of head_dim {pages.head_dim}")
-        out = _out(out, (T, H, D), out_dtype or (out.dtype if out is not None else q.dtype), q.device, st, stream)
-        kv = pages.struct(q_start, kv_len)
-        a = AttnStruct(T, H, T if max_q is None else int(max_q), q.data_ptr(), _rows(q), out.data_ptr(), _dtype(out), _rows(out),
-                       D ** -0.5 if scale is None else scale, int(window), int(sinks), None, 0)
-        n = lib().clb200_attention_work(self.handle, C.byref(kv), C.byref(a))
-        if n:
-            work = _empty(n, torch.uint8, q.device, st, stream)
-            a.work, a.work_bytes = work.data_ptr(), n
-        self._check(lib().clb200_attention(self.handle, C.byref(kv), C.byref(a), st.cuda_stream or CUDA_STREAM_LEGACY,
-                                           self._err, 512))
+        self._on_device(pages.k, q, q_start, kv_len, out)
+        st = self._raw_stream(stream)
+        if out is None:
+            out = _empty((T, H, D), out_dtype or q.dtype, q.device, stream)
+        elif out.shape != (T, H, D) or (out_dtype is not None and out.dtype != out_dtype):
+            raise ClutorError(f"out must be {[T, H, D]} of {out_dtype or out.dtype}")
+        pages.pack(self._kv, q_start, kv_len)
+        if max_q is None:
+            max_q = T
+        # the workspace depends on the heads, their size and whether few or many rows share a key/value head
+        size = self._work_bytes.get((H, pages.n_kv, D, max_q))
+        args = (T, H, max_q, q.data_ptr(), _rows(q), out.data_ptr(), _dtype(out.dtype), _rows(out), D ** -0.5 if scale is None else scale, window, sinks)
+        if size is None:
+            _ATTN.pack_into(self._args, 0, *args, 0, 0)
+            size = lib().clb200_attention_work(self.handle, self._kv_at, self._args_at)
+            self._work_bytes[(H, pages.n_kv, D, max_q)] = size
+        work = _empty(size, _torch().uint8, q.device, stream) if size else None   # 0: the call says what is wrong
+        _ATTN.pack_into(self._args, 0, *args, work.data_ptr() if size else 0, size)
+        if self._c_attention(self.handle, self._kv_at, self._args_at, st, self._err, 512):
+            self._work_bytes.pop((H, pages.n_kv, D, max_q), None)
+            raise ClutorError(self._err.value.decode())
         return out
 
     def sample(self, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, *, token=None, prob=None, stream=None):
         """clb200_sample on torch CUDA tensors: one token for each row of logits [rows, vocab] (float32, float16 or bfloat16)
         from u [rows] float32 in [0, 1) and, each None or [rows], temperature, top_p, min_p (float32) and top_k (int32).
         Returns (token [rows] int32, prob [rows] float32); asynchronous."""
-        import torch
-        st = _torch_stream(stream, self.device)
-        self._tensors(logits=logits, u=u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, token=token, prob=prob)
         R, V = logits.shape
-        if V > 1 and logits.stride(1) != 1:
+        step, along = logits.stride()
+        if V > 1 and along != 1:
             raise ClutorError("a row's logits must lie next to one another")
-        f32, i32 = torch.float32, torch.int32
-        for name, t, d in (("u", u, f32), ("temperature", temperature, f32), ("top_k", top_k, i32), ("top_p", top_p, f32),
-                           ("min_p", min_p, f32), ("token", token, i32), ("prob", prob, f32)):
+        self._on_device(logits, u, temperature, top_k, top_p, min_p, token, prob)
+        f32, i32 = _torch().float32, _torch().int32
+        for t, d in ((u, f32), (temperature, f32), (top_k, i32), (top_p, f32), (min_p, f32), (token, i32), (prob, f32)):
             if t is not None and (t.dtype != d or t.shape != (R,) or not t.is_contiguous()):
-                raise ClutorError(f"{name} must be a contiguous {d} tensor of {R} elements")
+                raise ClutorError(f"u, temperature, top_p, min_p, prob (float32) and top_k, token (int32) must be contiguous tensors "
+                                  f"of {R} elements: got {d} wanted, {t.dtype} {tuple(t.shape)}")
+        st = self._raw_stream(stream)
         if token is None:
-            token = _empty(R, i32, logits.device, st, stream)
+            token = _empty(R, i32, logits.device, stream)
         if prob is None:
-            prob = _empty(R, f32, logits.device, st, stream)
-        a = SamplingStruct(R, V, _dtype(logits), logits.data_ptr(), logits.stride(0), u.data_ptr(), _ptr(temperature), _ptr(top_k),
-                           _ptr(top_p), _ptr(min_p), token.data_ptr(), prob.data_ptr())
-        self._check(lib().clb200_sample(self.handle, C.byref(a), st.cuda_stream or CUDA_STREAM_LEGACY, self._err, 512))
+            prob = _empty(R, f32, logits.device, stream)
+        _SAMPLING.pack_into(self._args, 0, R, V, _dtype(logits.dtype), logits.data_ptr(), step, u.data_ptr(),
+                            0 if temperature is None else temperature.data_ptr(), 0 if top_k is None else top_k.data_ptr(),
+                            0 if top_p is None else top_p.data_ptr(), 0 if min_p is None else min_p.data_ptr(), token.data_ptr(),
+                            prob.data_ptr())
+        if self._c_sample(self.handle, self._args_at, st, self._err, 512):
+            raise ClutorError(self._err.value.decode())
         return token, prob
 
-    def _tensors(self, **given) -> None:
+    def _on_device(self, *tensors) -> None:
         """Raises unless every tensor given lies on this context's device."""
-        for name, t in given.items():
-            if t is not None and (not t.is_cuda or t.device.index != self.device):
-                raise ClutorError(f"{name} is on {t.device}, the context on cuda:{self.device}")
+        d = self.device
+        for t in tensors:
+            if t is not None and t.get_device() != d:
+                raise ClutorError(f"a tensor is on {t.device}, the context on cuda:{d}")
+
+    def _raw_stream(self, stream) -> int:
+        """The cudaStream_t of a torch stream, or of the device's current one."""
+        if stream is None:
+            st = _torch()._C._cuda_getCurrentRawStream(self.device)
+        else:
+            st = stream.cuda_stream
+        return st or CUDA_STREAM_LEGACY
 
 
-def _torch_stream(stream, device: int):
-    import torch
-    return torch.cuda.current_stream(device) if stream is None else stream
+# the argument structs above as byte layouts: packing one into a buffer that a context keeps costs a third of making a
+# ctypes structure, and these calls are made once a layer of every token
+_KV = struct.Struct("@PPIiiiiqqqPiiiPP0q")
+_QK = struct.Struct("@iiIPPPqqqiPPfPiiPq0q")
+_ATTN = struct.Struct("@iiiPqPIqfiiPN0q")
+_SAMPLING = struct.Struct("@iiIPqPPPPPPP0q")
+_torch_module = None
 
 
-def _empty(shape, dtype, device, st, stream):
-    """A new tensor whose memory belongs to the stream `st` (given as `stream`, or the current one if that is None)."""
-    import torch
+def _torch():
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+        _TYPES.update({torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16})
+    return _torch_module
+
+
+def _empty(shape, dtype, device, stream):
+    """A new tensor whose memory belongs to `stream`, or to the current stream if that is None."""
+    torch = _torch()
     if stream is None:
         return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(st):
+    with torch.cuda.stream(stream):
         return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _out(out, shape, dtype, device, st, stream):
-    if out is None:
-        return _empty(shape, dtype, device, st, stream)
-    if out.shape != shape or out.dtype != dtype:
-        raise ClutorError(f"out must be {list(shape)} of {dtype}")
-    return out
+_TYPES: dict = {}
 
 
-def _dtype(t) -> int:
-    """The ggml type id of a tensor's type."""
-    import torch
-    d = t.dtype
-    if d is torch.float32:
-        return T_F32
-    if d is torch.float16:
-        return T_F16
-    if d is torch.bfloat16:
-        return T_BF16
-    raise ClutorError(f"{d} is not float32, float16 or bfloat16")
+def _dtype(d) -> int:
+    """The ggml type id of a torch type."""
+    t = _TYPES.get(d)
+    if t is None:
+        _torch()
+        t = _TYPES.get(d)
+        if t is None:
+            raise ClutorError(f"{d} is not float32, float16 or bfloat16")
+    return t
 
 
 def _rows(t) -> int:
     """The stride of a [T, heads, head_dim] tensor's rows; the heads of a row must follow one another."""
+    a, b, c = t.stride()
     T, H, D = t.shape
-    st = t.stride()
-    if st[2] != 1 or (H > 1 and st[1] != D):
-        raise ClutorError(f"the heads of a row must follow one another (strides {st} of {tuple(t.shape)})")
-    return st[0] if T > 1 else max(st[0], H * D)
+    if c != 1 or (b != D and H > 1):
+        raise ClutorError(f"the heads of a row must follow one another (strides {t.stride()} of {tuple(t.shape)})")
+    return a if T > 1 else max(a, H * D)
 
 
 class KvPages:
     """A paged key/value cache on the device (clb200_kv): k and v [n_pages, page_size, n_kv, head_dim] float16 or bfloat16 (the
     same strides, head_dim contiguous), table [n_seq, width] int32: the pages of each sequence in order."""
 
+    __slots__ = ("k", "v", "table", "n_pages", "page_size", "n_kv", "head_dim", "_fixed")
+
     def __init__(self, k, v, table):
-        import torch
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride() or k.stride(3) != 1:
+        torch = _torch()
+        strides = k.stride()
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or strides != v.stride() or strides[3] != 1:
             raise ClutorError("k and v must be [n_pages, page_size, n_kv, head_dim] tensors of one type and layout")
         if k.dtype not in (torch.float16, torch.bfloat16):
             raise ClutorError(f"the cache is {k.dtype}: it must be float16 or bfloat16")
         if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
             raise ClutorError("table must be an int32 [n_seq, width] tensor")
-        if not k.is_cuda or v.device != k.device or table.device != k.device:
+        device = k.get_device()
+        if device < 0 or v.get_device() != device or table.get_device() != device:
             raise ClutorError("k, v and table must lie on one CUDA device")
         self.k, self.v, self.table = k, v, table
         self.n_pages, self.page_size, self.n_kv, self.head_dim = k.shape
+        n_seq, width = table.shape
+        self._fixed = (k.data_ptr(), v.data_ptr(), _dtype(k.dtype), self.n_pages, self.page_size, self.n_kv, self.head_dim, *strides[:3],
+                       table.data_ptr(), max(table.stride(0), width), width, n_seq)
 
-    def struct(self, q_start, kv_len) -> KvStruct:
-        """The clb200_kv of one call's sequences."""
-        import torch
-        k, t = self.k, self.table
-        n_seq, width = t.shape
-        if q_start.dtype != torch.int32 or kv_len.dtype != torch.int32 or q_start.shape != (n_seq + 1,) or kv_len.shape != (n_seq,) or \
+    def pack(self, buf, q_start, kv_len) -> None:
+        """The clb200_kv of one call's sequences, into buf."""
+        n_seq, i32 = self._fixed[-1], _torch().int32
+        if q_start.dtype != i32 or kv_len.dtype != i32 or q_start.shape != (n_seq + 1,) or kv_len.shape != (n_seq,) or \
                 not q_start.is_contiguous() or not kv_len.is_contiguous():
             raise ClutorError(f"q_start and kv_len must be contiguous int32 tensors of {n_seq + 1} and {n_seq} elements")
-        ps, ss, hs, _ = k.stride()
-        return KvStruct(k.data_ptr(), self.v.data_ptr(), T_F16 if k.dtype is torch.float16 else T_BF16, self.n_pages, self.page_size,
-                        self.n_kv, self.head_dim, ps, ss, hs, t.data_ptr(), max(t.stride(0), width), width, n_seq,
-                        q_start.data_ptr(), kv_len.data_ptr())
+        _KV.pack_into(buf, 0, *self._fixed, q_start.data_ptr(), kv_len.data_ptr())
 
 
 def backend() -> Backend:

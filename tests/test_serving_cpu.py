@@ -142,3 +142,13 @@ def test_plain_rotation_known_answers():
     assert np.allclose(y, [[-4, 3, 0, 0]])           # the pair (0, 1)
     y, _ = ref.qk_rope(x, np.full(4, 2.0), np.array([1.0, 1.0, 0.0, 0.0]), 2, False, 0)
     assert np.allclose(y, np.array([[3, 4, 0, 0]]) / 2.5 * 2)
+
+
+def test_packed_layouts_equal_the_structs():
+    """The byte layouts that the Python calls pack are those of the C structs, field for field."""
+    for S, layout in ((cb.KvStruct, cb._KV), (cb.QkStruct, cb._QK), (cb.AttnStruct, cb._ATTN), (cb.SamplingStruct, cb._SAMPLING)):
+        assert C.sizeof(S) == layout.size
+        values = [float(i + 1) if t is C.c_float else i + 1 for i, (_, t) in enumerate(S._fields_)]
+        buf = C.create_string_buffer(layout.size)
+        layout.pack_into(buf, 0, *values)
+        assert [getattr(S.from_buffer_copy(buf), f) for f, _ in S._fields_] == values
