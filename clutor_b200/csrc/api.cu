@@ -396,6 +396,7 @@ int clb200_set_option(clb200_ctx *c, int option, int value) {
     case CLB200_OPT_TEST_SPECULATION_MISS: c->force_miss = value != 0; ++c->graph_gen; return 0;
     case CLB200_OPT_TEST_STALL_WAIT: if (value < 0) return 1; c->stall_wait = static_cast<uint32_t>(value); ++c->graph_gen; return 0;
     case CLB200_OPT_COOPERATIVE: c->cooperative = value != 0; ++c->graph_gen; return 0;
+    case CLB200_OPT_PROMPT_ATTENTION: if (value < 0 || value > 1) return 1; c->prompt_attention = value != 0; return 0;
     default: return 1;
   }
 }

@@ -38,9 +38,18 @@ struct clb200_model {
   int pf_cap = 64;                 // tokens per batch: the reference's batch for a model in memory (c/src/forward.c:1048)
   int pf_alloc = 0;                // the batch the buffers below hold
   uint8_t *pf = nullptr;           // device: tokens, X, Q, K, V, rotated Q, attention, Q8_K activations
+  // the paged attention of the prompt path (CLB200_OPT_PROMPT_ATTENTION): a page table that names the cache's positions in
+  // order, one sequence's first rows and length, the operator's workspace
+  int *pg = nullptr;               // device: [0, 1] the rows, [2] the length, [4 ..] the table
+  uint8_t *pg_work = nullptr;
+  size_t pg_work_bytes = 0;
+  // sampled generation: u, then the probabilities [ctx] each, then temperature, top-k, top-p, min-p
+  float *sp = nullptr;
 };
 
 namespace {
+
+constexpr int MODEL_PAGE = 64;   // positions per page where a layer's cache is read as pages
 
 struct ArchSpec {
   const char *name;
@@ -201,7 +210,9 @@ static int model_setup(clb200_model *m, const Gguf &g, int n_ctx, char *err, siz
   // key/value cache and scratch
   const size_t kv_elems = static_cast<size_t>(a.n_layer) * a.ctx * a.n_kvw;
   auto take = [&](size_t bytes) { total = al(total, 256); const size_t at = total; total += bytes + 64; return at; };
-  const size_t o_kc = take(kv_elems * 2), o_vc = take(kv_elems * 2);
+  // (behind the last position, room for the rest of a page: the paged attention's copies read whole pages)
+  const size_t kv_rest = static_cast<size_t>(MODEL_PAGE) * a.n_kvw * 2;
+  const size_t o_kc = take(kv_elems * 2 + kv_rest), o_vc = take(kv_elems * 2 + kv_rest);
   const size_t o_x = take(a.E * 4), o_qkv = take((a.n_q + 2 * a.n_kvw) * 4), o_att = take(a.n_q * 4);
   const size_t o_rl = take(a.NE * 4), o_hg = take(static_cast<size_t>(a.K) * a.FF * 4), o_lg = take(static_cast<size_t>(a.vocab) * 4);
   const size_t o_rs = take(static_cast<size_t>(a.n_layer) * a.K * 4), o_rw = take(static_cast<size_t>(a.n_layer) * a.K * 4);
@@ -411,6 +422,9 @@ void clb200_model_close(clb200_model *m) {
   if (m->st_host) cudaFreeHost(m->st_host);
   if (m->route_host) cudaFreeHost(m->route_host);
   if (m->pf) cudaFree(m->pf);
+  if (m->pg) cudaFree(m->pg);
+  if (m->pg_work) cudaFree(m->pg_work);
+  if (m->sp) cudaFree(m->sp);
   if (m->stream) cudaStreamDestroy(m->stream);
   delete m;
 }
@@ -512,6 +526,58 @@ int clb200_model_generate(clb200_model *m, int token, int n, int *tokens_out, ch
   return 0;
 }
 
+int clb200_model_generate_sampled(clb200_model *m, int token, int n, const float *u, float temperature, int top_k, float top_p, float min_p,
+                                  int *tokens_out, float *probs_out, char *err, size_t errlen) {
+  if (!m) { errf(err, errlen, "no model"); return 1; }
+  const FwdArgs &a = m->args;
+  if (n < 1) return 0;
+  if (!u) { errf(err, errlen, "no random numbers"); return 1; }
+  if (token < 0 || token >= a.vocab) { errf(err, errlen, "token %d is outside the vocabulary", token); return 1; }
+  if (n > a.ctx - m->pos) { errf(err, errlen, "%d more tokens do not fit the context (%d of %d used)", n, m->pos, a.ctx); return 1; }
+  cudaSetDevice(m->device);
+  const size_t C = static_cast<size_t>(a.ctx);
+  if (!m->sp) CUDA_OR(cudaMalloc(&m->sp, (2 * C + 4) * 4), "allocating the sampling buffers");
+  const int start = m->pos;
+  float how[4] = {temperature, 0.f, top_p, min_p};
+  std::memcpy(how + 1, &top_k, 4);
+  CUDA_OR(cudaMemcpyAsync(m->sp, u, static_cast<size_t>(n) * 4, cudaMemcpyHostToDevice, m->stream), "random numbers upload");
+  CUDA_OR(cudaMemcpyAsync(m->sp + 2 * C, how, sizeof how, cudaMemcpyHostToDevice, m->stream), "settings upload");
+  FwdState s{};
+  s.token = token;
+  s.pos = start;
+  *m->st_host = s;
+  CUDA_OR(cudaMemcpyAsync(a.st, m->st_host, sizeof(FwdState), cudaMemcpyHostToDevice, m->stream), "state upload");
+  FwdArgs g = a;
+  g.feed = 0;
+  g.trace = nullptr;
+  g.force_miss = m->ctx->force_miss;
+  clb200_sampling sp{};
+  sp.rows = 1;
+  sp.vocab = a.vocab;
+  sp.type = T_F32;
+  sp.logits = a.logits;
+  sp.stride = a.vocab;
+  sp.temperature = m->sp + 2 * C;
+  sp.top_k = reinterpret_cast<const int *>(m->sp + 2 * C + 1);
+  sp.top_p = m->sp + 2 * C + 2;
+  sp.min_p = m->sp + 2 * C + 3;
+  for (int i = 0; i < n; ++i) {   // a step, the draw from its logits, the draw as the next token
+    CUDA_OR(fwd_launch(g, m->ctas, m->stream), "launching the step");
+    sp.u = m->sp + i;
+    sp.token = a.gen_out + start + i;
+    sp.prob = m->sp + C + i;
+    if (clb200_sample(m->ctx, &sp, m->stream, err, errlen)) return 1;
+    CUDA_OR(pf_feed(a.st, a.gen_out + start + i, m->stream), "feeding the token");
+  }
+  CUDA_OR(cudaMemcpyAsync(m->st_host, a.st, sizeof(FwdState), cudaMemcpyDeviceToHost, m->stream), "state download");
+  if (tokens_out) CUDA_OR(cudaMemcpyAsync(tokens_out, a.gen_out + start, static_cast<size_t>(n) * 4, cudaMemcpyDeviceToHost, m->stream), "tokens download");
+  if (probs_out) CUDA_OR(cudaMemcpyAsync(probs_out, m->sp + C, static_cast<size_t>(n) * 4, cudaMemcpyDeviceToHost, m->stream), "probabilities download");
+  CUDA_OR(cudaStreamSynchronize(m->stream), "generating");
+  if (m->st_host->err) { errf(err, errlen, "device error %d: %s", m->st_host->err, fwd_error_text(m->st_host->err)); return 1; }
+  m->pos = start + n;
+  return 0;
+}
+
 int clb200_model_generate_async(clb200_model *m, int token, int n, void *stream, char *err, size_t errlen) {
   // the same replay on a caller's stream with no host synchronisation (for timing); tokens via clb200_model_tokens
   if (!m) { errf(err, errlen, "no model"); return 1; }
@@ -587,6 +653,7 @@ static int prefill_batch(clb200_model *m, const int *tokens, int nb, float *logi
   const PfBufs b = pf_layout(a, m->pf_alloc, m->pf);
   int *errw = m->ctx->small;
   CUDA_OR(cudaMemcpyAsync(b.tok, tokens, static_cast<size_t>(nb) * 4, cudaMemcpyHostToDevice, st), "tokens upload");
+  if (m->ctx->prompt_attention) PF_OR(pf_rows(m->pg, nb, pos0 + nb, st), "the batch's rows");
   PF_OR(pf_embed(a.tok_embd, b.tok, nb, E, a.embed_scale, b.X, st), "the embedding");
   for (int l = 0; l < a.n_layer; ++l) {
     const FwdLayer &y = m->hl[static_cast<size_t>(l)];
@@ -602,10 +669,43 @@ static int prefill_batch(clb200_model *m, const int *tokens, int nb, float *logi
     PF_OR(dense(y.wq, NQ, E, b.Q, 0, 1.f), "the Q product");
     PF_OR(dense(y.wk, KW, E, b.K, 0, 1.f), "the K product");
     PF_OR(dense(y.wv, KW, E, b.V, 0, 1.f), "the V product");
-    PfQkArgs qa{b.Q, b.K, b.V, b.Qr, y.qn, y.kn, kc, vc, a.rope_cs, nb, pos0, a.n_head, a.n_kv, a.hd, a.qk_mode, a.rope_pairs, a.eps};
-    PF_OR(pf_qk(qa, st), "QK-norm and rotation");
-    PfAttnArgs aa{b.Qr, kc, vc, b.att, nb, pos0, a.n_head, a.n_kv, a.hd, KW, a.attn_scale};
-    PF_OR(pf_attn(aa, st), "the attention");
+    if (m->ctx->prompt_attention) {   // the serving operators, the layer's cache read as pages in order
+      clb200_kv kv{};
+      kv.k = kc;
+      kv.v = vc;
+      kv.type = T_F16;
+      kv.n_pages = (a.ctx + MODEL_PAGE - 1) / MODEL_PAGE;
+      kv.page_size = MODEL_PAGE;
+      kv.n_kv = a.n_kv;
+      kv.head_dim = a.hd;
+      kv.page_stride = static_cast<int64_t>(MODEL_PAGE) * KW;
+      kv.slot_stride = KW;
+      kv.head_stride = a.hd;
+      kv.table = m->pg + 4;
+      kv.table_stride = kv.table_width = kv.n_pages;
+      kv.n_seq = 1;
+      kv.q_start = m->pg;
+      kv.kv_len = m->pg + 2;
+      clb200_qk qk{nb, a.n_head, T_F32, b.Q, b.K, b.V, NQ, KW, KW, a.qk_mode, y.qn, y.kn, a.eps, a.rope_cs, a.ctx, a.rope_pairs, b.Qr, NQ};
+      if (clb200_qk_rope(m->ctx, &kv, &qk, st, err, errlen)) return 1;
+      clb200_attn at{nb, a.n_head, nb, b.Qr, NQ, b.att, T_F32, NQ, a.attn_scale, 0, 0, m->pg_work, m->pg_work_bytes};
+      const size_t need = clb200_attention_work(m->ctx, &kv, &at);
+      if (need > m->pg_work_bytes) {
+        CUDA_OR(cudaStreamSynchronize(st), "waiting for the device");
+        if (m->pg_work) cudaFree(m->pg_work);
+        m->pg_work = nullptr;
+        m->pg_work_bytes = 0;
+        CUDA_OR(cudaMalloc(&m->pg_work, need), "allocating the attention's workspace");
+        at.work = m->pg_work;
+        at.work_bytes = m->pg_work_bytes = need;
+      }
+      if (clb200_attention(m->ctx, &kv, &at, st, err, errlen)) return 1;
+    } else {
+      PfQkArgs qa{b.Q, b.K, b.V, b.Qr, y.qn, y.kn, kc, vc, a.rope_cs, nb, pos0, a.n_head, a.n_kv, a.hd, a.qk_mode, a.rope_pairs, a.eps};
+      PF_OR(pf_qk(qa, st), "QK-norm and rotation");
+      PfAttnArgs aa{b.Qr, kc, vc, b.att, nb, pos0, a.n_head, a.n_kv, a.hd, KW, a.attn_scale};
+      PF_OR(pf_attn(aa, st), "the attention");
+    }
     PF_OR(pf_q8k(b.att, nb, NQ, b.qs, b.dd, b.bs, st), "quantizing the attention");
     PF_OR(dense(y.wo, E, NQ, b.X, 1, a.resid_scale), "the O product");
     // the mixture of experts over the batch (c/src/forward.c:1131-1210): the batched kernels
@@ -639,13 +739,19 @@ int clb200_model_prefill(clb200_model *m, const int *tokens, int n, float *logit
   if (m->pos + n > a.ctx) { errf(err, errlen, "the context is full (%d tokens)", a.ctx); return 1; }
   for (int i = 0; i < n; ++i)
     if (tokens[i] < 0 || tokens[i] >= a.vocab) { errf(err, errlen, "token %d is outside the vocabulary", tokens[i]); return 1; }
-  if (m->pos + n > PF_MAX_CTX) { errf(err, errlen, "the batched prompt path takes at most %d positions", PF_MAX_CTX); return 1; }
+  if (m->pos + n > PF_MAX_CTX && !m->ctx->prompt_attention) { errf(err, errlen, "the batched prompt path takes at most %d positions", PF_MAX_CTX); return 1; }
   cudaSetDevice(m->device);
   const int cap = m->pf_cap;
   if (n > 1 && m->pf_alloc < cap) {
     if (m->pf) { CUDA_OR(cudaStreamSynchronize(m->stream), "waiting for the device"); cudaFree(m->pf); m->pf = nullptr; m->pf_alloc = 0; }
     CUDA_OR(cudaMalloc(&m->pf, pf_layout(a, cap, nullptr).total), "allocating the batched prompt buffers");
     m->pf_alloc = cap;
+  }
+  if (n > 1 && m->ctx->prompt_attention && !m->pg) {
+    std::vector<int> pg(4 + static_cast<size_t>(a.ctx + MODEL_PAGE - 1) / MODEL_PAGE, 0);
+    for (size_t i = 4; i < pg.size(); ++i) pg[i] = static_cast<int>(i) - 4;
+    CUDA_OR(cudaMalloc(&m->pg, pg.size() * 4), "allocating the page table");
+    CUDA_OR(cudaMemcpy(m->pg, pg.data(), pg.size() * 4, cudaMemcpyHostToDevice), "page table upload");
   }
   for (int i = 0; i < n; i += cap) {   // batches of cap tokens; a batch of one is a step (c/src/forward.c:1263-1266)
     const int nb = std::min(cap, n - i);

@@ -374,6 +374,14 @@ __global__ void counts_kernel(int *co, int nb) {
   co[2] = nb;
 }
 
+__global__ void rows_kernel(int *pg, int rows, int kv) {
+  pg[0] = 0;
+  pg[1] = rows;
+  pg[2] = kv;
+}
+
+__global__ void feed_kernel(FwdState *state, const int *token) { state->token = state->next = *token; }
+
 __global__ void resid_add_kernel(float *x, const float *v, size_t n, float scale) {
   for (size_t i = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < n; i += static_cast<size_t>(gridDim.x) * blockDim.x)
     x[i] = __fadd_rn(x[i], __fmul_rn(scale, v[i]));
@@ -415,6 +423,16 @@ int pf_mv(const FwdMat &m, int rows, int cols, int nb, const int8_t *qs, const f
   const dim3 grid((rows + MT_ROWS - 1) / MT_ROWS, (nb + MT_TOK - 1) / MT_TOK);
   mvt_kernel<<<grid, MT_THREADS, L.total, st>>>(m.p, m.type, m.rb, rows, cols, nb, qs, dd, bs, out, accum, scale, err);
   return static_cast<int>(cudaGetLastError());
+}
+
+cudaError_t pf_rows(int *pg, int rows, int kv, cudaStream_t st) {
+  rows_kernel<<<1, 1, 0, st>>>(pg, rows, kv);
+  return cudaGetLastError();
+}
+
+cudaError_t pf_feed(FwdState *state, const int *token, cudaStream_t st) {
+  feed_kernel<<<1, 1, 0, st>>>(state, token);
+  return cudaGetLastError();
 }
 
 cudaError_t pf_embed(const FwdMat &emb, const int *tok, int nb, int E, float embed_scale, float *X, cudaStream_t st) {

@@ -45,6 +45,11 @@ struct PfAttnArgs {
 };
 cudaError_t pf_attn(const PfAttnArgs &a, cudaStream_t st);
 
+// For the paged attention of a batch: pg[0, 1] = 0, rows (its first rows) and pg[2] = kv (the sequence's length with it).
+cudaError_t pf_rows(int *pg, int rows, int kv, cudaStream_t st);
+// The token that a draw chose becomes the next step's and the last step's choice.
+cudaError_t pf_feed(FwdState *state, const int *token, cudaStream_t st);
+
 // A dense product of a batch, out [nb][rows] (= or += scale *) m [rows][cols] times plain Q8_K activations: a CTA per 32
 // rows and 32 tokens for batches of 8 or more tokens, else the product kernel of backend.cu. Returns a CUDA error code.
 int pf_mv(const FwdMat &m, int rows, int cols, int nb, const int8_t *qs, const float *dd, const int16_t *bs, float *out, int accum,

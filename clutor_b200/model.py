@@ -30,6 +30,8 @@ def _bind(L) -> None:
                                     C.c_size_t]
     L.clb200_model_generate.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_char_p, C.c_size_t]
     L.clb200_model_generate_async.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_char_p, C.c_size_t]
+    L.clb200_model_generate_sampled.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_float, C.c_int, C.c_float, C.c_float,
+                                                C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]
     L.clb200_model_tokens.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_char_p, C.c_size_t]
     L.clb200_model_prefill.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_char_p, C.c_size_t]
     L.clb200_model_set_batch.argtypes = [C.c_void_p, C.c_int]
@@ -104,6 +106,19 @@ class Model:
         if self.L.clb200_model_generate(self.h, token, n, out.ctypes.data, self._err, 512):
             raise ClutorError(self._err.value.decode())
         return out.tolist()
+
+    def generate_sampled(self, token: int, n: int, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                         min_p: float = 0.0):
+        """Sampled generation on the device (clb200_model_generate_sampled): feeds `token`, then each drawn token, u [n] the random
+        numbers in [0, 1). Returns (the n tokens, their probabilities)."""
+        u = np.ascontiguousarray(u, np.float32)
+        if u.shape != (n,):
+            raise ClutorError(f"{n} tokens take {n} random numbers, got {u.shape}")
+        out, probs = np.zeros(n, np.int32), np.zeros(n, np.float32)
+        if self.L.clb200_model_generate_sampled(self.h, token, n, u.ctypes.data, temperature, top_k, top_p, min_p, out.ctypes.data,
+                                                probs.ctypes.data, self._err, 512):
+            raise ClutorError(self._err.value.decode())
+        return out.tolist(), probs.tolist()
 
     def generate_async(self, token: int, n: int, stream: int = 0) -> None:
         if self.L.clb200_model_generate_async(self.h, token, n, C.c_void_p(stream) if stream else None, self._err, 512):

@@ -96,8 +96,12 @@ int clb200_moe_ffn_dev(clb200_ctx *c, int layer, float *x, int T, int *sel, floa
  *   CLB200_OPT_COOPERATIVE: 1 (default): the one-token kernels are launched cooperatively, so the driver places every CTA
  *     at once or refuses the launch (their CTAs wait on one another). 0: plain launches, one CTA per SM, which costs less per
  *     launch; for hosts that own the whole device (no other kernel can hold an SM while a launch starts). Either way a CTA
- *     that waits too long ends the launch with a device error, not a hang. */
-enum { CLB200_OPT_DECODE_KERNEL = 1, CLB200_OPT_TEST_SPECULATION_MISS = 2, CLB200_OPT_TEST_STALL_WAIT = 3, CLB200_OPT_COOPERATIVE = 4 };
+ *     that waits too long ends the launch with a device error, not a hang.
+ *   CLB200_OPT_PROMPT_ATTENTION: which attention clb200_model_prefill runs in batches of two or more tokens. 0 (default): the
+ *     reference's float order, on prompts of up to 32768 positions. 1: clb200_qk_rope and clb200_attention on the model's
+ *     cache (tensor cores, queries and probabilities in half precision; any length that fits the context). */
+enum { CLB200_OPT_DECODE_KERNEL = 1, CLB200_OPT_TEST_SPECULATION_MISS = 2, CLB200_OPT_TEST_STALL_WAIT = 3, CLB200_OPT_COOPERATIVE = 4,
+       CLB200_OPT_PROMPT_ATTENTION = 5 };
 int clb200_set_option(clb200_ctx *c, int option, int value);
 /* No counterpart in the reference: an entry point for hosts that cannot allocate device memory once they run (their
  * device memory is carved out up front by another allocator, or cudaMalloc's device-wide synchronisation would break a
@@ -466,6 +470,12 @@ int clb200_model_generate(clb200_model *m, int token, int n, int *tokens_out, ch
 /* The same n steps queued on `stream` (NULL: the model's own) without waiting, after one clb200_model_generate; read the
  * tokens of positions [start, start + n) afterwards with clb200_model_tokens. */
 int clb200_model_generate_async(clb200_model *m, int token, int n, void *stream, char *err, size_t errlen);
+/* Sampled generation: feeds `token`, then n times the token that clb200_sample draws from the step's logits with u[i] (host, n
+ * numbers in [0, 1)) and one setting of temperature, top-k, top-p and min-p (the values that leave a filter out included);
+ * tokens_out and probs_out (host, n; either may be NULL) receive the tokens and their probabilities. Temperature 0 gives
+ * clb200_model_generate's tokens. */
+int clb200_model_generate_sampled(clb200_model *m, int token, int n, const float *u, float temperature, int top_k, float top_p, float min_p,
+                                  int *tokens_out, float *probs_out, char *err, size_t errlen);
 int clb200_model_tokens(clb200_model *m, int start, int n, int *tokens_out, char *err, size_t errlen);
 /* cl_fwd_prefill (forward.h:121, c/src/forward.c:1256-1282): feeds n tokens at the current position in batches (run_std,
  * :1078-1225): every dense matrix is multiplied with the whole batch, each token routes as it would alone and each chosen
