@@ -38,16 +38,6 @@ CLB_DEV void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename C>
-CLB_DEV uint32_t pack2(float a, float b) {   // a in the low half
-  if constexpr (__is_same(C, __half)) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-  }
-}
 // Byte offset of 16-byte chunk c of row r in rows of HD half-precision elements; eight rows' equal chunks in eight bank groups.
 template <int HD>
 CLB_DEV uint32_t chunk_at(int r, int c) { return static_cast<uint32_t>(r * HD * 2 + ((c ^ (r & 7)) << 4)); }

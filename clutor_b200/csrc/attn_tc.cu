@@ -74,19 +74,6 @@ CLB_DEV float2 exp2_poly(float2 x) {
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 
-template <typename C>
-CLB_DEV uint32_t pack_pair(float a, float b) {   // a in the low half
-  if constexpr (__is_same(C, __half)) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-  } else if constexpr (__is_same(C, float)) {
-    return 0;
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-  }
-}
-
 // What the roles need to know of an item; n 0: the run has ended.
 struct __align__(16) TcItem {
   int n, i0, sinks, start;     // this CTA's tiles [i0, i0 + n) of the item; tile i is i below sinks, else start + i
@@ -395,7 +382,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
             }
             if (i & 1) l1 = fadd2(l1, e);
             else l0 = fadd2(l0, e);
-            p[i] = pack_pair<C>(e.x, e.y);
+            p[i] = pack2<C>(e.x, e.y);
           }
           if constexpr (N == 128) tc::st_x32(s_col + 32 * h, p);
           else tc::st_x16(s_col + 16 * h, reinterpret_cast<const uint32_t(&)[16]>(p));
@@ -440,7 +427,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
           tc::wait_ld_x32(o);
           tc::wait_ld_x32(o + 32);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) u[i] = pack_pair<O>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+          for (int i = 0; i < 32; ++i) u[i] = pack2<O>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
           pass(u, c, false);
         }
       } else {

@@ -1,6 +1,7 @@
 // clb200_qk_rope: norms of queries and keys, rotation by position, and the store of keys and values into a paged cache, one
 // pass over the new tokens' rows.
 #include <algorithm>
+#include <type_traits>
 
 #include "ctx.cuh"
 #include "serve.cuh"
@@ -17,143 +18,196 @@ struct QkArgs {
   int *err;
 };
 
-// Eight consecutive elements as floats, and eight floats rounded to the cache's type.
+// Four consecutive elements as they lie in memory, as floats, and rounded to the cache's type.
 template <typename S>
-CLB_DEV void load8(const S *p, float (&x)[8]) {
-  if constexpr (sizeof(S) == 4) {
-    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  } else {
-    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+struct Raw4 {
+  using W = typename std::conditional<sizeof(S) == 4, uint4, uint2>::type;
+  W v;
+  CLB_DEV void load(const S *p) { v = *reinterpret_cast<const W *>(p); }
+  CLB_DEV void get(float *x) const {
     const S *h = reinterpret_cast<const S *>(&v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(h[i]);
+    for (int i = 0; i < 4; ++i) x[i] = to_f32(h[i]);
   }
+};
+CLB_DEV void load4(const float *p, float *x) {
+  const float4 v = *reinterpret_cast<const float4 *>(p);
+  x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
 }
 template <typename C>
-CLB_DEV void store8(C *p, const float (&x)[8]) {
-  uint4 v;
-  C *h = reinterpret_cast<C *>(&v);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) h[i] = from_f32<C>(x[i]);
-  *reinterpret_cast<uint4 *>(p) = v;
+CLB_DEV void put4(C *p, const float *x) {
+  *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<C>(x[0], x[1]), pack2<C>(x[2], x[3]));
 }
 
-// One CTA per token. A head is held by HD / 8 lanes, eight consecutive elements each, so a warp takes 32 / (HD / 8) heads at
-// a time and a lane's rotary row and head weights stay the same from head to head.
-template <typename S, typename C, int HD>
-__global__ void __launch_bounds__(QT) qk_rope_kernel(const QkArgs g) {
-  constexpr int LPH = HD / 8, HPW = 32 / LPH;   // lanes per head, heads per warp
+// One token by WARPS warps (a CTA's eight, or one of them). A head is held by HD / 8 lanes, each four consecutive elements of its
+// first half and the same four of its second, so both rotations stay inside the lane, and a lane's rotary values and head
+// weights are the same from head to head; a warp takes 32 / (HD / 8) heads at a time.
+// The bound is memory: every element is read and written once. What stands in its way is latency, since where a token's few
+// kilobytes go hangs on a chain of look-ups (the sequence by bisection, its length, the page). The queries, whose place depends
+// on the row alone, are requested before it, HOLD rounds of heads a warp. With a CTA per token the chain is a token's whole
+// time; a warp per token has as many tokens in flight as an SM has warps, and pays off once there are tokens for them.
+// At 5 ragged prompts of 64 + 4 + 4 heads of 128, bf16 (231 MB): 46 us with a warp per token (5.0 TB/s), 70 with a CTA; 68 while
+// a lane held eight consecutive elements, half of whose partners came by shuffles (192 instructions a round, the issue rate then
+// being the limit).
+template <typename S, typename C, int HD, int WARPS>
+__global__ void __launch_bounds__(QT, WARPS == 1 ? 3 : 1) qk_rope_kernel(const QkArgs g) {
+  constexpr int LPH = HD / 8, HPW = 32 / LPH, ROUND = WARPS * HPW, HALF = HD / 2;   // lanes per head, heads per warp, heads per round
+  constexpr int HOLD = sizeof(S) == 4 ? 3 : 4;                                       // rounds whose loads are in flight at once
   __shared__ float red[2][QW];
   const clb200_qk &a = g.a;
   const clb200_kv &kv = g.kv;
-  const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5, part = WARPS == 1 ? lane : threadIdx.x;
+  const int row = WARPS == 1 ? blockIdx.x * QW + (threadIdx.x >> 5) : blockIdx.x;
+  if (row >= a.T) return;
+  const int H = a.n_head, KV = kv.n_kv, at = 4 * (lane % LPH), mine = warp * HPW + lane / LPH;   // the lane's elements, its first head
+  const S *q = static_cast<const S *>(a.q) + row * a.q_stride + at, *k = static_cast<const S *>(a.k) + row * a.k_stride + at;
+  Raw4<S> raw[HOLD][2];
+  auto fetch = [&](const S *p, int h0, int n) {   // HOLD rounds of n heads from h0 on
+#pragma unroll
+    for (int u = 0; u < HOLD; ++u) {
+      const int h = h0 + u * ROUND + mine;
+      if (h < n) {
+        raw[u][0].load(p + h * HD);
+        raw[u][1].load(p + h * HD + HALF);
+      }
+    }
+  };
+  fetch(q, 0, H);
   if (row < kv.q_start[0] || row >= kv.q_start[kv.n_seq]) return;   // a row behind the last sequence
   const int s = seq_of_row(kv.q_start, kv.n_seq, row);
   const int pos = kv.kv_len[s] - kv.q_start[s + 1] + row;
   if (pos < 0 || pos >= a.n_pos) {
-    if (threadIdx.x == 0) set_error(g.err, ERR_BAD_ROWS);
+    if (part == 0) set_error(g.err, ERR_BAD_ROWS);
     return;
   }
-  const int H = a.n_head, KV = kv.n_kv, li = lane % LPH;   // li: the lane's place in its head
-  const S *q = static_cast<const S *>(a.q) + row * a.q_stride, *k = static_cast<const S *>(a.k) + row * a.k_stride;
-  const S *v = static_cast<const S *>(a.v) + row * a.v_stride;
+  const int page = page_of(kv, s, pos, g.err);
+  // the cosines and sines of the lane's pairs: (i, i + HALF) for its four i, or (2i, 2i + 1), two in each half
+  const float *cs = a.rope + static_cast<int64_t>(pos) * HD;
+  float c[4], n[4], wq[8], wk[8];
+  if (a.pairs) {
+    const float2 c0 = *reinterpret_cast<const float2 *>(cs + at / 2), c1 = *reinterpret_cast<const float2 *>(cs + HALF / 2 + at / 2);
+    const float2 n0 = *reinterpret_cast<const float2 *>(cs + HALF + at / 2), n1 = *reinterpret_cast<const float2 *>(cs + HALF + HALF / 2 + at / 2);
+    c[0] = c0.x; c[1] = c0.y; c[2] = c1.x; c[3] = c1.y;
+    n[0] = n0.x; n[1] = n0.y; n[2] = n1.x; n[3] = n1.y;
+  } else {
+    load4(cs + at, c);
+    load4(cs + HALF + at, n);
+  }
+  if (a.norm == CLB200_QK_NORM_HEAD) {
+    load4(a.q_norm + at, wq);
+    load4(a.q_norm + HALF + at, wq + 4);
+    load4(a.k_norm + at, wk);
+    load4(a.k_norm + HALF + at, wk + 4);
+  }
   float qs = 1.f, ks = 1.f;
-  if (a.norm == CLB200_QK_NORM_ROW) {
-    float sq = 0.f, sk = 0.f, x[8];
-    for (int i = threadIdx.x; i < H * LPH; i += QT) {
-      load8(q + 8 * i, x);
+  if (WARPS > 1 && a.norm == CLB200_QK_NORM_ROW) {
+    auto squares = [&](const S *p, int heads) {
+      float t = 0.f;
+      for (int h0 = 0; h0 < heads; h0 += HOLD * ROUND) {
+        fetch(p, h0, heads);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sq = fmaf(x[e], x[e], sq);
-    }
-    for (int i = threadIdx.x; i < KV * LPH; i += QT) {
-      load8(k + 8 * i, x);
+        for (int u = 0; u < HOLD; ++u) {
+          if (h0 + u * ROUND + mine >= heads) continue;
+          float x[8];
+          raw[u][0].get(x);
+          raw[u][1].get(x + 4);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sk = fmaf(x[e], x[e], sk);
-    }
+          for (int e = 0; e < 8; ++e) t = fmaf(x[e], x[e], t);
+        }
+      }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) { sq += __shfl_xor_sync(FULL_MASK, sq, o); sk += __shfl_xor_sync(FULL_MASK, sk, o); }
-    if (lane == 0) { red[0][warp] = sq; red[1][warp] = sk; }
+      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(FULL_MASK, t, o);
+      return t;
+    };
+    const float tk = squares(k, KV), tq = squares(q, H);
+    if (lane == 0) { red[0][warp] = tq; red[1][warp] = tk; }
     __syncthreads();
-    sq = sk = 0.f;
+    float sq = 0.f, sk = 0.f;
     for (int w = 0; w < QW; ++w) { sq += red[0][w]; sk += red[1][w]; }
     qs = 1.0f / sqrtf(sq / static_cast<float>(H * HD) + a.eps);
     ks = 1.0f / sqrtf(sk / static_cast<float>(KV * HD) + a.eps);
+    if (H > HOLD * ROUND) fetch(q, 0, H);   // the first rounds' registers hold the last ones
   }
-  const int page = page_of(kv, s, pos, g.err);
-  const int64_t slot = page * kv.page_stride + (pos % kv.page_size) * kv.slot_stride;
-  // the lane's cosines and sines: its elements' pairs are (i, i + HD / 2), or (2i, 2i + 1) inside the lane
-  const float *cs = a.rope + static_cast<int64_t>(pos) * HD;
-  float c[8], n[8];
-  if (a.pairs) {
+  // the heads of p, HOLD rounds at a time: the first rounds are on their way already
+  auto turn = [&](const S *p, int heads, const float *norm, const float (&w)[8], float scale, C *dst, int64_t dst_stride, bool store) {
+    for (int h0 = 0; h0 < heads; h0 += HOLD * ROUND) {
+      if (h0) fetch(p, h0, heads);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { c[e] = cs[4 * li + e]; n[e] = cs[HD / 2 + 4 * li + e]; }
-  } else {
-    load8(cs + 8 * (li % (LPH / 2)), c);
-    load8(cs + HD / 2 + 8 * (li % (LPH / 2)), n);
-  }
-  const int hh = lane / LPH;
-  for (int h0 = warp * HPW; h0 < H + KV; h0 += QW * HPW) {
-    const int h = h0 + hh;
-    const bool live = h < H + KV, isk = h >= H;
-    const int head = isk ? h - H : h;
-    float x[8];
-    if (live) load8((isk ? k : q) + head * HD + 8 * li, x);
-    else
+      for (int u = 0; u < HOLD; ++u) {
+        if (h0 + u * ROUND + warp * HPW >= heads) break;   // none of the warp's
+        const int h = h0 + u * ROUND + mine;
+        float x[8], y[8];
+        raw[u][0].get(x);
+        raw[u][1].get(x + 4);
+        if (a.norm == CLB200_QK_NORM_HEAD) {
+          float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = 0.f;
-    if (a.norm != CLB200_QK_NORM_NONE) {
-      float scale = isk ? ks : qs;
-      if (a.norm == CLB200_QK_NORM_HEAD) {
-        float ss = 0.f;
+          for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+          for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(FULL_MASK, ss, o);
+          ss = rsqrtf(fmaf(ss, 1.0f / HD, a.eps));   // within 2^-22
 #pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(FULL_MASK, ss, o);
-        scale = 1.0f / sqrtf(ss * (1.0f / HD) + a.eps);
-      }
-      if (live) {
-        const float *wp = (isk ? a.k_norm : a.q_norm) + (a.norm == CLB200_QK_NORM_ROW ? head * HD : 0) + 8 * li;
-        float w[8];
-        load8(wp, w);
+          for (int e = 0; e < 8; ++e) x[e] *= ss * w[e];
+        } else if (WARPS > 1 && a.norm == CLB200_QK_NORM_ROW && h < heads) {
+          load4(norm + h * HD + at, y);
+          load4(norm + h * HD + HALF + at, y + 4);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * scale * w[e];
+          for (int e = 0; e < 8; ++e) x[e] *= scale * y[e];
+        }
+        if (a.pairs) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[2 * e] = fmaf(x[2 * e], c[e], -(x[2 * e + 1] * n[e]));
+            y[2 * e + 1] = fmaf(x[2 * e], n[e], x[2 * e + 1] * c[e]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[e] = fmaf(x[e], c[e], -(x[e + 4] * n[e]));
+            y[e + 4] = fmaf(x[e], n[e], x[e + 4] * c[e]);
+          }
+        }
+        if (store && h < heads) {
+          put4(dst + h * dst_stride, y);
+          put4(dst + h * dst_stride + HALF, y + 4);
+        }
       }
     }
-    float y[8];
-    if (a.pairs) {
+  };
+  turn(q, H, a.q_norm, wq, qs, static_cast<C *>(a.out) + row * a.out_stride + at, HD, true);
+  const int64_t slot = page * kv.page_stride + (pos % kv.page_size) * kv.slot_stride + at;
+  fetch(k, 0, KV);
+  turn(k, KV, a.k_norm, wk, ks, static_cast<C *>(kv.k) + slot, kv.head_stride, page >= 0);
+  if (page < 0) return;
+  const S *v = static_cast<const S *>(a.v) + row * a.v_stride + at;
+  C *vd = static_cast<C *>(kv.v) + slot;
+  for (int h0 = 0; h0 < KV; h0 += HOLD * ROUND) {
+    fetch(v, h0, KV);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[2 * e] = fmaf(x[2 * e], c[e], -(x[2 * e + 1] * n[e]));
-        y[2 * e + 1] = fmaf(x[2 * e], n[e], x[2 * e + 1] * c[e]);
-      }
-    } else {
-      const bool hi = li >= LPH / 2;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float o = __shfl_xor_sync(FULL_MASK, x[e], LPH / 2);
-        y[e] = hi ? fmaf(o, n[e], x[e] * c[e]) : fmaf(x[e], c[e], -(o * n[e]));
-      }
-    }
-    if (!live) continue;
-    if (!isk) store8(static_cast<C *>(a.out) + row * a.out_stride + head * HD + 8 * li, y);
-    else if (page >= 0) store8(static_cast<C *>(kv.k) + slot + head * kv.head_stride + 8 * li, y);
-  }
-  if (page >= 0)
-    for (int i = threadIdx.x; i < KV * LPH; i += QT) {
+    for (int u = 0; u < HOLD; ++u) {
+      const int h = h0 + u * ROUND + mine;
+      if (h >= KV) continue;
       float x[8];
-      load8(v + 8 * i, x);
-      store8(static_cast<C *>(kv.v) + slot + (i / LPH) * kv.head_stride + 8 * (i % LPH), x);
+      raw[u][0].get(x);
+      raw[u][1].get(x + 4);
+      put4(vd + h * kv.head_stride, x);
+      put4(vd + h * kv.head_stride + HALF, x + 4);
     }
+  }
 }
 
+template <typename S, typename C, int HD>
+void launch(const QkArgs &g, int sms, cudaStream_t st) {
+  // a warp per token once they fill the SMs (24 warps each); the norm over the whole row needs the CTA's warps together
+  if (g.a.norm != CLB200_QK_NORM_ROW && g.a.T >= 24 * sms / 2) qk_rope_kernel<S, C, HD, 1><<<(g.a.T + QW - 1) / QW, QT, 0, st>>>(g);
+  else qk_rope_kernel<S, C, HD, QW><<<g.a.T, QT, 0, st>>>(g);
+}
 template <typename S, typename C>
-void launch_hd(const QkArgs &g, cudaStream_t st) {
+void launch_hd(const QkArgs &g, int sms, cudaStream_t st) {
   switch (g.kv.head_dim) {
-    case 64: qk_rope_kernel<S, C, 64><<<g.a.T, QT, 0, st>>>(g); break;
-    case 128: qk_rope_kernel<S, C, 128><<<g.a.T, QT, 0, st>>>(g); break;
-    default: qk_rope_kernel<S, C, 256><<<g.a.T, QT, 0, st>>>(g); break;
+    case 64: launch<S, C, 64>(g, sms, st); break;
+    case 128: launch<S, C, 128>(g, sms, st); break;
+    default: launch<S, C, 256>(g, sms, st); break;
   }
 }
 
@@ -227,11 +281,11 @@ extern "C" int clb200_qk_rope(clb200_ctx *c, const clb200_kv *kv, const clb200_q
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : c->stream;
   const bool f32 = a->src_type == T_F32;
   if (kv->type == T_F16) {
-    if (f32) launch_hd<float, __half>(g, st);
-    else launch_hd<__half, __half>(g, st);
+    if (f32) launch_hd<float, __half>(g, c->sms, st);
+    else launch_hd<__half, __half>(g, c->sms, st);
   } else {
-    if (f32) launch_hd<float, __nv_bfloat16>(g, st);
-    else launch_hd<__nv_bfloat16, __nv_bfloat16>(g, st);
+    if (f32) launch_hd<float, __nv_bfloat16>(g, c->sms, st);
+    else launch_hd<__nv_bfloat16, __nv_bfloat16>(g, c->sms, st);
   }
   CUDA_OR(cudaGetLastError(), "launching the rotation");
   return 0;

@@ -30,6 +30,20 @@ CLB_DEV __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <>
 CLB_DEV __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Two floats rounded to a half-precision type, a in the low half.
+template <typename C>
+CLB_DEV uint32_t pack2(float a, float b) {
+  if constexpr (__is_same(C, __half)) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else if constexpr (__is_same(C, __nv_bfloat16)) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    return 0;   // not reached: floats are not packed
+  }
+}
+
 // Four floats times f, rounded to O (16 or 8 bytes, aligned).
 template <typename O>
 CLB_DEV void store4(O *p, float4 v, float f) {
