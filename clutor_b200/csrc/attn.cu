@@ -63,8 +63,12 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
   while (run.more()) {
     const AttnSeq q = run.q;
     const AttnSpan span = attn_span<RN>(g, q, run.qt);
-    const int i0 = run.i0, n = run.tiles(span), t0 = run.qt * g.tpi, head = run.head, s = run.s;
+    const int i0 = run.first(g), n = run.tiles(g, span), t0 = run.qt * g.tpi, head = run.head, s = run.s;
     const bool whole = n == span.nt;
+    if (n == 0) {   // the run ends in the item's lead
+      run.advance(g, span);
+      continue;
+    }
     __syncthreads();   // the last item's queries and joined states have been read
     for (int i = tid; i < ROWS * (HD / 8); i += RT) {
       const int r = i / (HD / 8), c = i % (HD / 8), tr = attn_token(g, r), t = t0 + tr, h = head * g.group + r - tr * g.group;
@@ -205,7 +209,7 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
       issue(i + S::STAGES - 1);
     }
     cp_wait<0>();
-    if (!run.more() || run.at + n >= run.end) grid_launch_dependents();
+    if (run.at + span.nt + g.lead - run.u0 >= run.end) grid_launch_dependents();
     // the warps' states: maximum and sum of each row, values in fp32, joined in warp order
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -250,66 +254,77 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
         if (c == 0) g.piece_ml[static_cast<int64_t>(slot) * g.rows + r] = make_float2(mm, ll);
       }
     }
-    if (!whole && i0 == 0 && tid == 0) g.joins[cta] = make_int4(s, head, run.qt, run.pieces(span.nt - n));
-    run.advance(g, n);
+    if (!whole && i0 == 0 && tid == 0) g.joins[cta] = make_int4(q.row + t0, min(g.tpi, q.nq - t0), head, run.pieces(span.nt - n));
+    run.advance(g, span);
   }
 }
 
 // ---- joining the pieces of items that fell into several runs ---------------------------------------------------------------
 
-constexpr int JT = 128, JW = JT / 32;
+constexpr int JT = 256;
 
-// The largest of the pieces' maxima first, then their values scaled to it. BY_ROW: a warp per row, the pieces in run order (many
-// rows in few pieces). Else a CTA per row, its warps taking every JW-th piece and their sums added in warp order (few rows in
-// many pieces).
+// HD / 4 threads hold a row, four elements each. BY_ROW: a CTA takes as many rows as it has such groups, each going through the
+// pieces in run order (many rows in few pieces: the prompt kernel's). Else a CTA takes one row, its groups every so-many-th piece,
+// and their states are joined in group order (few rows in many pieces: a long cache's).
 template <typename O, int HD, bool BY_ROW>
 __global__ void __launch_bounds__(JT) attn_join_kernel(const AttnArgs g) {
-  constexpr int EPL = HD / 32;
-  __shared__ float sum[JW][HD], den[JW];
+  constexpr int TPR = HD / 4, GROUPS = JT / TPR;
+  __shared__ float4 sum[BY_ROW ? 1 : GROUPS][TPR];
+  __shared__ float2 state[GROUPS];
+  const int grp = threadIdx.x / TPR, e = threadIdx.x % TPR;
+  const int r = BY_ROW ? blockIdx.y * GROUPS + grp : blockIdx.y;
   grid_dependency_wait();
   const int4 j = g.joins[blockIdx.x];
-  if (j.w == 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = BY_ROW ? blockIdx.y * JW + warp : blockIdx.y;
-  const AttnSeq q = attn_seq(g, j.x, false);
-  const int t = j.z * g.tpi + r / g.group;
-  if (r >= g.tpi * g.group || t >= q.nq) return;
+  const int tr = attn_token(g, r);
+  if (j.w == 0 || tr >= j.y) return;   // no item, or no such row (of the whole CTA, where its threads meet below)
   // piece i: slot 1 of this CTA, then slot 0 of the CTAs that follow
   auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * g.rows + r; };
-  float mm = -INFINITY;
-  for (int i = lane; i <= j.w; i += 32) mm = fmaxf(mm, g.piece_ml[slot(i)].x);
+  float m = -INFINITY, l = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int U = 4;   // pieces on their way at once
+  for (int i0 = BY_ROW ? 0 : grp; i0 <= j.w; i0 += U * (BY_ROW ? 1 : GROUPS)) {
+    float2 ml[U];
+    float4 o[U];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(FULL_MASK, mm, o));
-  float v[EPL], l = 0.f;
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * (BY_ROW ? 1 : GROUPS);
+      ml[u] = make_float2(-INFINITY, 0.f);
+      o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i <= j.w) {
+        ml[u] = g.piece_ml[slot(i)];
+        o[u] = *reinterpret_cast<const float4 *>(g.piece_o + slot(i) * HD + 4 * e);
+      }
+    }
+    float mm = m;
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) v[e] = 0.f;
-#pragma unroll 4
-  for (int i = BY_ROW ? 0 : warp; i <= j.w; i += BY_ROW ? 1 : JW) {
-    const float2 ml = g.piece_ml[slot(i)];
-    const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - mm);
-    const float *src = g.piece_o + slot(i) * HD;
-    l = fmaf(f, ml.y, l);
+    for (int u = 0; u < U; ++u) mm = fmaxf(mm, ml[u].x);
+    const float f0 = m == -INFINITY ? 0.f : exp2_approx(m - mm);
+    l *= f0;
+    v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
+    m = mm;
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) v[e] = fmaf(f, src[lane + 32 * e], v[e]);
+    for (int u = 0; u < U; ++u) {
+      const float f = ml[u].x == -INFINITY ? 0.f : exp2_approx(ml[u].x - mm);
+      l = fmaf(f, ml[u].y, l);
+      v.x = fmaf(f, o[u].x, v.x); v.y = fmaf(f, o[u].y, v.y); v.z = fmaf(f, o[u].z, v.z); v.w = fmaf(f, o[u].w, v.w);
+    }
   }
-  O *dst = static_cast<O *>(g.a.out) + (q.row + t) * g.a.out_stride + (j.y * g.group + r % g.group) * HD;
-  if constexpr (BY_ROW) {
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) dst[lane + 32 * e] = from_f32<O>(v[e] * inv);
-    return;
+  if constexpr (!BY_ROW) {
+    sum[grp][e] = v;
+    if (e == 0) state[grp] = make_float2(m, l);
+    __syncthreads();
+    if (grp != 0) return;
+    for (int k = 0; k < GROUPS; ++k) m = fmaxf(m, state[k].x);
+    l = 0.f;
+    v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < GROUPS; ++k) {
+      const float f = state[k].x == -INFINITY ? 0.f : exp2_approx(state[k].x - m);
+      const float4 o = sum[k][e];
+      l = fmaf(f, state[k].y, l);
+      v.x = fmaf(f, o.x, v.x); v.y = fmaf(f, o.y, v.y); v.z = fmaf(f, o.z, v.z); v.w = fmaf(f, o.w, v.w);
+    }
   }
-#pragma unroll
-  for (int e = 0; e < EPL; ++e) sum[warp][lane + 32 * e] = v[e];
-  if (lane == 0) den[warp] = l;
-  __syncthreads();
-  l = 0.f;
-  for (int w = 0; w < JW; ++w) l += den[w];
-  const float inv = l > 0.f ? 1.0f / l : 0.f;
-  for (int d = threadIdx.x; d < HD; d += JT) {
-    float o = 0.f;
-    for (int w = 0; w < JW; ++w) o += sum[w][d];
-    dst[d] = from_f32<O>(o * inv);
-  }
+  store4<O>(static_cast<O *>(g.a.out) + (j.x + tr) * g.a.out_stride + (j.z * g.group + r - tr * g.group) * HD + 4 * e, v, l > 0.f ? 1.0f / l : 0.f);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -328,7 +343,8 @@ template <typename O, int HD>
 cudaError_t launch_join(const AttnArgs &g, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
   const bool by_row = g.rows > 32;
-  cfg.gridDim = dim3(g.nc, by_row ? (g.tpi * g.group + JW - 1) / JW : g.tpi * g.group);
+  const int groups = JT / (HD / 4);
+  cfg.gridDim = dim3(g.nc, by_row ? (g.tpi * g.group + groups - 1) / groups : g.tpi * g.group);
   cfg.blockDim = dim3(JT);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -445,7 +461,8 @@ extern "C" int clb200_attention(clb200_ctx *c, const clb200_kv *kv, const clb200
     g.rows = p.rows;
     g.tpi = p.tpi;
     g.nc = p.nc;
-    g.min_run = p.rows <= 32 ? 4 : 2;
+    g.min_run = p.rows <= 32 ? 1 : 2;
+    g.lead = p.rows <= 32 ? 4 : 2;
     g.piece_o = reinterpret_cast<float *>(w);
     g.piece_ml = reinterpret_cast<float2 *>(w + p.off_ml);
     g.joins = reinterpret_cast<int4 *>(w + p.off_joins);

@@ -3,8 +3,10 @@
 // An item is one sequence, one key/value head and up to `tpi` of the sequence's new tokens, whose tpi x group rows (row = token
 // x group + query head of the group) share every key and value they read. Its keys come in tiles of N positions: those up to
 // the last token's position, without the tiles that a window hides from all of its tokens. Every item has at least one tile (a
-// fully hidden one gives zeros). The tiles of all items, item after item, are dealt to the CTAs in equal runs, so ragged
-// batches and long caches balance by themselves; an item that falls into several runs leaves one partial state (running
+// fully hidden one gives zeros). The tiles of all items, item after item, each item with `lead` units more at its front for what
+// beginning and ending it costs, are dealt to the CTAs in equal runs, so ragged batches and long caches balance by themselves
+// (the prompt of 8192: 439 us with a lead of 2, 531 without, when the CTA that got the 40 shortest items took a quarter longer
+// than the others); an item that falls into several runs leaves one partial state (running
 // maximum, sum, unnormalised values per row) per run in the workspace, and a second kernel joins them. A CTA's run holds at
 // most two such pieces: the first item's, when an earlier CTA began it (slot 0), and the last item's, when this CTA begins and
 // does not finish it (slot 1).
@@ -22,12 +24,13 @@ struct AttnArgs {
   int group, tpi;     // query heads per key/value head, new tokens per item
   uint32_t group_inv; // (65536 + group - 1) / group: row / group = row * group_inv >> 16 for rows below 4096
   int page_shift;     // log2 of the page size where it is a power of two, else -1
-  int nc, min_run;    // CTAs, tiles a CTA takes at least
+  int nc, min_run;    // CTAs, units a CTA takes at least
+  int lead;           // units of an item besides its tiles
   int rows;           // rows of a piece (>= tpi x group)
   float *piece_o;     // [nc][2][rows][head_dim]
   float2 *piece_ml;   // [nc][2][rows] maximum (times log2 e) and sum
-  int4 *joins;        // [nc] the item that begins in this CTA and does not end there: sequence, head, q tile, pieces that
-                      // follow; pieces 0: none
+  int4 *joins;        // [nc] the item that begins in this CTA and does not end there: its first row, tokens, head, and the
+                      // pieces that follow (0: there is no such item)
 };
 
 struct AttnSeq {
@@ -107,7 +110,7 @@ CLB_DEV void attn_prefix(const AttnArgs &g, int64_t *prefix, int cta) {
     const AttnSeq t = attn_seq(g, k, cta == 0 && lane == 0);
     const int nqt = (t.nq + g.tpi - 1) / g.tpi;
     int64_t sum = 0;
-    for (int i = lane; i < nqt; i += 32) sum += attn_span<N>(g, t, i).nt;
+    for (int i = lane; i < nqt; i += 32) sum += attn_span<N>(g, t, i).nt + g.lead;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL_MASK, sum, o);
     if (lane == 0) prefix[k + 1] = sum * g.kv.n_kv;
@@ -136,9 +139,9 @@ CLB_DEV void attn_prefix(const AttnArgs &g, int64_t *prefix, int cta) {
 // A CTA's run of tiles, walked by whole warps (every lane holds the same state).
 template <int N>
 struct AttnRun {
-  int64_t at, end;        // tiles of all items: the next, and the first that is another CTA's
-  int64_t run;            // tiles a CTA takes
-  int s, head, qt, i0;    // the next item, and its first tile that is this CTA's
+  int64_t at, end;        // units of all items: the next, and the first that is another CTA's
+  int64_t run;            // units a CTA takes
+  int s, head, qt, u0;    // the next item, and its first unit that is this CTA's
   AttnSeq q;
 
   CLB_DEV void init(const AttnArgs &g, const int64_t *prefix, int cta) {
@@ -161,7 +164,7 @@ struct AttnRun {
     head = static_cast<int>(r / per_head);
     r -= head * per_head;
     for (int base = 0;; base += 32) {   // the q tile, 32 at a time
-      const int nt = (base + lane) * static_cast<int64_t>(g.tpi) < q.nq ? attn_span<N>(g, q, base + lane).nt : 0;
+      const int nt = (base + lane) * static_cast<int64_t>(g.tpi) < q.nq ? attn_span<N>(g, q, base + lane).nt + g.lead : 0;
       int64_t sum = nt;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -172,18 +175,22 @@ struct AttnRun {
       if (hit || base * static_cast<int64_t>(g.tpi) >= q.nq) {
         const int l = hit ? __ffs(hit) - 1 : 0;
         qt = base + l;
-        i0 = static_cast<int>(r - __shfl_sync(FULL_MASK, sum - nt, l));
+        u0 = static_cast<int>(r - __shfl_sync(FULL_MASK, sum - nt, l));
         break;
       }
       r -= __shfl_sync(FULL_MASK, sum, 31);
     }
   }
-  // The next item's tiles that are this CTA's; false at the end of the run.
   CLB_DEV bool more() const { return at < end; }
-  CLB_DEV int tiles(const AttnSpan &p) const { return static_cast<int>(min(static_cast<int64_t>(p.nt - i0), end - at)); }
-  CLB_DEV void advance(const AttnArgs &g, int n) {
-    at += n;
-    i0 = 0;
+  // This CTA's tiles of the next item: n (0 where its run ends inside the item's lead) from first() on.
+  CLB_DEV int first(const AttnArgs &g) const { return max(u0 - g.lead, 0); }
+  CLB_DEV int tiles(const AttnArgs &g, const AttnSpan &p) const {
+    const int64_t u1 = min(static_cast<int64_t>(p.nt + g.lead), u0 + end - at);
+    return static_cast<int>(u1 > g.lead ? u1 - g.lead : 0) - first(g);
+  }
+  CLB_DEV void advance(const AttnArgs &g, const AttnSpan &p) {
+    at += p.nt + g.lead - u0;
+    u0 = 0;
     if (at >= end) return;
     if (++qt * g.tpi < q.nq) return;
     qt = 0;

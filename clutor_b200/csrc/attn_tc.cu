@@ -79,7 +79,7 @@ struct __align__(16) TcItem {
   int n, i0, sinks, start;     // this CTA's tiles [i0, i0 + n) of the item; tile i is i below sinks, else start + i
   int s, head, kv, row;        // sequence, key/value head, length, first token's row
   int tokens, lo, hi, whole;   // tokens, positions of the first and last, whether all of its tiles are here
-  int qt, pieces, pad[2];      // q tile, CTAs that hold the rest of an item that begins here
+  int pieces, pad[3];          // CTAs that hold the rest of an item that begins here
   CLB_DEV int tile(int i) const { return i0 + i + (i0 + i < sinks ? 0 : start); }
 };
 constexpr int ITEMS = 4;       // items in shared memory at once
@@ -148,14 +148,14 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
         const uint32_t k = it % ITEMS;
         if (it >= ITEMS && !wait_bar(&item_free[k], (it / ITEMS - 1) & 1)) { ok = false; break; }
         TcItem x{};
-        if (run.more()) {
+        while (run.more() && x.n == 0) {
           const AttnSpan p = attn_span<N>(g, run.q, run.qt);
-          x.n = run.tiles(p);
-          x.i0 = run.i0; x.sinks = p.sinks; x.start = p.start;
+          x.n = run.tiles(g, p);
+          x.i0 = run.first(g); x.sinks = p.sinks; x.start = p.start;
           x.s = run.s; x.head = run.head; x.kv = run.q.kv; x.row = run.q.row + run.qt * g.tpi;
           x.tokens = min(g.tpi, run.q.nq - run.qt * g.tpi); x.lo = p.lo; x.hi = p.hi; x.whole = x.n == p.nt;
-          x.qt = run.qt; x.pieces = run.i0 == 0 && !x.whole ? run.pieces(p.nt - x.n) : 0;
-          run.advance(g, x.n);
+          x.pieces = x.i0 == 0 && !x.whole ? run.pieces(p.nt - x.n) : 0;
+          run.advance(g, p);
         }
         if (lane == 0) {
           items[k] = x;
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
         }
       }
       if (!ok) break;
-      if (x.pieces && tid == 0) g.joins[cta] = make_int4(x.s, x.head, x.qt, x.pieces);
+      if (x.pieces && tid == 0) g.joins[cta] = make_int4(x.row, x.tokens, x.head, x.pieces);
       if (!wait_bar(&o_full[w], o_cnt++ & 1)) { ok = false; break; }
       tc::fence_after_sync();
       const float l = (l0.x + l0.y) + (l1.x + l1.y), inv = x.whole ? (l > 0.f ? 1.0f / l : 0.f) : 1.0f;
