@@ -416,29 +416,39 @@ class Context:
         and kv_len [n_seq] int32; rope [n_pos, head_dim] float32 (cosines, then sines). Returns the turned q, [T, n_head,
         head_dim] of the cache's type (`out`, or a new tensor); asynchronous."""
         T, H, D = q.shape
-        KV, dt = pages.n_kv, q.dtype
-        if k.shape != (T, KV, D) or v.shape != (T, KV, D) or D != pages.head_dim:
+        KV, dt, f32 = pages.n_kv, q.dtype, _float32
+        rows = T, KV, D
+        if k.shape != rows or v.shape != rows or D != pages.head_dim:
             raise ClutorError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit a cache of "
                               f"{KV} heads of {pages.head_dim}")
-        if k.dtype != dt or v.dtype != dt:
+        if k.dtype is not dt or v.dtype is not dt:
             raise ClutorError("q, k and v must have one type")
-        self._on_device(pages.k, q, k, v, rope, q_start, kv_len, q_norm, k_norm, out)
-        if rope.dtype != _torch().float32 or rope.dim() != 2 or rope.shape[1] != D or not rope.is_contiguous():
+        device = self.device
+        if not (pages.device == device == q.get_device() == k.get_device() == v.get_device() == rope.get_device()):
+            self._on_device(pages.k, q, k, v, rope)
+        if rope.dtype is not f32 or rope.dim() != 2 or rope.shape[1] != D or not rope.is_contiguous():
             raise ClutorError("rope must be a contiguous float32 [n_pos, head_dim] tensor")
+        qn = kn = 0
         if norm:
-            for w, n in ((q_norm, D if norm == QK_NORM_HEAD else H * D), (k_norm, D if norm == QK_NORM_HEAD else KV * D)):
-                if w is None or w.dtype != _torch().float32 or w.numel() != n or not w.is_contiguous():
-                    raise ClutorError("the norm's weights must be contiguous float32 tensors of head_dim elements, or for the "
-                                      "whole row of its heads' elements")
+            self._on_device(q_norm, k_norm)
+            one = norm == QK_NORM_HEAD
+            if q_norm is None or k_norm is None or q_norm.dtype is not f32 or k_norm.dtype is not f32 or \
+                    q_norm.numel() != (D if one else H * D) or k_norm.numel() != (D if one else KV * D) or \
+                    not q_norm.is_contiguous() or not k_norm.is_contiguous():
+                raise ClutorError("the norm's weights must be contiguous float32 tensors of head_dim elements, or for the "
+                                  "whole row of its heads' elements")
+            qn, kn = q_norm.data_ptr(), k_norm.data_ptr()
         st = self._raw_stream(stream)
         if out is None:
-            out = _empty((T, H, D), pages.k.dtype, q.device, stream)
-        elif out.shape != (T, H, D) or out.dtype != pages.k.dtype:
-            raise ClutorError(f"out must be {[T, H, D]} of {pages.k.dtype}")
+            out = _empty((T, H, D), pages.dtype, q.device, stream)
+            out_row = H * D
+        elif out.shape != (T, H, D) or out.dtype is not pages.dtype or out.get_device() != device:
+            raise ClutorError(f"out must be {[T, H, D]} of {pages.dtype} on cuda:{device}")
+        else:
+            out_row = _rows(out)
         pages.pack(self._kv, q_start, kv_len)
         _QK.pack_into(self._args, 0, T, H, _dtype(dt), q.data_ptr(), k.data_ptr(), v.data_ptr(), _rows(q), _rows(k), _rows(v), norm,
-                      q_norm.data_ptr() if q_norm is not None else 0, k_norm.data_ptr() if k_norm is not None else 0, eps,
-                      rope.data_ptr(), rope.shape[0], 1 if pairs else 0, out.data_ptr(), _rows(out))
+                      qn, kn, eps, rope.data_ptr(), rope.shape[0], 1 if pairs else 0, out.data_ptr(), out_row)
         if self._c_qk(self.handle, self._kv_at, self._args_at, st, self._err, 512):
             raise ClutorError(self._err.value.decode())
         return out
@@ -450,28 +460,37 @@ class Context:
         defaults to head_dim ** -0.5. Returns [T, n_head, head_dim] (`out`, or a new tensor of out_dtype, by default q's type);
         asynchronous. The call's workspace is allocated for the stream, so calls may overlap."""
         T, H, D = q.shape
-        if D != pages.head_dim or q.dtype != pages.k.dtype:
-            raise ClutorError(f"q {tuple(q.shape)} of {q.dtype} does not fit a {pages.k.dtype} cache of head_dim {pages.head_dim}")
-        self._on_device(pages.k, q, q_start, kv_len, out)
+        dt = q.dtype
+        if D != pages.head_dim or dt is not pages.dtype:
+            raise ClutorError(f"q {tuple(q.shape)} of {dt} does not fit a {pages.dtype} cache of head_dim {pages.head_dim}")
+        device = self.device
+        if pages.device != device or q.get_device() != device:
+            self._on_device(pages.k, q)
         st = self._raw_stream(stream)
         if out is None:
-            out = _empty((T, H, D), out_dtype or q.dtype, q.device, stream)
-        elif out.shape != (T, H, D) or (out_dtype is not None and out.dtype != out_dtype):
-            raise ClutorError(f"out must be {[T, H, D]} of {out_dtype or out.dtype}")
+            odt = out_dtype or dt
+            out = _empty((T, H, D), odt, q.device, stream)
+            out_row = H * D
+        elif out.shape != (T, H, D) or (out_dtype is not None and out.dtype is not out_dtype) or out.get_device() != device:
+            raise ClutorError(f"out must be {[T, H, D]} of {out_dtype or out.dtype} on cuda:{device}")
+        else:
+            odt, out_row = out.dtype, _rows(out)
         pages.pack(self._kv, q_start, kv_len)
         if max_q is None:
             max_q = T
+        if scale is None:
+            scale = D ** -0.5
         # the workspace depends on the heads, their size and whether few or many rows share a key/value head
-        size = self._work_bytes.get((H, pages.n_kv, D, max_q))
-        args = (T, H, max_q, q.data_ptr(), _rows(q), out.data_ptr(), _dtype(out.dtype), _rows(out), D ** -0.5 if scale is None else scale, window, sinks)
+        key = H, pages.n_kv, D, max_q
+        size = self._work_bytes.get(key)
+        qp, qr, op, ot = q.data_ptr(), _rows(q), out.data_ptr(), _dtype(odt)
         if size is None:
-            _ATTN.pack_into(self._args, 0, *args, 0, 0)
-            size = lib().clb200_attention_work(self.handle, self._kv_at, self._args_at)
-            self._work_bytes[(H, pages.n_kv, D, max_q)] = size
-        work = _empty(size, _torch().uint8, q.device, stream) if size else None   # 0: the call says what is wrong
-        _ATTN.pack_into(self._args, 0, *args, work.data_ptr() if size else 0, size)
+            _ATTN.pack_into(self._args, 0, T, H, max_q, qp, qr, op, ot, out_row, scale, window, sinks, 0, 0)
+            size = self._work_bytes[key] = lib().clb200_attention_work(self.handle, self._kv_at, self._args_at)
+        work = _empty(size, _uint8, q.device, stream) if size else None   # 0: the call says what is wrong
+        _ATTN.pack_into(self._args, 0, T, H, max_q, qp, qr, op, ot, out_row, scale, window, sinks, work.data_ptr() if size else 0, size)
         if self._c_attention(self.handle, self._kv_at, self._args_at, st, self._err, 512):
-            self._work_bytes.pop((H, pages.n_kv, D, max_q), None)
+            self._work_bytes.pop(key, None)
             raise ClutorError(self._err.value.decode())
         return out
 
@@ -479,14 +498,16 @@ class Context:
         """clb200_sample on torch CUDA tensors: one token for each row of logits [rows, vocab] (float32, float16 or bfloat16)
         from u [rows] float32 in [0, 1) and, each None or [rows], temperature, top_p, min_p (float32) and top_k (int32).
         Returns (token [rows] int32, prob [rows] float32); asynchronous."""
+        if _new is None:
+            _use_torch()
         R, V = logits.shape
         step, along = logits.stride()
         if V > 1 and along != 1:
             raise ClutorError("a row's logits must lie next to one another")
         self._on_device(logits, u, temperature, top_k, top_p, min_p, token, prob)
-        f32, i32 = _torch().float32, _torch().int32
+        f32, i32 = _float32, _int32
         for t, d in ((u, f32), (temperature, f32), (top_k, i32), (top_p, f32), (min_p, f32), (token, i32), (prob, f32)):
-            if t is not None and (t.dtype != d or t.shape != (R,) or not t.is_contiguous()):
+            if t is not None and (t.dtype is not d or t.shape != (R,) or not t.is_contiguous()):
                 raise ClutorError(f"u, temperature, top_p, min_p, prob (float32) and top_k, token (int32) must be contiguous tensors "
                                   f"of {R} elements: got {d} wanted, {t.dtype} {tuple(t.shape)}")
         st = self._raw_stream(stream)
@@ -511,11 +532,7 @@ class Context:
 
     def _raw_stream(self, stream) -> int:
         """The cudaStream_t of a torch stream, or of the device's current one."""
-        if stream is None:
-            st = _torch()._C._cuda_getCurrentRawStream(self.device)
-        else:
-            st = stream.cuda_stream
-        return st or CUDA_STREAM_LEGACY
+        return (_current_stream(self.device) if stream is None else stream.cuda_stream) or CUDA_STREAM_LEGACY
 
 
 # the argument structs above as byte layouts: packing one into a buffer that a context keeps costs a third of making a
@@ -524,38 +541,37 @@ _KV = struct.Struct("@PPIiiiiqqqPiiiPP0q")
 _QK = struct.Struct("@iiIPPPqqqiPPfPiiPq0q")
 _ATTN = struct.Struct("@iiiPqPIqfiiPN0q")
 _SAMPLING = struct.Struct("@iiIPqPPPPPPP0q")
-_torch_module = None
+_TYPES: dict = {}   # torch types to ggml type ids
+# of torch, which is imported when the first of these calls is prepared: its types, its allocator, and the raw handle of a current stream
+_float32 = _int32 = _uint8 = _new = _current_stream = None
 
 
-def _torch():
-    global _torch_module
-    if _torch_module is None:
-        import torch
-        _torch_module = torch
+def _use_torch() -> None:
+    global _float32, _int32, _uint8, _new, _current_stream
+    if _new is None:
+        try:
+            import torch
+        except ImportError:   # the calls on host arrays do without
+            return
         _TYPES.update({torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16})
-    return _torch_module
+        _float32, _int32, _uint8, _new = torch.float32, torch.int32, torch.uint8, torch.empty
+        _current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _empty(shape, dtype, device, stream):
     """A new tensor whose memory belongs to `stream`, or to the current stream if that is None."""
-    torch = _torch()
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return _new(shape, dtype=dtype, device=device)
+    import torch
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
-
-
-_TYPES: dict = {}
+        return _new(shape, dtype=dtype, device=device)
 
 
 def _dtype(d) -> int:
     """The ggml type id of a torch type."""
     t = _TYPES.get(d)
     if t is None:
-        _torch()
-        t = _TYPES.get(d)
-        if t is None:
-            raise ClutorError(f"{d} is not float32, float16 or bfloat16")
+        raise ClutorError(f"{d} is not float32, float16 or bfloat16")
     return t
 
 
@@ -572,32 +588,33 @@ class KvPages:
     """A paged key/value cache on the device (clb200_kv): k and v [n_pages, page_size, n_kv, head_dim] float16 or bfloat16 (the
     same strides, head_dim contiguous), table [n_seq, width] int32: the pages of each sequence in order."""
 
-    __slots__ = ("k", "v", "table", "n_pages", "page_size", "n_kv", "head_dim", "_fixed")
+    __slots__ = ("k", "v", "table", "n_pages", "page_size", "n_kv", "head_dim", "dtype", "device", "_fixed")
 
     def __init__(self, k, v, table):
-        torch = _torch()
-        strides = k.stride()
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or strides != v.stride() or strides[3] != 1:
+        _use_torch()
+        strides, shape, dt = k.stride(), k.shape, k.dtype
+        if len(shape) != 4 or shape != v.shape or dt is not v.dtype or strides != v.stride() or strides[3] != 1:
             raise ClutorError("k and v must be [n_pages, page_size, n_kv, head_dim] tensors of one type and layout")
-        if k.dtype not in (torch.float16, torch.bfloat16):
-            raise ClutorError(f"the cache is {k.dtype}: it must be float16 or bfloat16")
-        if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
+        kind = _TYPES.get(dt)
+        if kind != T_F16 and kind != T_BF16:
+            raise ClutorError(f"the cache is {dt}: it must be float16 or bfloat16")
+        n_seq, width = table.shape if table.dim() == 2 else (0, 0)
+        row, along = table.stride() if table.dim() == 2 else (0, 0)
+        if table.dim() != 2 or table.dtype is not _int32 or (width > 1 and along != 1):
             raise ClutorError("table must be an int32 [n_seq, width] tensor")
-        device = k.get_device()
+        self.device = device = k.get_device()
         if device < 0 or v.get_device() != device or table.get_device() != device:
             raise ClutorError("k, v and table must lie on one CUDA device")
-        self.k, self.v, self.table = k, v, table
-        self.n_pages, self.page_size, self.n_kv, self.head_dim = k.shape
-        n_seq, width = table.shape
-        self._fixed = (k.data_ptr(), v.data_ptr(), _dtype(k.dtype), self.n_pages, self.page_size, self.n_kv, self.head_dim, *strides[:3],
-                       table.data_ptr(), max(table.stride(0), width), width, n_seq)
+        self.k, self.v, self.table, self.dtype = k, v, table, dt
+        self.n_pages, self.page_size, self.n_kv, self.head_dim = shape
+        self._fixed = (k.data_ptr(), v.data_ptr(), kind, *shape, *strides[:3], table.data_ptr(), max(row, width), width, n_seq)
 
     def pack(self, buf, q_start, kv_len) -> None:
         """The clb200_kv of one call's sequences, into buf."""
-        n_seq, i32 = self._fixed[-1], _torch().int32
-        if q_start.dtype != i32 or kv_len.dtype != i32 or q_start.shape != (n_seq + 1,) or kv_len.shape != (n_seq,) or \
-                not q_start.is_contiguous() or not kv_len.is_contiguous():
-            raise ClutorError(f"q_start and kv_len must be contiguous int32 tensors of {n_seq + 1} and {n_seq} elements")
+        n_seq, i32, device = self._fixed[-1], _int32, self.device
+        if q_start.dtype is not i32 or kv_len.dtype is not i32 or q_start.shape != (n_seq + 1,) or kv_len.shape != (n_seq,) or \
+                not q_start.is_contiguous() or not kv_len.is_contiguous() or q_start.get_device() != device or kv_len.get_device() != device:
+            raise ClutorError(f"q_start and kv_len must be contiguous int32 tensors of {n_seq + 1} and {n_seq} elements on cuda:{device}")
         _KV.pack_into(buf, 0, *self._fixed, q_start.data_ptr(), kv_len.data_ptr())
 
 

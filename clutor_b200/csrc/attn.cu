@@ -403,7 +403,7 @@ int check(const clb200_kv *kv, const clb200_attn *a, char *err, size_t errlen) {
   }
   if (a->max_q < 0) { errf(err, errlen, "max_q %d", a->max_q); return 1; }
   if (a->out_type != T_F32 && a->out_type != kv->type) { errf(err, errlen, "out is %s: it must be F32 or the cache's type", type_name(a->out_type)); return 1; }
-  if (!a->q || !a->out) { errf(err, errlen, "a buffer is missing"); return 1; }
+  if (a->T > 0 && (!a->q || !a->out)) { errf(err, errlen, "a buffer is missing"); return 1; }
   if (!(a->scale > 0.f) || a->scale > 3.0e38f) { errf(err, errlen, "scale %g: a positive number", a->scale); return 1; }
   if (a->window < 0 || a->sinks < 0) { errf(err, errlen, "window %d, sinks %d: not negative", a->window, a->sinks); return 1; }
   const int64_t nq = static_cast<int64_t>(a->n_head) * kv->head_dim;

@@ -748,10 +748,9 @@ int clb200_model_prefill(clb200_model *m, const int *tokens, int n, float *logit
     m->pf_alloc = cap;
   }
   if (n > 1 && m->ctx->prompt_attention && !m->pg) {
-    std::vector<int> pg(4 + static_cast<size_t>(a.ctx + MODEL_PAGE - 1) / MODEL_PAGE, 0);
-    for (size_t i = 4; i < pg.size(); ++i) pg[i] = static_cast<int>(i) - 4;
-    CUDA_OR(cudaMalloc(&m->pg, pg.size() * 4), "allocating the page table");
-    CUDA_OR(cudaMemcpy(m->pg, pg.data(), pg.size() * 4, cudaMemcpyHostToDevice), "page table upload");
+    const int pages = (a.ctx + MODEL_PAGE - 1) / MODEL_PAGE;
+    CUDA_OR(cudaMalloc(&m->pg, (4 + static_cast<size_t>(pages)) * 4), "allocating the page table");
+    CUDA_OR(pf_pages(m->pg + 4, pages, m->stream), "the page table");
   }
   for (int i = 0; i < n; i += cap) {   // batches of cap tokens; a batch of one is a step (c/src/forward.c:1263-1266)
     const int nb = std::min(cap, n - i);

@@ -380,6 +380,10 @@ __global__ void rows_kernel(int *pg, int rows, int kv) {
   pg[2] = kv;
 }
 
+__global__ void pages_kernel(int *table, int n) {
+  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) table[i] = i;
+}
+
 __global__ void feed_kernel(FwdState *state, const int *token) { state->token = state->next = *token; }
 
 __global__ void resid_add_kernel(float *x, const float *v, size_t n, float scale) {
@@ -423,6 +427,11 @@ int pf_mv(const FwdMat &m, int rows, int cols, int nb, const int8_t *qs, const f
   const dim3 grid((rows + MT_ROWS - 1) / MT_ROWS, (nb + MT_TOK - 1) / MT_TOK);
   mvt_kernel<<<grid, MT_THREADS, L.total, st>>>(m.p, m.type, m.rb, rows, cols, nb, qs, dd, bs, out, accum, scale, err);
   return static_cast<int>(cudaGetLastError());
+}
+
+cudaError_t pf_pages(int *table, int n, cudaStream_t st) {
+  pages_kernel<<<std::min((n + 255) / 256, 148), 256, 0, st>>>(table, n);
+  return cudaGetLastError();
 }
 
 cudaError_t pf_rows(int *pg, int rows, int kv, cudaStream_t st) {

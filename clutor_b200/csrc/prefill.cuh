@@ -45,6 +45,8 @@ struct PfAttnArgs {
 };
 cudaError_t pf_attn(const PfAttnArgs &a, cudaStream_t st);
 
+// A page table that names n pages in order.
+cudaError_t pf_pages(int *table, int n, cudaStream_t st);
 // For the paged attention of a batch: pg[0, 1] = 0, rows (its first rows) and pg[2] = kv (the sequence's length with it).
 cudaError_t pf_rows(int *pg, int rows, int kv, cudaStream_t st);
 // The token that a draw chose becomes the next step's and the last step's choice.

@@ -216,7 +216,7 @@ int check(const clb200_kv *kv, const clb200_qk *a, char *err, size_t errlen) {
   if (check_kv(kv, err, errlen)) return 1;
   if (a->T < 0 || a->n_head < 1 || a->n_head > 1024) { errf(err, errlen, "%d rows of %d query heads: out of range", a->T, a->n_head); return 1; }
   if (a->src_type != T_F32 && a->src_type != kv->type) { errf(err, errlen, "q, k and v are %s: they must be F32 or the cache's type", type_name(a->src_type)); return 1; }
-  if (!a->q || !a->k || !a->v || !a->out || !a->rope) { errf(err, errlen, "a buffer is missing"); return 1; }
+  if ((a->T > 0 && (!a->q || !a->k || !a->v || !a->out)) || !a->rope) { errf(err, errlen, "a buffer is missing"); return 1; }
   if (a->norm < CLB200_QK_NORM_NONE || a->norm > CLB200_QK_NORM_HEAD) { errf(err, errlen, "norm %d: 0 (none), 1 (row) or 2 (head)", a->norm); return 1; }
   if (a->norm && (!a->q_norm || !a->k_norm)) { errf(err, errlen, "the norm's weights are missing"); return 1; }
   if (a->pairs != 0 && a->pairs != 1) { errf(err, errlen, "pairs %d: 0 or 1", a->pairs); return 1; }
@@ -256,7 +256,7 @@ int check_kv(const clb200_kv *kv, char *err, size_t errlen) {
          kv->n_seq, kv->table_width);
     return 1;
   }
-  if (static_cast<int64_t>(kv->table_width) * kv->page_size > INT32_MAX) { errf(err, errlen, "a table of %d pages of %d slots: positions must fit 31 bits", kv->table_width, kv->page_size); return 1; }
+  if (static_cast<int64_t>(kv->table_width) * kv->page_size > (1 << 30)) { errf(err, errlen, "a table of %d pages of %d slots: at most 2^30 positions", kv->table_width, kv->page_size); return 1; }
   if (kv->page_stride < 0 || kv->slot_stride < 0 || kv->head_stride < 0 || kv->page_stride % 8 || kv->slot_stride % 8 || kv->head_stride % 8 ||
       (kv->n_kv > 1 && kv->head_stride < kv->head_dim) || kv->slot_stride < kv->head_dim || (kv->n_pages > 1 && kv->page_stride < kv->head_dim)) {
     errf(err, errlen, "cache strides %lld %lld %lld: multiples of 8 elements that keep heads, slots and pages apart", (long long)kv->page_stride,

@@ -263,13 +263,16 @@ struct Found {
 // The end of the shortest prefix of the order, among the tokens that `among` keeps, whose values (masses, or ones) sum to at
 // least `want` -- for masses ceil(share x their total). Histograms over ever finer runs of the order, summed over the cluster,
 // narrow it to a bin of at most CAP tokens, which are sorted, or to one key, whose tokens count by id. Where the tokens before
-// the bin are few as well (allow_few) they are all listed and left to the caller.
+// the bin are few as well (allow_few) they are all listed and left to the caller. largest: each thread's largest logit, for a
+// first try on counts: the want-th largest of those is a lower bound of the want-th largest of all, so the tokens from its bin on
+// are listed without a histogram of all of them.
 template <int CL, bool MASS>
-CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool allow_few) {
+CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool allow_few, const float *largest = nullptr) {
   Shared *sh = r.sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t lo = 0, hi = 0, shift = 0;   // the run that a level divides: at level 0 everything, then the keys [lo, hi]
   Found f{};
+  bool quick = !MASS && largest;
   for (int level = 0;; ++level) {
     const bool whole = level == 0 && among.all();
     auto inside = [&](float x, uint32_t i) {
@@ -301,6 +304,8 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
           if (up) atomicAdd(&sh->hi[b], up);
         }
       }
+    } else if (quick) {
+      atomicAdd(&sh->lo[r.bin(*largest)], 1u);
     } else {
 #pragma unroll 4
       for (uint32_t i = tid; i < r.n; i += ST) {
@@ -385,10 +390,10 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
     __syncthreads();
     const uint32_t k0 = static_cast<uint32_t>(sh->found[0]), k1 = static_cast<uint32_t>(sh->found[0] >> 32) - 1;   // the bin's keys: k0 .. k1
     const u64 before = sh->found[1];
-    want = sh->found[3] - before;
+    if (!quick) want = sh->found[3] - before;
     if (level == 0) f.total = sh->found[4];
     // list the bin's tokens and, where counts say that it fits, those before it
-    const bool with_above = !MASS && allow_few && level == 0 && before + sh->found[2] <= CAP;
+    const bool with_above = quick || (!MASS && allow_few && level == 0 && before + sh->found[2] <= CAP);
     auto list = [&](bool bin, bool above) {
       uint32_t seen = 0;
 #pragma unroll 4
@@ -437,6 +442,12 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
       const u64 w = sh->found[5];
       f.lim = Limit{static_cast<uint32_t>(w >> 32), 0xffffffffu - static_cast<uint32_t>(w)};
       return f;
+    }
+    if (quick) {   // too many: start over with all of them
+      quick = false;
+      level = -1;
+      cluster_sync<CL>();   // lists and histograms have been read
+      continue;
     }
     // the range of that bin's keys over the cluster
     uint32_t kmin = 0xffffffffu, kmax = 0;
@@ -572,6 +583,7 @@ __global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, 
   if (r.top == INFINITY) {   // those at infinity share everything
     for (uint32_t i = tid; i < r.n; i += ST) r.x[i] = r.x[i] == INFINITY ? 0.f : -INFINITY;
     r.top = 0.f;
+    best = best == INFINITY ? 0.f : -INFINITY;
     __syncthreads();
   }
   r.half_top = 0.5f * r.top;
@@ -591,7 +603,9 @@ __global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, 
   };
   Limit lim{KEY_LOWEST, 0xffffffffu};
   if (by_k || by_p) {
-    Found f = by_k ? search<CL, false>(r, lim, static_cast<u64>(k), 0.0, true) : search<CL, true>(r, lim, 0, static_cast<double>(share), true);
+    // each thread has several tokens and their largest ones are more than enough
+    const float *quick = by_k && k <= CAP / 2 && s.vocab >= 4 * CL * ST ? &best : nullptr;
+    Found f = by_k ? search<CL, false>(r, lim, static_cast<u64>(k), 0.0, true, quick) : search<CL, true>(r, lim, 0, static_cast<double>(share), true);
     if (f.few) {   // the candidates, sorted, a thread each: the filters are prefixes, the draw goes by id
       const uint32_t q = static_cast<uint32_t>(f.word >> 32), id = 0xffffffffu - static_cast<uint32_t>(f.word);
       const bool cand = static_cast<uint32_t>(tid) < f.n && (!by_k || tid < k);
@@ -697,7 +711,7 @@ int check(const clb200_sampling *s, char *err, size_t errlen) {
     return 1;
   }
   if (s->type != T_F32 && s->type != T_F16 && s->type != T_BF16) { errf(err, errlen, "logits are %s: F32, F16 or BF16", type_name(s->type)); return 1; }
-  if (!s->logits || !s->u || !s->token) { errf(err, errlen, "a buffer is missing"); return 1; }
+  if (s->rows > 0 && (!s->logits || !s->u || !s->token)) { errf(err, errlen, "a buffer is missing"); return 1; }
   if (s->rows > 1 && s->stride < s->vocab) { errf(err, errlen, "rows %lld elements apart do not hold %d logits", (long long)s->stride, s->vocab); return 1; }
   if (reinterpret_cast<uintptr_t>(s->logits) % (s->type == T_F32 ? 4 : 2)) { errf(err, errlen, "the logits do not start on a boundary of their type"); return 1; }
   return 0;

@@ -8,6 +8,8 @@ Bars, each a bound by arithmetic on the operator's own roundings:
     value sums are fp32 (n + 64 roundings at worst), the exponentials are good to 2^-21, the result is rounded once.
   sample: token equal; prob a quotient of two values good to 2^-40, rounded once.
 """
+import copy
+
 import numpy as np
 import pytest
 
@@ -334,4 +336,197 @@ def test_steps_together_captured(ctx):
         torch.cuda.synchronize()
         assert (tok.tolist(), prob.tolist()) == eager[i]
     assert torch.equal(c.k.contiguous().view(torch.int16), want_k.contiguous().view(torch.int16))
+    ctx.status()
+
+
+def test_attention_many_sequences(ctx):
+    """More sequences than one launch takes (512), and sequences without rows between others; few and many rows a head."""
+    import torch
+    rng = np.random.default_rng(8)
+    for q_max, KV, H, D in ((1, 2, 6, 64), (9, 1, 8, 128)):
+        n = 1100
+        q = [int(v) for v in rng.integers(0, q_max + 1, n)]
+        kv = [int(v) for v in np.maximum(rng.integers(0, 60, n), q)]
+        b = Batch(kv, q, KV, D, 16, "bf16", seed=D)
+        b.fill(1)
+        x = torch.randn(b.T, H, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4)).to(torch.bfloat16)
+        out = ctx.attention(x, b.pages, b.q_start_d, b.kv_len_d, max_q=q_max)
+        ctx.status()
+        attn_check(b, x, out, H, "bf16", 0, 0, D ** -0.5)
+
+
+def test_attention_large_offsets(ctx):
+    """A cache whose elements lie beyond 2^31 elements and 2^32 bytes from its start."""
+    import torch
+
+    import clutor_b200 as cb
+    KV, D, page, stride = 2, 64, 16, (1 << 31) // 3 // 8 * 8
+    pool = torch.empty(2, 3 * stride + page * KV * D, dtype=torch.float16, device="cuda")
+    k, v = (pool[i].as_strided((4, page, KV, D), (stride, KV * D, D, 1), pool[i].storage_offset()) for i in (0, 1))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    table = torch.tensor([[3, 0, 2], [1, 3, 2]], dtype=torch.int32, device="cuda")
+    for p in range(4):
+        k[p], v[p] = (torch.randn(page, KV, D, generator=g, device="cuda").half() for _ in range(2))
+    pages = cb.KvPages(k, v, table)
+    kv = torch.tensor([45, 33], dtype=torch.int32, device="cuda")
+    for q in ([1, 1], [40, 33]):
+        qs = torch.tensor([0, q[0], sum(q)], dtype=torch.int32, device="cuda")
+        x = torch.randn(sum(q), 8, D, generator=g, device="cuda").half()
+        out = ctx.attention(x, pages, qs, kv, max_q=max(q)).double().cpu().numpy()
+        ctx.status()
+        for s, (n, t) in enumerate(((45, [3, 0, 2]), (33, [1, 3, 2]))):
+            kk, vv = (c[torch.tensor(t, device="cuda")].flatten(0, 1)[:n].double().cpu().numpy() for c in (k, v))
+            for i in range(q[s]):
+                r = int(qs[s]) + i
+                y, mag, flat, big = ref.attention(x[r].double().cpu().numpy(), kk, vv, n - q[s] + i, D ** -0.5, 0, 0)
+                assert (np.abs(out[r] - y) <= 2.0 ** -11 * np.abs(y) + mag * (2.0 ** -11 + 132 * 2.0 ** -24 * big + 2.0 ** -20) * 1.01 + 2.0 ** -25 * (flat + 1)).all()
+    # and the store
+    x = torch.randn(2, 8 + 2 * KV, D, generator=g, device="cuda")
+    rope = torch.cat([torch.ones(64, D // 2), torch.zeros(64, D // 2)], 1).cuda()
+    ctx.qk_rope(x[:, :8], x[:, 8:8 + KV], x[:, 8 + KV:], pages, torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"), kv, rope, norm=0)
+    ctx.status()
+    assert torch.equal(v[2, 44 % 16], x[0, 8 + KV:].half()) and torch.equal(k[2, 32 % 16], x[1, 8:8 + KV].half())
+
+
+def test_streams_and_two_graphs_at_once(ctx):
+    """Calls on a stream of their own, and two captured graphs of the same calls replayed at the same time: each has its own
+    workspace, so neither disturbs the other. The lengths in device memory change between replays."""
+    import torch
+    H, KV, D = 16, 2, 128
+    made = []
+    for i, (kv, q) in enumerate((([900, 400], [1, 1]), ([500, 260], [130, 70]))):
+        b = Batch(kv, q, KV, D, 32, "bf16", seed=i)
+        b.fill(i)
+        g = torch.Generator(device="cuda").manual_seed(i)
+        x = torch.randn(b.T, H, D, generator=g, device="cuda").to(torch.bfloat16)
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        stream.wait_stream(torch.cuda.current_stream())
+        first = ctx.attention(x, b.pages, b.q_start_d, b.kv_len_d, max_q=max(q), stream=stream)
+        torch.cuda.synchronize()
+        attn_check(b, x, first, H, "bf16", 0, 0, D ** -0.5)
+        with torch.cuda.graph(graph):
+            out = ctx.attention(x, b.pages, b.q_start_d, b.kv_len_d, max_q=max(q))
+        made.append((b, x, stream, graph, out))
+    for less in (0, 7, 100):
+        for b, x, stream, graph, out in made:
+            b.kv = [n - less for n in b.kv]
+            b.kv_len_d.copy_(torch.tensor(b.kv, device="cuda"))
+        torch.cuda.synchronize()
+        for _ in range(10):
+            for b, x, stream, graph, out in made:
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for b, x, stream, graph, out in made:
+            attn_check(b, x, out, H, "bf16", 0, 0, D ** -0.5)
+    ctx.status()
+
+
+@pytest.mark.parametrize("rows,vocab", [(80, 50304), (160, 1000), (80, 60001), (40, 100003), (3, 151936), (1, 8191)])
+def test_sample_row_splits(ctx, rows, vocab):
+    """Every number of CTAs a row (1, 2, 4, 8)."""
+    import torch
+    rng = np.random.default_rng(rows + vocab)
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    lg = 2 * torch.randn(rows, vocab, generator=g, device="cuda")
+    lg.scatter_add_(1, torch.randint(vocab, (rows, 8), generator=g, device="cuda"), 9 * torch.rand(rows, 8, generator=g, device="cuda"))
+    sample_check(ctx, lg, [float(v) for v in rng.random(rows).astype(np.float32)], [float(v) for v in rng.choice([0.0, 0.6, 1.0, 1.4], rows)],
+                 [int(v) for v in rng.choice([0, 1, 30, 200, 256, 257, 3000], rows)], [float(v) for v in rng.choice([0.2, 0.9, 0.99, 1.0], rows)],
+                 [float(v) for v in rng.choice([0.0, 0.03], rows)])
+
+
+# ---- what only the device can see ------------------------------------------------------------------------------------------
+
+def status_says(ctx, text):
+    import clutor_b200 as cb
+    with pytest.raises(cb.ClutorError, match=text):
+        ctx.status()
+    ctx.status()   # reported once
+
+
+@pytest.mark.parametrize("q", [1, 40])
+def test_bad_pages_and_rows_are_reported(ctx, q):
+    """Page ids out of range, a table too short and more rows than max_q: skipped on the device and reported; the other sequence's
+    rows are right, and the next call is."""
+    import torch
+    H, KV, D = 8, 1, 128
+    b = Batch([70, 90], [q, q], KV, D, 16, "f16", seed=3)
+    b.fill(2)
+    x = torch.randn(b.T, H, D, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").half()
+    good = ctx.attention(x, b.pages, b.q_start_d, b.kv_len_d, max_q=q)
+    ctx.status()
+    for bad in (-1, b.pages.n_pages, 2 ** 31 - 1):
+        keep = b.pages.table[0, 2].clone()
+        b.pages.table[0, 2] = bad
+        out = ctx.attention(x, b.pages, b.q_start_d, b.kv_len_d, max_q=q)
+        status_says(ctx, "page")
+        assert torch.equal(out[q:], good[q:])
+        b.pages.table[0, 2] = keep
+    b.kv_len_d[0] = 16 * b.pages.table.shape[1] + 1
+    out = torch.full_like(good, 5.0)
+    ctx.attention(x, b.pages, b.q_start_d, b.kv_len_d, max_q=q, out=out)
+    status_says(ctx, "page")
+    assert torch.equal(out[q:], good[q:]) and (out[:q] == 5.0).all()
+    b.kv_len_d[0] = 70
+    starts = torch.tensor([0, q, 2 * q + 9], dtype=torch.int32, device="cuda")   # past the rows there are
+    ctx.attention(x, b.pages, starts, b.kv_len_d, max_q=q + 9, out=out)
+    status_says(ctx, "rows")
+    first = copy.copy(b)   # another max_q may choose another kernel: the same values within the bar, not the same bits
+    first.kv, first.q_start = [70], b.q_start[:2]
+    attn_check(first, x, out, H, "f16", 0, 0, D ** -0.5)
+    out.fill_(5.0)
+    if q > 1:
+        ctx.attention(x, b.pages, b.q_start_d, b.kv_len_d, max_q=q - 1, out=out)
+        status_says(ctx, "rows")
+        assert (out == 5.0).all()
+    assert torch.equal(ctx.attention(x, b.pages, b.q_start_d, b.kv_len_d, max_q=q), good)
+    ctx.status()
+
+
+def test_bad_positions_in_the_rotation_are_reported(ctx):
+    import torch
+    H, KV, D = 4, 2, 64
+    b = Batch([20, 30], [2, 3], KV, D, 16, "bf16", seed=3)
+    x = torch.randn(b.T, H + 2 * KV, D, device="cuda")
+    rope = torch.ones(25, D, device="cuda")           # positions 27..29 of the second sequence are past it
+    before = b.pool.clone()
+    out = torch.full((b.T, H, D), 9.0, dtype=torch.bfloat16, device="cuda")
+    ctx.qk_rope(x[:, :H], x[:, H:H + KV], x[:, H + KV:], b.pages, b.q_start_d, b.kv_len_d, rope, norm=0, out=out)
+    status_says(ctx, "rows")
+    assert (out[2:] == 9.0).all() and (out[:2] != 9.0).any()
+    p, i = b.where(0, np.arange(18, 20))
+    changed = b.pool.view(torch.int16) != before.view(torch.int16)
+    b.pool.copy_(before)
+    b.k[p, i] = 1.0
+    b.v[p, i] = 1.0
+    assert not (changed & ~(b.pool.view(torch.int16) != before.view(torch.int16))).any()   # only those two slots
+    b.pages.table[0, 1] = 10 ** 6
+    ctx.qk_rope(x[:, :H], x[:, H:H + KV], x[:, H + KV:], b.pages, b.q_start_d, b.kv_len_d, torch.ones(64, D, device="cuda"), norm=0, out=out)
+    status_says(ctx, "page")
+
+
+def test_python_refusals(ctx):
+    import torch
+
+    import clutor_b200 as cb
+    H, KV, D = 4, 2, 64
+    b = Batch([20], [2], KV, D, 16, "bf16", seed=3)
+    b.fill(1)
+    x = torch.randn(2, H, D, device="cuda").to(torch.bfloat16)
+    good = (x, b.pages, b.q_start_d, b.kv_len_d)
+    cases = [lambda: ctx.attention(x.cpu(), *good[1:]), lambda: ctx.attention(x.half(), *good[1:]), lambda: ctx.attention(x[..., :32], *good[1:]),
+             lambda: ctx.attention(x, b.pages, b.q_start_d.long(), b.kv_len_d), lambda: ctx.attention(x, b.pages, b.q_start_d, b.kv_len_d.cpu()),
+             lambda: ctx.attention(*good, out=x[:1]), lambda: ctx.attention(*good, out=x), lambda: ctx.attention(*good, scale=-1.0),
+             lambda: ctx.attention(x.transpose(1, 2).contiguous().transpose(1, 2), *good[1:]), lambda: ctx.attention(x[:, :3], *good[1:]),
+             lambda: cb.KvPages(b.k, b.v.half(), b.pages.table), lambda: cb.KvPages(b.k.float(), b.v.float(), b.pages.table),
+             lambda: cb.KvPages(b.k, b.v, b.pages.table.long()), lambda: cb.KvPages(b.k, b.v, b.pages.table.cpu()),
+             lambda: ctx.sample(x[0], torch.rand(3, device="cuda")), lambda: ctx.sample(x[0].float(), torch.rand(H, device="cuda"), top_k=torch.ones(H, device="cuda")),
+             lambda: ctx.sample(x[0].float().t(), torch.rand(D, device="cuda")), lambda: ctx.sample(torch.zeros(1, (1 << 18) + 1, device="cuda"), torch.rand(1, device="cuda"))]
+    for f in cases:
+        with pytest.raises(cb.ClutorError):
+            f()
+    assert ctx.attention(*good).shape == x.shape
+    empty = x[:0]
+    assert ctx.attention(empty, b.pages, torch.zeros(2, dtype=torch.int32, device="cuda"), b.kv_len_d).shape == (0, H, D)
+    assert ctx.sample(torch.zeros(0, 9, device="cuda"), torch.zeros(0, device="cuda"))[0].shape == (0,)
     ctx.status()

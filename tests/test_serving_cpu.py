@@ -67,7 +67,7 @@ def test_good_calls_reach_the_context(L):
     ({"type": cb.T_F32}, "cache is F32"), ({"type": 77}, "unsupported"), ({"head_dim": 96}, "head_dim 96"),
     ({"page_size": 8}, "page_size 8"), ({"page_size": 40}, "page_size 40"), ({"page_size": 0}, "page_size 0"), ({"n_kv": 0}, "out of range"),
     ({"n_pages": 0}, "out of range"), ({"n_seq": -1}, "out of range"), ({"n_seq": 1 << 17}, "out of range"),
-    ({"table_width": -1}, "out of range"), ({"table_stride": 7}, "out of range"), ({"table_width": 1 << 26, "table_stride": 1 << 26}, "31 bits"),
+    ({"table_width": -1}, "out of range"), ({"table_stride": 7}, "out of range"), ({"table_width": (1 << 24) + 1, "table_stride": 1 << 25}, "2^30 positions"),
     ({"slot_stride": 100}, "strides"), ({"slot_stride": 516}, "strides"), ({"head_stride": 64}, "strides"), ({"page_stride": -8}, "strides"),
     ({"page_stride": 0}, "strides"), ({"k": None}, "missing"), ({"v": None}, "missing"), ({"q_start": None}, "missing"),
     ({"kv_len": None}, "missing"), ({"table": None}, "missing"), ({"k": P + 8}, "16-byte"), ({"v": P + 2}, "16-byte")])
