@@ -106,14 +106,24 @@ CLB_DEV bool attn_sees(const AttnArgs &g, int p, int j) {
 template <int N>
 CLB_DEV void attn_prefix(const AttnArgs &g, int64_t *prefix, int cta) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5, n_seq = g.kv.n_seq;
-  for (int k = warp; k < n_seq; k += nw) {
-    const AttnSeq t = attn_seq(g, k, cta == 0 && lane == 0);
+  for (int k0 = 32 * warp; k0 < n_seq; k0 += 32 * nw) {   // a lane per sequence, so that their look-ups run side by side
+    AttnSeq t{0, 0, 0};
+    if (k0 + lane < n_seq) t = attn_seq(g, k0 + lane, cta == 0);
     const int nqt = (t.nq + g.tpi - 1) / g.tpi;
     int64_t sum = 0;
-    for (int i = lane; i < nqt; i += 32) sum += attn_span<N>(g, t, i).nt + g.lead;
+    if (nqt <= 4)
+      for (int i = 0; i < nqt; ++i) sum += attn_span<N>(g, t, i).nt + g.lead;
+    // a sequence of many items by the whole warp
+    for (unsigned many = __ballot_sync(FULL_MASK, nqt > 4); many; many &= many - 1) {
+      const int l = __ffs(many) - 1, n = __shfl_sync(FULL_MASK, nqt, l);
+      const AttnSeq u{__shfl_sync(FULL_MASK, t.row, l), __shfl_sync(FULL_MASK, t.nq, l), __shfl_sync(FULL_MASK, t.kv, l)};
+      int64_t part = 0;
+      for (int i = lane; i < n; i += 32) part += attn_span<N>(g, u, i).nt + g.lead;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL_MASK, sum, o);
-    if (lane == 0) prefix[k + 1] = sum * g.kv.n_kv;
+      for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(FULL_MASK, part, o);
+      if (lane == l) sum = part;
+    }
+    if (k0 + lane < n_seq) prefix[k0 + lane + 1] = sum * g.kv.n_kv;
   }
   if (threadIdx.x == 0) prefix[0] = 0;
   __syncthreads();

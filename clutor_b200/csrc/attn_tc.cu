@@ -320,6 +320,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
       const TcItem x = x_;
       if (x.tokens <= w * tps) continue;
       const int pos = x.lo + w * tps + tr;
+      const bool row_live = r < tps * g.group && w * tps + tr < x.tokens;
       float m = -INFINITY;
       float2 l0 = make_float2(0.f, 0.f), l1 = l0;
       for (int j = 0; j < x.n; ++j) {
@@ -349,7 +350,8 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
           }
         }
         const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-        if (__any_sync(FULL_MASK, mn > m + 8.0f)) {   // also where m is still -infinity
+        // also where m is still -infinity; rows that are nobody's hold anything and have no say, so that the bits do not hang on them
+        if (__any_sync(FULL_MASK, row_live && mn > m + 8.0f)) {
           const float mb = fmaxf(m, mn), f = m == -INFINITY ? 0.f : exp2_approx(m - mb);
           m = mb;
           l0.x *= f; l0.y *= f; l1.x *= f; l1.y *= f;

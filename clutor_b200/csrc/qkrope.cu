@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(QT, WARPS == 1 ? 3 : 1) qk_rope_kernel(const Q
     load4(a.k_norm + HALF + at, wk + 4);
   }
   float qs = 1.f, ks = 1.f;
-  if (WARPS > 1 && a.norm == CLB200_QK_NORM_ROW) {
+  if (a.norm == CLB200_QK_NORM_ROW) {
     auto squares = [&](const S *p, int heads) {
       float t = 0.f;
       for (int h0 = 0; h0 < heads; h0 += HOLD * ROUND) {
@@ -119,11 +119,13 @@ __global__ void __launch_bounds__(QT, WARPS == 1 ? 3 : 1) qk_rope_kernel(const Q
       for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(FULL_MASK, t, o);
       return t;
     };
-    const float tk = squares(k, KV), tq = squares(q, H);
-    if (lane == 0) { red[0][warp] = tq; red[1][warp] = tk; }
-    __syncthreads();
-    float sq = 0.f, sk = 0.f;
-    for (int w = 0; w < QW; ++w) { sq += red[0][w]; sk += red[1][w]; }
+    float sk = squares(k, KV), sq = squares(q, H);
+    if constexpr (WARPS > 1) {
+      if (lane == 0) { red[0][warp] = sq; red[1][warp] = sk; }
+      __syncthreads();
+      sq = sk = 0.f;
+      for (int w = 0; w < WARPS; ++w) { sq += red[0][w]; sk += red[1][w]; }
+    }
     qs = 1.0f / sqrtf(sq / static_cast<float>(H * HD) + a.eps);
     ks = 1.0f / sqrtf(sk / static_cast<float>(KV * HD) + a.eps);
     if (H > HOLD * ROUND) fetch(q, 0, H);   // the first rounds' registers hold the last ones
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(QT, WARPS == 1 ? 3 : 1) qk_rope_kernel(const Q
           ss = rsqrtf(fmaf(ss, 1.0f / HD, a.eps));   // within 2^-22
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] *= ss * w[e];
-        } else if (WARPS > 1 && a.norm == CLB200_QK_NORM_ROW && h < heads) {
+        } else if (a.norm == CLB200_QK_NORM_ROW && h < heads) {
           load4(norm + h * HD + at, y);
           load4(norm + h * HD + HALF + at, y + 4);
 #pragma unroll
@@ -198,8 +200,8 @@ __global__ void __launch_bounds__(QT, WARPS == 1 ? 3 : 1) qk_rope_kernel(const Q
 
 template <typename S, typename C, int HD>
 void launch(const QkArgs &g, int sms, cudaStream_t st) {
-  // a warp per token once they fill the SMs (24 warps each); the norm over the whole row needs the CTA's warps together
-  if (g.a.norm != CLB200_QK_NORM_ROW && g.a.T >= 24 * sms / 2) qk_rope_kernel<S, C, HD, 1><<<(g.a.T + QW - 1) / QW, QT, 0, st>>>(g);
+  // a warp per token once they half fill the SMs (24 warps each)
+  if (g.a.T >= 24 * sms / 2) qk_rope_kernel<S, C, HD, 1><<<(g.a.T + QW - 1) / QW, QT, 0, st>>>(g);
   else qk_rope_kernel<S, C, HD, QW><<<g.a.T, QT, 0, st>>>(g);
 }
 template <typename S, typename C>

@@ -530,3 +530,22 @@ def test_python_refusals(ctx):
     assert ctx.attention(empty, b.pages, torch.zeros(2, dtype=torch.int32, device="cuda"), b.kv_len_d).shape == (0, H, D)
     assert ctx.sample(torch.zeros(0, 9, device="cuda"), torch.zeros(0, device="cuda"))[0].shape == (0,)
     ctx.status()
+
+
+@pytest.mark.parametrize("H,KV,D", [(14, 2, 64), (12, 4, 128), (5, 1, 256), (8, 1, 128)])
+def test_attention_padding_has_no_say(ctx, H, KV, D):
+    """What stands in the rows of a padded batch, NaN included, changes no bit of the others (a group that does not divide the
+    kernel's 128 rows leaves rows that belong to nobody too)."""
+    import torch
+    b = Batch([300, 128, 57], [255, 1, 57], KV, D, 32, "f16", seed=D)
+    b.fill(5)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = (2 * torch.randn(b.T + 40, H, D, generator=g, device="cuda")).half()
+    outs = []
+    for pad in (0.0, float("nan"), 300.0, float("inf")):
+        x[b.T:] = pad
+        for _ in range(3):
+            outs.append(ctx.attention(x, b.pages, b.q_start_d, b.kv_len_d, max_q=255)[:b.T].clone())
+    ctx.status()
+    for o in outs:
+        assert torch.equal(o, outs[0])
