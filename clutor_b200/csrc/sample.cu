@@ -12,11 +12,11 @@
 namespace clb {
 namespace {
 
-constexpr int ST = 1024, SW = ST / 32;       // threads and warps of a CTA
 constexpr int NB = 2048;                     // bins of a histogram
-constexpr int CAP = 512;                     // tokens that are sorted directly
+constexpr int CAP = 512;                     // tokens that are sorted directly, at most (a thread each)
 constexpr int E = 4;                         // tokens a thread weighs at once
 constexpr int SAMPLE_MAX_VOCAB = 1 << 18;
+constexpr int SMALL_VOCAB = 6144;            // up to this a row is a small CTA's
 constexpr double UNIT = 17592186044416.0;    // 2^44
 constexpr float BINS_PER_NAT = 64.f;         // the first histogram's bins cover 32 e-foldings: lighter weights are below 2^-44
 
@@ -72,7 +72,7 @@ struct Shared {
   u64 coarse[32];            // the sums of NB / 32 bins each
   u64 list[CAP];             // this CTA's tokens of a search, as token_word
   u64 all[CAP];              // every CTA's
-  u64 part[SW];
+  u64 part[32];
   u64 mine[4];               // what this CTA tells the others
   u64 found[7];              // what a search found, for the CTA's threads
   uint32_t n_list, n_above;
@@ -176,13 +176,15 @@ CLB_DEV u64 warp_scan(u64 s) {
   return s;
 }
 // The sum of the threads' values before this thread's, and (total) of all.
+template <int ST>
 CLB_DEV u64 block_scan(Shared *sh, u64 v, u64 &total) {
+  constexpr int SW = ST / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const u64 s = warp_scan(v);
   __syncthreads();
   if (lane == 31) sh->part[warp] = s;
   __syncthreads();
-  const u64 w = warp_scan(sh->part[lane]);   // SW = 32 warps
+  const u64 w = warp_scan(lane < SW ? sh->part[lane] : 0);
   total = __shfl_sync(FULL_MASK, w, 31);
   const u64 before = __shfl_sync(FULL_MASK, w, max(warp - 1, 0));
   return (warp ? before : 0) + s - v;
@@ -207,7 +209,8 @@ CLB_DEV u64 cluster_scan(Row &r, u64 v, u64 &total) {
   }
   return before;
 }
-// Threads 0 .. n - 1 (n <= CAP) hold words, the others 0; sorts them descending (bitonic).
+// Threads 0 .. n - 1 (n at most MOST) hold words, the others 0; sorts them descending (bitonic).
+template <int MOST>
 CLB_DEV u64 sort_words(Shared *sh, u64 x, int n) {
   const int tid = threadIdx.x;
   int size = 1;
@@ -216,10 +219,10 @@ CLB_DEV u64 sort_words(Shared *sh, u64 x, int n) {
     for (int j = k >> 1; j > 0; j >>= 1) {
       u64 y;
       if (j >= 32) {
-        if (tid < CAP) {   // whole warps
-          asm volatile("bar.sync 1, %0;" ::"n"(CAP) : "memory");
+        if (tid < MOST) {   // whole warps
+          asm volatile("bar.sync 1, %0;" ::"n"(MOST) : "memory");
           sh->all[tid] = x;
-          asm volatile("bar.sync 1, %0;" ::"n"(CAP) : "memory");
+          asm volatile("bar.sync 1, %0;" ::"n"(MOST) : "memory");
           y = sh->all[tid ^ j];
         } else {
           y = 0;
@@ -262,12 +265,13 @@ struct Found {
 
 // The end of the shortest prefix of the order, among the tokens that `among` keeps, whose values (masses, or ones) sum to at
 // least `want` -- for masses ceil(share x their total). Histograms over ever finer runs of the order, summed over the cluster,
-// narrow it to a bin of at most CAP tokens, which are sorted, or to one key, whose tokens count by id. Where the tokens before
+// narrow it to a bin of at most MOST tokens, which are sorted, or to one key, whose tokens count by id. Where the tokens before
 // the bin are few as well (allow_few) they are all listed and left to the caller. largest: each thread's largest logit, for a
 // first try on counts: the want-th largest of those is a lower bound of the want-th largest of all, so the tokens from its bin on
 // are listed without a histogram of all of them.
-template <int CL, bool MASS>
+template <int CL, int ST, bool MASS>
 CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool allow_few, const float *largest = nullptr) {
+  constexpr int SW = ST / 32, MOST = ST < CAP ? ST : CAP;
   Shared *sh = r.sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t lo = 0, hi = 0, shift = 0;   // the run that a level divides: at level 0 everything, then the keys [lo, hi]
@@ -314,13 +318,13 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
       }
     }
     __syncthreads();
-    {   // a warp adds NB / 32 bins
+    for (int c = warp; c < 32; c += SW) {   // a warp adds NB / 32 bins
       u64 v = 0;
 #pragma unroll
-      for (int b = 0; b < NB / 32; b += 32) v += (static_cast<u64>(sh->hi[NB / 32 * warp + b + lane]) << 32) + sh->lo[NB / 32 * warp + b + lane];
+      for (int b = 0; b < NB / 32; b += 32) v += (static_cast<u64>(sh->hi[NB / 32 * c + b + lane]) << 32) + sh->lo[NB / 32 * c + b + lane];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
-      if (lane == 0) sh->coarse[warp] = v;
+      if (lane == 0) sh->coarse[c] = v;
     }
     cluster_sync<CL>();
     if (warp == 0) {   // the NB / 32 bins that hold the border, then the one, then its keys
@@ -357,7 +361,9 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
 #pragma unroll
       for (int e = 1; e < PER; ++e)
         if (at + value < want) { at += value; value = bv[e]; ++b; }
-      b = __shfl_sync(FULL_MASK, b, fl);
+      b = __shfl_sync(FULL_MASK, b, fl);   // the border's lane speaks for the warp: what follows is the warp's together
+      at = __shfl_sync(FULL_MASK, at, fl);
+      value = __shfl_sync(FULL_MASK, value, fl);
       // the bin's keys: bins do not grow with the key, so its ends are found by halving, 32 ways at a time
       uint32_t first, after;
       const uint32_t top_key = key_of(r.top);
@@ -374,7 +380,7 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
           return base;
         };
         first = b < NB - 1 ? least(b) : KEY_LOWEST;
-        after = b ? least(b - 1) : top_key + 1;
+        after = b && (MASS || !(quick || (allow_few && at + value <= MOST))) ? least(b - 1) : top_key + 1;   // where all from `first` on are listed, their end
       } else {
         after = hi - (b << shift) + 1;
         first = after - (1u << shift) < lo || after < (1u << shift) ? lo : after - (1u << shift);
@@ -393,7 +399,7 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
     if (!quick) want = sh->found[3] - before;
     if (level == 0) f.total = sh->found[4];
     // list the bin's tokens and, where counts say that it fits, those before it
-    const bool with_above = quick || (!MASS && allow_few && level == 0 && before + sh->found[2] <= CAP);
+    const bool with_above = quick || (!MASS && allow_few && level == 0 && before + sh->found[2] <= MOST);
     auto list = [&](bool bin, bool above) {
       uint32_t seen = 0;
 #pragma unroll 4
@@ -402,7 +408,7 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
         if (k < k0 || !among.keeps(k, r.base + i)) continue;
         if (k <= k1 ? bin : above) {
           const uint32_t q = atomicAdd(&sh->n_list, 1u);
-          if (q < CAP) sh->list[q] = token_word(k, r.base + i);
+          if (q < MOST) sh->list[q] = token_word(k, r.base + i);
         } else {
           ++seen;
         }
@@ -420,9 +426,9 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
       n_bin += remote<CL>(&sh->n_list, c);
       if (MASS) n_above += remote<CL>(&sh->n_above, c);
     }
-    if (n_bin <= CAP) {
+    if (n_bin <= MOST) {
       f.few = with_above;
-      if (MASS && allow_few && level == 0 && n_bin + n_above <= CAP) {
+      if (MASS && allow_few && level == 0 && n_bin + n_above <= MOST) {
         cluster_sync<CL>();   // the counts have been read
         list(false, true);
         cluster_sync<CL>();
@@ -430,13 +436,13 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
       }
       u64 x = gather<CL>(r, f.n);
       cluster_sync<CL>();   // lists and histograms have been read
-      x = sort_words(sh, x, static_cast<int>(f.n));
+      x = sort_words<MOST>(sh, x, static_cast<int>(f.n));
       f.word = x;
       if (f.few) return f;
       const uint32_t k = static_cast<uint32_t>(x >> 32);
       const u64 val = static_cast<uint32_t>(tid) < f.n ? (MASS ? r.mass(k) : 1ull) : 0ull;
       u64 t;
-      const u64 s = block_scan(sh, val, t);
+      const u64 s = block_scan<ST>(sh, val, t);
       if (s < want && s + val >= want) sh->found[5] = x;
       __syncthreads();
       const u64 w = sh->found[5];
@@ -461,8 +467,8 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
     if (lane == 0) sh->part[warp] = (static_cast<u64>(kmax) << 32) | kmin;
     __syncthreads();
     if (warp == 0) {
-      kmin = __reduce_min_sync(FULL_MASK, static_cast<uint32_t>(sh->part[lane]));
-      kmax = __reduce_max_sync(FULL_MASK, static_cast<uint32_t>(sh->part[lane] >> 32));
+      kmin = __reduce_min_sync(FULL_MASK, static_cast<uint32_t>(sh->part[lane % SW]));
+      kmax = __reduce_max_sync(FULL_MASK, static_cast<uint32_t>(sh->part[lane % SW] >> 32));
       if (lane == 0) sh->mine[1] = (static_cast<u64>(kmax) << 32) | kmin;
     }
     cluster_sync<CL>();
@@ -479,7 +485,7 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
       u64 c = 0, t, cl_total;
       const uint32_t i0 = min(tid * r.per_thread, r.n), i1 = min(i0 + r.per_thread, r.n);
       for (uint32_t i = i0; i < i1; ++i) c += key_of(r.x[i]) == lo && among.keeps(lo, r.base + i);
-      u64 s = block_scan(sh, c, t);
+      u64 s = block_scan<ST>(sh, c, t);
       s += cluster_scan<CL>(r, t, cl_total);
       if (tid == 0) sh->mine[2] = 0;
       __syncthreads();
@@ -503,7 +509,7 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
 
 // n logits from src into shared memory, which starts where the first 16-byte boundary of src falls on one there too; returns the
 // first's place. best: the thread's largest.
-template <typename T>
+template <int ST, typename T>
 CLB_DEV float *load_logits(const T *src, float *dst, uint32_t n, float &best) {
   constexpr uint32_t V = 16 / sizeof(T);
   auto clean = [&](float v) {   // NaN as -infinity, -0 as 0
@@ -530,8 +536,9 @@ CLB_DEV float *load_logits(const T *src, float *dst, uint32_t n, float &best) {
 }
 
 // One row by CL CTAs: its logits lie in their shared memory, a slice each, and are read from memory once.
-template <int CL>
-__global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, const uint32_t slice) {
+template <int CL, int ST>
+__global__ void __launch_bounds__(ST, 1024 / ST) sample_kernel(const clb200_sampling s, const uint32_t slice) {
+  constexpr int SW = ST / 32, MOST = ST < CAP ? ST : CAP;
   extern __shared__ __align__(16) uint8_t sm[];
   Shared *sh = reinterpret_cast<Shared *>(sm);
   float *room = reinterpret_cast<float *>(sh + 1);   // slice + 3
@@ -545,16 +552,16 @@ __global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, 
   if (tid < 128) sh->exp2_128[tid] = EXP2_128[tid];
   float best = -INFINITY;
   const int64_t at = row * s.stride + r.base;
-  if (s.type == T_F32) r.x = load_logits(static_cast<const float *>(s.logits) + at, room, r.n, best);
-  else if (s.type == T_F16) r.x = load_logits(static_cast<const __half *>(s.logits) + at, room, r.n, best);
-  else r.x = load_logits(static_cast<const __nv_bfloat16 *>(s.logits) + at, room, r.n, best);
+  if (s.type == T_F32) r.x = load_logits<ST>(static_cast<const float *>(s.logits) + at, room, r.n, best);
+  else if (s.type == T_F16) r.x = load_logits<ST>(static_cast<const __half *>(s.logits) + at, room, r.n, best);
+  else r.x = load_logits<ST>(static_cast<const __nv_bfloat16 *>(s.logits) + at, room, r.n, best);
   auto largest = [&](u64 v) {   // of the row's threads
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(FULL_MASK, v, o));
     __syncthreads();
     if (lane == 0) sh->part[tid >> 5] = v;
     __syncthreads();
-    v = sh->part[lane];
+    v = sh->part[lane % SW];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(FULL_MASK, v, o));
     if constexpr (CL > 1) {
@@ -604,14 +611,14 @@ __global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, 
   Limit lim{KEY_LOWEST, 0xffffffffu};
   if (by_k || by_p) {
     // each thread has several tokens and their largest ones are more than enough
-    const float *quick = by_k && k <= CAP / 2 && s.vocab >= 4 * CL * ST ? &best : nullptr;
-    Found f = by_k ? search<CL, false>(r, lim, static_cast<u64>(k), 0.0, true, quick) : search<CL, true>(r, lim, 0, static_cast<double>(share), true);
+    const float *quick = by_k && k <= MOST / 2 && s.vocab >= 4 * CL * ST ? &best : nullptr;
+    Found f = by_k ? search<CL, ST, false>(r, lim, static_cast<u64>(k), 0.0, true, quick) : search<CL, ST, true>(r, lim, 0, static_cast<double>(share), true);
     if (f.few) {   // the candidates, sorted, a thread each: the filters are prefixes, the draw goes by id
       const uint32_t q = static_cast<uint32_t>(f.word >> 32), id = 0xffffffffu - static_cast<uint32_t>(f.word);
       const bool cand = static_cast<uint32_t>(tid) < f.n && (!by_k || tid < k);
       double w = cand ? r.weight(logit_of(q)) : 0.0;
       u64 m = units(w), total, kept;
-      const u64 before = block_scan(sh, m, total);
+      const u64 before = block_scan<ST>(sh, m, total);
       if (by_p) {
         if (!by_k) total = f.total;
         const double x = ceil(static_cast<double>(share) * static_cast<double>(total));
@@ -620,13 +627,13 @@ __global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, 
       }
       if (w < min_w) m = 0;
       __syncthreads();
-      if (tid < CAP) sh->list[tid] = m;
+      if (tid < MOST) sh->list[tid] = m;
       __syncthreads();
       // by id: the complement of the id above, the place below
-      const u64 x = sort_words(sh, m ? (static_cast<u64>(0xffffffffu - id) << 32) | static_cast<uint32_t>(tid) : 0ull, by_k ? min(static_cast<int>(f.n), k) : static_cast<int>(f.n));
+      const u64 x = sort_words<MOST>(sh, m ? (static_cast<u64>(0xffffffffu - id) << 32) | static_cast<uint32_t>(tid) : 0ull, by_k ? min(static_cast<int>(f.n), k) : static_cast<int>(f.n));
       const uint32_t place = static_cast<uint32_t>(x);
-      m = x ? sh->list[place & (CAP - 1)] : 0;
-      const u64 s0 = block_scan(sh, m, kept);
+      m = x ? sh->list[place & (MOST - 1)] : 0;
+      const u64 s0 = block_scan<ST>(sh, m, kept);
       const u64 want = border(u, kept);
       if (r.rank == 0 && s0 <= want && want < s0 + m) {
         const uint32_t token = 0xffffffffu - static_cast<uint32_t>(x >> 32);
@@ -640,7 +647,7 @@ __global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, 
       return;
     }
     lim = f.lim;
-    if (by_k && by_p) lim = search<CL, true>(r, lim, 0, static_cast<double>(share), false).lim;
+    if (by_k && by_p) lim = search<CL, ST, true>(r, lim, 0, static_cast<double>(share), false).lim;
   }
   const bool every = lim.all();
   auto kept = [&](float x, uint32_t i) -> u64 {
@@ -666,7 +673,7 @@ __global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, 
 #pragma unroll
     for (int e = 0; e < E; ++e) mine += w[e] >= min_w ? units(w[e]) : 0ull;
   }
-  u64 before = block_scan(sh, mine, cta_total);
+  u64 before = block_scan<ST>(sh, mine, cta_total);
   before += cluster_scan<CL>(r, cta_total, total);
   const u64 want = border(u, total);
   if (before <= want && want < before + mine) {
@@ -681,12 +688,12 @@ __global__ void __launch_bounds__(ST, 1) sample_kernel(const clb200_sampling s, 
   cluster_sync<CL>();
 }
 
-template <int CL>
+template <int CL, int ST>
 cudaError_t launch_sample(const clb200_sampling &s, int device, cudaStream_t st) {
   const uint32_t slice = (static_cast<uint32_t>(s.vocab) + CL - 1) / CL;
   static bool done[64] = {};
   if (device >= 64 || !done[device]) {
-    const cudaError_t e = cudaFuncSetAttribute(sample_kernel<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, SAMPLE_SMEM);
+    const cudaError_t e = cudaFuncSetAttribute(sample_kernel<CL, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, SAMPLE_SMEM);
     if (e != cudaSuccess) return e;
     if (device < 64) done[device] = true;
   }
@@ -701,7 +708,7 @@ cudaError_t launch_sample(const clb200_sampling &s, int device, cudaStream_t st)
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<CL>, s, slice);
+  return cudaLaunchKernelEx(&cfg, sample_kernel<CL, ST>, s, slice);
 }
 
 int check(const clb200_sampling *s, char *err, size_t errlen) {
@@ -727,13 +734,18 @@ extern "C" int clb200_sample(clb200_ctx *c, const clb200_sampling *s, void *stre
   if (!c) { errf(err, errlen, "no context"); return 1; }
   if (s->rows == 0) return 0;
   const OnDevice on(c->device);
-  // the fewest CTAs a row that hold it, and more while the rows leave SMs idle: at 256 rows of 50304 a CTA a row takes @A@ us,
-  // eight @B@; one row of 151936 takes @C@ us with eight, @D@ with four
-  int cl = 1;
-  while (cl < 8 && ((s->vocab + cl - 1) / cl > static_cast<int>(MAX_SLICE) || (static_cast<int64_t>(s->rows) * cl * 2 <= c->sms && s->vocab >= 2048 * cl))) cl *= 2;
+  // A small vocabulary by a CTA of 256 threads, four to an SM (278 rows of 669: 14.5 us; 28.8 with 1024). Else the fewest CTAs of
+  // 1024 that hold a row, since the exchange costs more than it saves once the SMs are busy (256 rows of 50304: 89 us with one a
+  // row, 123 with two, 190 with four), and more of them for long rows while that leaves no row waiting (a GPC takes two clusters
+  // of eight: 17 rows of 151936 take 23 us with four each and 33 with eight; one takes 18.4 with eight; filters want few CTAs,
+  // sums over everything many: 8 rows of 14678 with top-k 17.4 us with one, 20.0 with four; 15 rows of 39554 without filters 15.6
+  // with one, 11.2 with four).
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : c->stream;
-  const cudaError_t e = cl == 1 ? launch_sample<1>(*s, c->device, st) : cl == 2 ? launch_sample<2>(*s, c->device, st)
-                        : cl == 4 ? launch_sample<4>(*s, c->device, st) : launch_sample<8>(*s, c->device, st);
+  int cl = 1;
+  while (cl < 8 && ((s->vocab + cl - 1) / cl > static_cast<int>(MAX_SLICE) || (static_cast<int64_t>(s->rows) * cl * 2 <= 128 && s->vocab >= 12288 * cl))) cl *= 2;
+  const cudaError_t e = s->vocab <= SMALL_VOCAB ? launch_sample<1, 256>(*s, c->device, st) : cl == 1 ? launch_sample<1, 1024>(*s, c->device, st)
+                        : cl == 2 ? launch_sample<2, 1024>(*s, c->device, st) : cl == 4 ? launch_sample<4, 1024>(*s, c->device, st)
+                                                                                        : launch_sample<8, 1024>(*s, c->device, st);
   CUDA_OR(e, "launching the sampling");
   return 0;
 }
