@@ -12,6 +12,8 @@
 //           sequence's end come from outside the tensor, as zeros, except inside the last box;
 //   MMA     (one warp): S_w = Q_w K^T (both operands in shared memory), O_w += P_w V (P_w from TMEM). While group 0 works on
 //           its scores the tensor cores run the other stream's products.
+// With heads of 256 elements O takes half of the TMEM: there is one stream, and its scores have two buffers that take turns, so
+// that the next tile's are computed while the softmax is at this one's.
 // The maximum that scales a row's sums is only moved when the row's maximum has grown by more than 2^8 (the probabilities then
 // reach 2^8 at most, far inside fp16 and fp32), so rescaling O_w, a round trip through the registers, is rare.
 // The values of positions past the sequence's end inside the last box may be anything, and 0 x NaN is NaN: the keys' warp zeroes
@@ -36,7 +38,7 @@ struct TcAttn {
   static constexpr uint32_t Q_TILE = 128 * HD * 2, STAGE = N * HD * 2;
   static constexpr int STAGES = HD == 64 ? 8 : 4;
   static constexpr uint32_t OUT = 4096;                      // a softmax warp's buffer for 32 rows on their way out, 128 bytes each
-  static constexpr int N_BARS = 3 * STAGES + 6 * STREAMS + 2 * 4 + 1;
+  static constexpr int N_BARS = 3 * STAGES + 3 * STREAMS + 8 + 2 * 4 + 1;
   static constexpr uint32_t SMEM = 1024 + STREAMS * Q_TILE + STAGES * STAGE + 4 * STREAMS * OUT + 8 * N_BARS + 16;
   static constexpr uint32_t S_COL = 0, O_COL = 256;          // S_w at 128 w (P_w over its first half), O_w at 256 + HD w
   static_assert(SMEM <= 232448, "shared memory budget");
@@ -97,8 +99,8 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
   uint8_t *ring = sm + ST * S::Q_TILE;
   uint8_t *out_sm = ring + S::STAGES * S::STAGE;
   uint64_t *kv_full = reinterpret_cast<uint64_t *>(out_sm + 4 * ST * S::OUT), *kv_free = kv_full + S::STAGES;
-  uint64_t *q_full = kv_free + S::STAGES, *q_free = q_full + ST, *s_full = q_free + ST, *p_half = s_full + ST, *o_full = p_half + 2 * ST;
-  uint64_t *item_full = o_full + ST, *item_free = item_full + ITEMS, *v_whole = item_free + ITEMS, *mma_done = v_whole + S::STAGES;
+  uint64_t *q_full = kv_free + S::STAGES, *q_free = q_full + ST, *s_full = q_free + ST, *p_half = s_full + 2, *o_full = p_half + 4, *pv_done = o_full + ST;
+  uint64_t *item_full = pv_done + 2, *item_free = item_full + ITEMS, *v_whole = item_free + ITEMS, *mma_done = v_whole + S::STAGES;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
   const clb200_attn &a = g.a;
@@ -114,10 +116,13 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
     for (int w = 0; w < ST; ++w) {
       mbar_init(&q_full[w], 1);
       mbar_init(&q_free[w], 1);
+      mbar_init(&o_full[w], 1);
+    }
+    for (int w = 0; w < 2; ++w) {
       mbar_init(&s_full[w], 1);
+      mbar_init(&pv_done[w], 1);
       mbar_init(&p_half[2 * w], 4);
       mbar_init(&p_half[2 * w + 1], 4);
-      mbar_init(&o_full[w], 1);
     }
     for (int i = 0; i < ITEMS; ++i) { mbar_init(&item_full[i], 1); mbar_init(&item_free[i], 4 * ST + 3); }   // warps that read items
     mbar_init(mma_done, 1);
@@ -239,11 +244,11 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
       const uint32_t q_lo = tc::sw128_lo(smem_addr(sm)), k_lo = tc::sw128_lo(smem_addr(ring)), v_lo = tc::sw128_lo(smem_addr(ring), N * 128);
       uint32_t st = 0, round = 0, q_cnt[2] = {0, 0}, p_cnt[2] = {0, 0};   // the next stage and its phase; items and tiles consumed
       uint32_t tails = 0;                                                   // the phase of each stage's v_whole
-      auto scores = [&](int w, uint32_t k) {   // S_w = Q_w K^T
+      auto scores = [&](int w, int b, uint32_t k) {   // S_b = Q_w K^T
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
-          tc::mma_ss(tmem + S::S_COL + 128 * w, q_lo + w * (S::Q_TILE / 16) + (kk / 4) * (128 * 128 / 16) + 2 * (kk % 4), k + (kk / 4) * (N * 128 / 16) + 2 * (kk % 4), ID_S, kk != 0);
-        tc::commit(&s_full[w]);
+          tc::mma_ss(tmem + S::S_COL + 128 * b, q_lo + w * (S::Q_TILE / 16) + (kk / 4) * (128 * 128 / 16) + 2 * (kk % 4), k + (kk / 4) * (N * 128 / 16) + 2 * (kk % 4), ID_S, kk != 0);
+        tc::commit(&s_full[b]);
       };
       auto stage = [&]() {   // the next stage, once it is full
         const uint32_t k = st;
@@ -265,7 +270,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
           if (w == 1 && !two) break;
           if (!wait_bar(&q_full[w], q_cnt[w]++ & 1)) ok = false;
           if (!ok) break;
-          scores(w, k_lo + ks * (S::STAGE / 16));
+          scores(w, ST == 1 ? p_cnt[0] & 1 : w, k_lo + ks * (S::STAGE / 16));
           if (n == 1) tc::commit(&q_free[w]);
         }
         if (!ok) break;
@@ -273,6 +278,13 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
         for (int j = 0; j < n; ++j) {
           const bool more = j + 1 < n;
           if (more) ks = stage();
+          if constexpr (ST == 1) {   // the next tile's scores, in the other buffer, while the softmax is at this one's
+            if (more && ok) {
+              scores(0, (p_cnt[0] + 1) & 1, k_lo + ks * (S::STAGE / 16));
+              tc::commit(&kv_free[ks]);
+              if (j + 2 == n) tc::commit(&q_free[0]);
+            }
+          }
           vs = stage();
           if (tail && !more) {
             if (!wait_bar(&v_whole[vs], (tails >> vs) & 1)) ok = false;
@@ -285,23 +297,30 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
             if (w == 1 && !two) break;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (!wait_bar(&p_half[2 * w + h], p_cnt[w] & 1)) ok = false;
+              // (one stream: the buffers take turns, each with its own barriers and every other tile)
+              const int b = ST == 1 ? p_cnt[0] & 1 : w;
+              if (!wait_bar(&p_half[2 * b + h], (ST == 1 ? p_cnt[0] >> 1 : p_cnt[w]) & 1)) ok = false;
               if (!ok) break;
               tc::fence_after_sync();
 #pragma unroll
               for (int kk = 0; kk < N / 32; ++kk)
-                tc::mma_ts(tmem + S::O_COL + HD * w, tmem + S::S_COL + 128 * w + 8 * (N / 32 * h + kk), v + 128 * (N / 32 * h + kk), ID_O,
+                tc::mma_ts(tmem + S::O_COL + HD * w, tmem + S::S_COL + 128 * b + 8 * (N / 32 * h + kk), v + 128 * (N / 32 * h + kk), ID_O,
                            (h != 0 || kk != 0) ? true : j != 0);
             }
             ++p_cnt[w];
             if (!ok) break;
-            if (more) scores(w, k);
-            else tc::commit(&o_full[w]);
-            if (j + 2 == n) tc::commit(&q_free[w]);
+            if constexpr (ST == 1) {
+              tc::commit(&pv_done[(p_cnt[0] - 1) & 1]);
+              if (!more) tc::commit(&o_full[0]);
+            } else {
+              if (more) scores(w, w, k);
+              else tc::commit(&o_full[w]);
+              if (j + 2 == n) tc::commit(&q_free[w]);
+            }
           }
           if (!ok) break;
           tc::commit(&kv_free[vs]);
-          if (more) tc::commit(&kv_free[ks]);
+          if (ST == 2 && more) tc::commit(&kv_free[ks]);
         }
         if (!ok) break;
       }
@@ -312,7 +331,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
     if constexpr (ST == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int w = warp >> 2, r = tid & 127, tr = attn_token(g, r);
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-    const uint32_t s_col = tmem + lanes + S::S_COL + 128 * w, o_col = tmem + lanes + S::O_COL + HD * w;
+    const uint32_t s_col0 = tmem + lanes + S::S_COL + 128 * w, o_col = tmem + lanes + S::O_COL + HD * w;
     const float sc = a.scale * LOG2E;
     uint32_t o_cnt = 0, s_cnt = 0;
     TcItem x_;
@@ -324,7 +343,10 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
       float m = -INFINITY;
       float2 l0 = make_float2(0.f, 0.f), l1 = l0;
       for (int j = 0; j < x.n; ++j) {
-        if (!wait_bar(&s_full[w], s_cnt++ & 1)) { ok = false; break; }
+        const int b = ST == 1 ? s_cnt & 1 : w;   // the buffer
+        const uint32_t s_col = ST == 1 ? s_col0 + 128 * b : s_col0;
+        if (!wait_bar(&s_full[b], (ST == 1 ? s_cnt >> 1 : s_cnt) & 1)) { ok = false; break; }
+        ++s_cnt;
         tc::fence_after_sync();
         uint32_t xr[N];
         float *v = reinterpret_cast<float *>(xr);
@@ -355,7 +377,11 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
           const float mb = fmaxf(m, mn), f = m == -INFINITY ? 0.f : exp2_approx(m - mb);
           m = mb;
           l0.x *= f; l0.y *= f; l1.x *= f; l1.y *= f;
-          if (j > 0) {   // the products before this tile's scores are complete: O_w is at rest
+          if (j > 0) {   // O_w is at rest once the products before this tile are complete: they came before its scores, or are waited for
+            // one stream: tile s_cnt - 2's products, on the barrier of its buffer (the tile before it there was done long before
+            // this tile's scores: a parity tells one phase from the next only)
+            if (ST == 1 && !wait_bar(&pv_done[s_cnt & 1], ((s_cnt - 2) >> 1) & 1)) { ok = false; break; }
+            if (ST == 1) tc::fence_after_sync();
 #pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {
               uint32_t o[32];
@@ -391,7 +417,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
           tc::wait_st();
           tc::fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_half[2 * w + h]);
+          if (lane == 0) mbar_arrive(&p_half[2 * b + h]);
         }
       }
       if (!ok) break;
