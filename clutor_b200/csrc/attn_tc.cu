@@ -14,6 +14,11 @@
 //           its scores the tensor cores run the other stream's products.
 // With heads of 256 elements O takes half of the TMEM: there is one stream, and its scores have two buffers that take turns, so
 // that the next tile's are computed while the softmax is at this one's.
+// What bounds it: a tile of one stream is 1024 cycles of products (heads of 128), 16384 exponentials (1024 cycles of the
+// special-function units, a quarter of them moved to the FMA pipes) and about 900 more of reading, comparing and writing, so two
+// streams keep the tensor cores at most busy and the softmax is never far behind. Measured: 2940 cycles for a tile of both streams
+// where the products need 2048; a prompt of 8192, 32 heads over 4 of 128, bf16: 439 to 452 us, 1.22 PFLOP/s (73 % of the measured
+// burst rate), and 521 to 531 us in long runs, where the power cap lowers the clock.
 // The maximum that scales a row's sums is only moved when the row's maximum has grown by more than 2^8 (the probabilities then
 // reach 2^8 at most, far inside fp16 and fp32), so rescaling O_w, a round trip through the registers, is rare.
 // The values of positions past the sequence's end inside the last box may be anything, and 0 x NaN is NaN: the keys' warp zeroes
