@@ -468,9 +468,8 @@ class Context:
             self._on_device(pages.k, q)
         st = self._raw_stream(stream)
         if out is None:
-            odt = out_dtype or dt
-            out = _empty((T, H, D), odt, q.device, stream)
-            out_row = H * D
+            odt, out_row = out_dtype or dt, H * D
+            out = _like(q) if odt is dt and stream is None and q.is_contiguous() else _empty((T, H, D), odt, q.device, stream)
         elif out.shape != (T, H, D) or (out_dtype is not None and out.dtype is not out_dtype) or out.get_device() != device:
             raise ClutorError(f"out must be {[T, H, D]} of {out_dtype or out.dtype} on cuda:{device}")
         else:
@@ -543,18 +542,18 @@ _ATTN = struct.Struct("@iiiPqPIqfiiPN0q")
 _SAMPLING = struct.Struct("@iiIPqPPPPPPP0q")
 _TYPES: dict = {}   # torch types to ggml type ids
 # of torch, which is imported when the first of these calls is prepared: its types, its allocator, and the raw handle of a current stream
-_float32 = _int32 = _uint8 = _new = _current_stream = None
+_float32 = _int32 = _uint8 = _new = _like = _current_stream = None
 
 
 def _use_torch() -> None:
-    global _float32, _int32, _uint8, _new, _current_stream
+    global _float32, _int32, _uint8, _new, _like, _current_stream
     if _new is None:
         try:
             import torch
         except ImportError:   # the calls on host arrays do without
             return
         _TYPES.update({torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16})
-        _float32, _int32, _uint8, _new = torch.float32, torch.int32, torch.uint8, torch.empty
+        _float32, _int32, _uint8, _new, _like = torch.float32, torch.int32, torch.uint8, torch.empty, torch.empty_like
         _current_stream = torch._C._cuda_getCurrentRawStream
 
 

@@ -20,9 +20,11 @@ namespace {
 // Up to 16 x MT rows (new tokens x query heads of a key/value head): bound by the bytes of the cache, each read once. A warp
 // takes 16 positions of every tile of 64 through a ring of its own (cp.async, so positions past the sequence's end come as zeros
 // whatever the slots hold) and keeps its own (m, l, values) for them, so warps do not wait on one another inside an item; their
-// states are joined at its end. Products on m16n8k16: at 8 of 16 rows in use they are far from the limit, while eight warps an SM
-// with two stages each on their way cover HBM's latency. 64 sequences of up to 8000 positions, 32 heads over 4 of 128: 106 us =
-// 5.98 TB/s, 91 % of the measured copy rate; one token over 500 positions 9.7 us with the join.
+// states are joined at its end, under the first loads of the next item (200 sequences of up to 300 positions, 32 heads over 8:
+// 40 us, 45 with those loads behind the join; the states handed from warp to warp through one buffer instead: 50). Products on
+// m16n8k16: at 8 of 16 rows in use they are far from the limit, while eight warps an SM with two stages each on their way cover
+// HBM's latency. 64 sequences of up to 8000 positions, 32 heads over 4 of 128: 105 us = 6.05 TB/s, 92 % of the measured copy
+// rate; one token over 500 positions 9.5 us with the join.
 constexpr int RT = 128, RW = RT / 32, RN = 16 * RW;   // threads, warps, positions per tile (16 per warp)
 
 template <int HD, int MT>
@@ -30,10 +32,11 @@ struct RowsShape {
   static constexpr int ROWS = 16 * MT;
   static constexpr int STAGES = HD == 64 ? 6 : 3;
   static constexpr uint32_t HALF = 16 * HD * 2, STAGE = 2 * HALF;         // a warp's keys (then values) of one tile
-  static constexpr uint32_t Q = ROWS * HD * 2, KV = RW * STAGES * STAGE;  // KV: also the warps' states when they are joined
-  static constexpr uint32_t SMEM = Q + KV + 2 * RW * ROWS * 4;
+  static constexpr uint32_t Q = ROWS * HD * 2, KV = RW * STAGES * STAGE;
+  static constexpr uint32_t SMEM = Q + KV + RW * 16 * 8;
   static constexpr int PER_SM = HD == 256 ? 1 : 2;
-  static_assert(RW * ROWS * HD * 4 <= static_cast<int>(KV), "the joined states fit the stages");
+  static_assert(16 * HD * 4 <= STAGE, "a warp's values of 16 rows fit a stage");
+  static_assert((ATTN_MAX_SEQ + 1) * 8 <= static_cast<int>(KV), "the prefix sums fit the stages");
 };
 
 CLB_DEV void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -61,58 +64,62 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
   constexpr int KK = HD / 16, ROWS = S::ROWS;
   constexpr bool QREG = MT * KK <= 8;   // the query fragments stay in registers
   extern __shared__ __align__(128) uint8_t sm[];
-  __shared__ int64_t prefix[ATTN_MAX_SEQ + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
   const clb200_attn &a = g.a;
   const clb200_kv &kv = g.kv;
   const uint32_t q_sm = smem_addr(sm), kv_sm = q_sm + S::Q + warp * S::STAGES * S::STAGE;
-  float *join = reinterpret_cast<float *>(sm + S::Q), *join_m = reinterpret_cast<float *>(sm + S::Q + S::KV), *join_l = join_m + RW * ROWS;
+  float2 *states = reinterpret_cast<float2 *>(sm + S::Q + S::KV);   // [RW][16] a warp's maximum and sum of a row
   const float sc = a.scale * LOG2E;
   const int gr = lane >> 2, gc = (lane & 3) * 2;   // the lane's row and first column in an accumulator
   if (tid == 0) g.joins[cta] = make_int4(0, 0, 0, 0);
+  int64_t *prefix = reinterpret_cast<int64_t *>(sm + S::Q);
   attn_prefix<RN>(g, prefix, cta);
   AttnRun<RN> run;
   run.init(g, prefix, cta);
-  while (run.more()) {
-    const AttnSeq q = run.q;
-    const AttnSpan span = attn_span<RN>(g, q, run.qt);
-    const int i0 = run.first(g), n = run.tiles(g, span), t0 = run.qt * g.tpi, head = run.head, s = run.s;
-    const bool whole = n == span.nt;
-    if (n == 0) {   // the run ends in the item's lead
-      run.advance(g, span);
-      continue;
-    }
-    __syncthreads();   // the last item's queries and joined states have been read
-    for (int i = tid; i < ROWS * (HD / 8); i += RT) {
-      const int r = i / (HD / 8), c = i % (HD / 8), tr = attn_token(g, r), t = t0 + tr, h = head * g.group + r - tr * g.group;
-      const bool live = r < g.tpi * g.group && t < q.nq;
-      const C *src = static_cast<const C *>(a.q) + (live ? (q.row + t) * a.q_stride + h * HD + 8 * c : 0);
-      cp_async16(q_sm + chunk_at<HD>(r, c), src, live);
-    }
-    cp_commit();
-    // this warp's 16 positions of tile i of the item
-    auto issue = [&](int i) {
-      if (i < n) {
-        const int j0 = span.tile(i0 + i) * RN + warp * 16;
-        if (j0 <= span.hi) {
-          const AttnSlot at0 = attn_slot(g, s, j0);
-          const int page = at0.page;
-          const int64_t base = (page < 0 ? 0 : page * kv.page_stride + at0.slot * kv.slot_stride) + head * kv.head_stride;
-          const uint32_t dst = kv_sm + (i % S::STAGES) * S::STAGE;
-          const int left = page < 0 ? 0 : q.kv - j0;   // positions behind the sequence's end come as zeros
+  __syncthreads();   // the prefix sums have been read: the stages take their place
+  AttnSpan span;
+  int n = 0, i0 = 0, base = 0;   // the item's tiles, its first, and the stage of that one
+  auto issue = [&](int i) {   // this warp's 16 positions of tile i of the item
+    if (i < n) {
+      const int j0 = span.tile(i0 + i) * RN + warp * 16;
+      if (j0 <= span.hi) {
+        const AttnSlot at0 = attn_slot(g, run.s, j0);
+        const int64_t from = (at0.page < 0 ? 0 : at0.page * kv.page_stride + at0.slot * kv.slot_stride) + run.head * kv.head_stride;
+        const uint32_t dst = kv_sm + (base + i) % S::STAGES * S::STAGE;
+        const int left = at0.page < 0 ? 0 : run.q.kv - j0;   // positions behind the sequence's end come as zeros
 #pragma unroll
-          for (int e = lane; e < 16 * (HD / 8); e += 32) {
-            const int r = e / (HD / 8), c = e % (HD / 8);
-            const int64_t at = r < left ? base + r * kv.slot_stride + 8 * c : 0;
-            cp_async16(dst + chunk_at<HD>(r, c), static_cast<const C *>(kv.k) + at, r < left);
-            cp_async16(dst + S::HALF + chunk_at<HD>(r, c), static_cast<const C *>(kv.v) + at, r < left);
-          }
+        for (int e = lane; e < 16 * (HD / 8); e += 32) {
+          const int r = e / (HD / 8), c = e % (HD / 8);
+          const int64_t at = r < left ? from + r * kv.slot_stride + 8 * c : 0;
+          cp_async16(dst + chunk_at<HD>(r, c), static_cast<const C *>(kv.k) + at, r < left);
+          cp_async16(dst + S::HALF + chunk_at<HD>(r, c), static_cast<const C *>(kv.v) + at, r < left);
         }
       }
-      cp_commit();
-    };
+    }
+    cp_commit();
+  };
+  // The next item with tiles for this CTA becomes the current one; its queries and first tiles are sent for.
+  auto begin = [&]() {   // false at the end of the run
+    for (n = 0; run.more(); run.advance(g, span)) {
+      span = attn_span<RN>(g, run.q, run.qt);
+      i0 = run.first(g);
+      n = run.tiles(g, span);
+      if (n) break;   // else the run ends in the item's lead
+    }
+    if (n == 0) return false;
+    const int t0 = run.qt * g.tpi;
+    for (int i = tid; i < ROWS * (HD / 8); i += RT) {
+      const int r = i / (HD / 8), c = i % (HD / 8), tr = attn_token(g, r), t = t0 + tr, h = run.head * g.group + r - tr * g.group;
+      const bool live = r < g.tpi * g.group && t < run.q.nq;
+      cp_async16(q_sm + chunk_at<HD>(r, c), static_cast<const C *>(a.q) + (live ? (run.q.row + t) * a.q_stride + h * HD + 8 * c : 0), live);
+    }
+    cp_commit();
 #pragma unroll
     for (int i = 0; i < S::STAGES - 1; ++i) issue(i);
+    return true;
+  };
+  bool more = begin();
+  while (more) {
     cp_wait<S::STAGES - 1>();   // the queries
     __syncthreads();
     uint32_t qf[QREG ? MT : 1][QREG ? KK : 1][4];
@@ -139,7 +146,7 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
       __syncwarp();
       const int j0 = span.tile(i0 + i) * RN + warp * 16;
       if (j0 <= span.hi) {
-        const uint32_t ks = kv_sm + (i % S::STAGES) * S::STAGE, vs = ks + S::HALF;
+        const uint32_t ks = kv_sm + (base + i) % S::STAGES * S::STAGE, vs = ks + S::HALF;
         float x[MT][2][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -221,55 +228,59 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
       __syncwarp();   // the stage has been read by every lane
       issue(i + S::STAGES - 1);
     }
-    cp_wait<0>();
-    if (run.at + span.nt + g.lead - run.u0 >= run.end) grid_launch_dependents();
-    // the warps' states: maximum and sum of each row, values in fp32, joined in warp order
+    // what the join needs of this item, then the next one's first loads
+    const int row = run.q.row + run.qt * g.tpi, tokens = min(g.tpi, run.q.nq - run.qt * g.tpi), head = run.head;
+    const bool whole = n == span.nt;
+    const int slot = 2 * cta + (i0 == 0 ? 1 : 0);
+    if (!whole && i0 == 0 && tid == 0) g.joins[cta] = make_int4(row, tokens, head, run.pieces(span.nt - n));
+    base = (base + n) % S::STAGES;
+    run.advance(g, span);
+    // The warps' states (maximum and sum of each row, values in fp32), 16 rows at a time, each in the stage that the warp's next
+    // item takes last; then joined in warp order.
+    const uint32_t spare = (base + S::STAGES - 1) % S::STAGES * S::STAGE;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int mt = 0; mt < MT; ++mt) {
+      float *mine = reinterpret_cast<float *>(sm + S::Q + warp * S::STAGES * S::STAGE + spare);
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         l[mt][w] += __shfl_xor_sync(FULL_MASK, l[mt][w], 1);
         l[mt][w] += __shfl_xor_sync(FULL_MASK, l[mt][w], 2);
-        if ((lane & 3) == 0) {
-          join_m[warp * ROWS + 16 * mt + gr + 8 * w] = m[mt][w];
-          join_l[warp * ROWS + 16 * mt + gr + 8 * w] = l[mt][w];
+        if ((lane & 3) == 0) states[warp * 16 + gr + 8 * w] = make_float2(m[mt][w], l[mt][w]);
+#pragma unroll
+        for (int d = 0; d < HD / 8; ++d)   // four rows' pairs in four groups of banks
+          *reinterpret_cast<float2 *>(mine + (gr + 8 * w) * HD + 8 * (d ^ (gr & 3)) + gc) = make_float2(o[mt][d][2 * w], o[mt][d][2 * w + 1]);
+      }
+      __syncthreads();   // (the queries, too, have been read)
+      if (mt == 0) {
+        more = begin();
+        if (!more) grid_launch_dependents();
+      }
+      for (int i = tid; i < 16 * (HD / 4); i += RT) {
+        const int rr = i / (HD / 4), c = 4 * (i % (HD / 4)), r = 16 * mt + rr, tr = attn_token(g, r);
+        if (r >= g.tpi * g.group || tr >= tokens) continue;
+        float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+        for (int w = 0; w < RW; ++w) mm = fmaxf(mm, states[w * 16 + rr].x);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < RW; ++w) {
+          const float2 st = states[w * 16 + rr];
+          const float f = st.x == -INFINITY ? 0.f : exp2_approx(st.x - mm);
+          const float4 u = *reinterpret_cast<const float4 *>(sm + S::Q + w * S::STAGES * S::STAGE + spare + 4 * (rr * HD + (c ^ ((rr & 3) << 3))));
+          ll = fmaf(f, st.y, ll);
+          v.x = fmaf(f, u.x, v.x); v.y = fmaf(f, u.y, v.y); v.z = fmaf(f, u.z, v.z); v.w = fmaf(f, u.w, v.w);
+        }
+        if (whole) {
+          store4<O>(static_cast<O *>(a.out) + (row + tr) * a.out_stride + (head * g.group + r - tr * g.group) * HD + c, v, ll > 0.f ? 1.0f / ll : 0.f);
+        } else {
+          *reinterpret_cast<float4 *>(g.piece_o + (static_cast<int64_t>(slot) * g.rows + r) * HD + c) = v;
+          if (c == 0) g.piece_ml[static_cast<int64_t>(slot) * g.rows + r] = make_float2(mm, ll);
         }
       }
-    __syncthreads();   // every warp's stages are free
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int d = 0; d < HD / 8; ++d)
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
-          *reinterpret_cast<float2 *>(join + (warp * ROWS + 16 * mt + gr + 8 * w) * HD + 8 * d + gc) = make_float2(o[mt][d][2 * w], o[mt][d][2 * w + 1]);
-    __syncthreads();
-    const int slot = 2 * cta + (i0 == 0 ? 1 : 0);
-    for (int i = tid; i < ROWS * (HD / 4); i += RT) {
-      const int r = i / (HD / 4), c = 4 * (i % (HD / 4)), tr = attn_token(g, r), t = t0 + tr;
-      if (r >= g.tpi * g.group || t >= q.nq) continue;
-      float mm = -INFINITY, ll = 0.f;
-#pragma unroll
-      for (int w = 0; w < RW; ++w) mm = fmaxf(mm, join_m[w * ROWS + r]);
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < RW; ++w) {
-        const float mw = join_m[w * ROWS + r], f = mw == -INFINITY ? 0.f : exp2_approx(mw - mm);
-        const float4 u = *reinterpret_cast<const float4 *>(join + (w * ROWS + r) * HD + c);
-        ll = fmaf(f, join_l[w * ROWS + r], ll);
-        v.x = fmaf(f, u.x, v.x); v.y = fmaf(f, u.y, v.y); v.z = fmaf(f, u.z, v.z); v.w = fmaf(f, u.w, v.w);
-      }
-      if (whole) {
-        const float inv = ll > 0.f ? 1.0f / ll : 0.f;
-        store4<O>(static_cast<O *>(a.out) + (q.row + t) * a.out_stride + (head * g.group + r - tr * g.group) * HD + c, v, inv);
-      } else {
-        *reinterpret_cast<float4 *>(g.piece_o + (static_cast<int64_t>(slot) * g.rows + r) * HD + c) = v;
-        if (c == 0) g.piece_ml[static_cast<int64_t>(slot) * g.rows + r] = make_float2(mm, ll);
-      }
+      if (mt + 1 < MT) __syncthreads();   // these have been read
     }
-    if (!whole && i0 == 0 && tid == 0) g.joins[cta] = make_int4(q.row + t0, min(g.tpi, q.nq - t0), head, run.pieces(span.nt - n));
-    run.advance(g, span);
   }
+  cp_wait<0>();
 }
 
 // ---- joining the pieces of items that fell into several runs ---------------------------------------------------------------
@@ -475,7 +486,7 @@ extern "C" int clb200_attention(clb200_ctx *c, const clb200_kv *kv, const clb200
     g.tpi = p.tpi;
     g.nc = p.nc;
     g.min_run = p.rows <= 32 ? 1 : 2;
-    g.lead = p.rows <= 32 ? 4 : 2;
+    g.lead = p.rows <= 32 ? 3 : 2;   // (200 short sequences 40.0 us, 40.4 with 4; 64 of 32 heads over 32: 116, 122 with 2)
     g.piece_o = reinterpret_cast<float *>(w);
     g.piece_ml = reinterpret_cast<float2 *>(w + p.off_ml);
     g.joins = reinterpret_cast<int4 *>(w + p.off_joins);
