@@ -82,7 +82,7 @@ struct Shared {
   u64 mine[4];               // what this CTA tells the others
   u64 found[7];              // what a search found, for the CTA's threads
   uint32_t n_list, n_above;
-  double exp2_128[128];      // 2^(i / 128)
+  double exp2_128[128];      // 2^(i / 128), i << 13 taken from the upper word
 };
 static_assert(sizeof(Shared) % 16 == 0, "the logits follow on a 16-byte boundary");
 
@@ -127,18 +127,21 @@ struct Row {
   float *x;              // [n] logits of tokens [base, base + n): NaN as -infinity, no -0
   uint32_t n, base, rank, per_thread;
   float top, half_top, inv_f;   // the largest logit (finite), half of it; 1 / temperature
+  float floor;           // logits up to this weigh nothing
   double top_d, scale;   // log2(e) / temperature
 
   // (top - x) / (2 temperature): halved so that it does not overflow; NaN for infinity x 0.
   CLB_DEV float distance(float v) const { return __fmul_rn(fmaf(v, -0.5f, half_top), inv_f); }
   // exp((x - top) / temperature) = 2^y with y = n / 128 + r: 2^(n/128) from a table and 2^r by its series (|r| <= 1 / 256: the
-  // first term left out is below 1.3e-15), the table-driven method of Tang (1989). Weights below 2^-45 count as 0. COUNT at once
-  // and without branches: one alone is a chain of a dozen dependent double-precision operations.
+  // first term left out is below 1.3e-15), the table-driven method of Tang (1989). COUNT at once and without branches: one alone is
+  // a chain of a dozen dependent double-precision operations. What bounds them is the ALU pipe (compares, selects, logic), which
+  // takes a warp's instruction in two cycles: so the table's entries have i << 13 taken from their upper words, and n << 13 added
+  // to one gives 2^(n/128) in a single multiply-add.
   template <int COUNT>
   CLB_DEV void weights(const float (&v)[COUNT], double (&w)[COUNT]) const {
     double y[COUNT], t[COUNT];
 #pragma unroll
-    for (int e = 0; e < COUNT; ++e) y[e] = (static_cast<double>(v[e]) - top_d) * scale;
+    for (int e = 0; e < COUNT; ++e) y[e] = (static_cast<double>(v[e] > floor ? v[e] : top) - top_d) * scale;
 #pragma unroll
     for (int e = 0; e < COUNT; ++e) t[e] = fma(y[e], 128.0, 6755399441055744.0);   // 1.5 * 2^52: the nearest integer in the low bits
 #pragma unroll
@@ -150,11 +153,11 @@ struct Row {
 #pragma unroll
     for (int e = 0; e < COUNT; ++e) w[e] = fma(w[e], y[e], 0.6931471805599453);
 #pragma unroll
-    for (int e = 0; e < COUNT; ++e) w[e] = fma(w[e], y[e], 1.0) * sh->exp2_128[__double2loint(t[e]) & 127];
-#pragma unroll
     for (int e = 0; e < COUNT; ++e) {
-      const double u = __hiloint2double(__double2hiint(w[e]) + (__double2loint(t[e]) >> 7) * (1 << 20), __double2loint(w[e]));
-      w[e] = distance(v[e]) < 16.f ? u : 0.0;
+      const int n = __double2loint(t[e]);
+      const double p = sh->exp2_128[n & 127];
+      // what weighs nothing keeps the lower word alone: below 2^-1022
+      w[e] = fma(w[e], y[e], 1.0) * __hiloint2double(v[e] > floor ? n * 8192 + __double2hiint(p) : 0, __double2loint(p));
     }
   }
   CLB_DEV double weight(float v) const {
@@ -167,7 +170,7 @@ struct Row {
   // (top - x) / temperature in bins: equal or larger for smaller logits, so a bin holds one run of the order.
   CLB_DEV uint32_t bin(float v) const {
     const float d = __fmul_rn(distance(v), 2.f * BINS_PER_NAT);
-    return d < static_cast<float>(NB - 1) ? static_cast<uint32_t>(d) : static_cast<uint32_t>(NB - 1);
+    return static_cast<uint32_t>(fminf(d, static_cast<float>(NB - 1)));
   }
 };
 
@@ -295,25 +298,28 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
     if (tid == 0) { sh->n_list = 0; sh->n_above = 0; }
     __syncthreads();
     if (MASS) {
-      for (uint32_t i = tid; i < r.n; i += E * ST) {
+      auto weigh = [&](uint32_t i, bool end) {
         float x[E];
         double w[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {   // what does not belong here weighs nothing
           const uint32_t q = i + e * ST;
-          x[e] = q < r.n ? r.x[q] : -INFINITY;
-          if (!inside(x[e], q)) x[e] = -INFINITY;
+          x[e] = !end || q < r.n ? r.x[q] : -INFINITY;
+          if (!whole && !inside(x[e], q)) x[e] = -INFINITY;
         }
         r.weights(x, w);
 #pragma unroll
         for (int e = 0; e < E; ++e) {   // in 32-bit halves with the carry, since only those add in one instruction
+          if (!(x[e] > r.floor)) continue;
           const u64 m = units(w[e]);
-          if (!m) continue;
           const uint32_t b = place(x[e]), l = static_cast<uint32_t>(m);
           const uint32_t up = static_cast<uint32_t>(m >> 32) + (atomicAdd(&sh->lo[b], l) > ~l ? 1u : 0u);
           if (up) atomicAdd(&sh->hi[b], up);
         }
-      }
+      };
+      uint32_t i = tid;
+      for (; i + (E - 1) * ST < r.n; i += E * ST) weigh(i, false);
+      if (i < r.n) weigh(i, true);
     } else if (quick) {
       atomicAdd(&sh->lo[r.bin(*largest)], 1u);
     } else {
@@ -374,19 +380,22 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
       uint32_t first, after;
       const uint32_t top_key = key_of(r.top);
       if (level == 0) {
-        auto least = [&](uint32_t most) {   // the smallest key whose bin is at most `most`
-          uint32_t base = 0;
+        // the smallest key whose bin is at most b, and the smallest of the bins before it
+        const bool to_top = b == 0 || (!MASS && (quick || (allow_few && at + value <= MOST)));   // all from `first` on are listed
+        first = after = 0;
 #pragma unroll 1
-          for (int sh5 = 27; sh5 > -5; sh5 -= 5) {   // 5 bits a round, the last of 2
-            const int sft = max(sh5, 0), ways = sh5 < 0 ? 4 : 32;
+        for (int sh5 = 27; sh5 > -5; sh5 -= 5) {   // 5 bits a round, the last of 2
+          const int sft = max(sh5, 0), ways = sh5 < 0 ? 4 : 32;
+          auto reach = [&](uint32_t base, uint32_t most) {
             const uint32_t probe = base + ((static_cast<uint32_t>(lane) + 1) << sft) - 1;   // the last key of the lane's part
-            const bool reach = lane < ways && (probe >= top_key || (probe >= KEY_LOWEST && r.bin(logit_of(probe)) <= most));
-            base += static_cast<uint32_t>(__ffs(__ballot_sync(FULL_MASK, reach)) - 1) << sft;
-          }
-          return base;
-        };
-        first = b < NB - 1 ? least(b) : KEY_LOWEST;
-        after = b && (MASS || !(quick || (allow_few && at + value <= MOST))) ? least(b - 1) : top_key + 1;   // where all from `first` on are listed, their end
+            return lane < ways && (probe >= top_key || (probe >= KEY_LOWEST && r.bin(logit_of(probe)) <= most));
+          };
+          const unsigned h0 = __ballot_sync(FULL_MASK, reach(first, b)), h1 = __ballot_sync(FULL_MASK, to_top || reach(after, b - 1));
+          first += static_cast<uint32_t>(__ffs(h0) - 1) << sft;
+          after += static_cast<uint32_t>(__ffs(h1) - 1) << sft;
+        }
+        if (b >= NB - 1) first = KEY_LOWEST;
+        if (to_top) after = top_key + 1;
       } else {
         after = hi - (b << shift) + 1;
         first = after - (1u << shift) < lo || after < (1u << shift) ? lo : after - (1u << shift);
@@ -406,19 +415,31 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
     if (level == 0) f.total = sh->found[4];
     // list the bin's tokens and, where counts say that it fits, those before it
     const bool with_above = quick || (!MASS && allow_few && level == 0 && before + sh->found[2] <= MOST);
+    const float x0 = logit_of(max(k0, KEY_LOWEST)), x1 = logit_of(k1 == 0x7fffffffu ? k1 - 1 : k1);   // (no -0)
+    const bool every = among.all();
     auto list = [&](bool bin, bool above) {
       uint32_t seen = 0;
-#pragma unroll 4
-      for (uint32_t i = tid; i < r.n; i += ST) {
-        const uint32_t k = key_of(r.x[i]);
-        if (k < k0 || !among.keeps(k, r.base + i)) continue;
-        if (k <= k1 ? bin : above) {
+      auto look = [&](float x, uint32_t i) {   // (floats stand in the order of their keys)
+        if (x < x0) return;
+        const uint32_t k = key_of(x);
+        if (!every && !among.keeps(k, r.base + i)) return;
+        if (x <= x1 ? bin : above) {
           const uint32_t q = atomicAdd(&sh->n_list, 1u);
           if (q < MOST) sh->list[q] = token_word(k, r.base + i);
         } else {
           ++seen;
         }
+      };
+      uint32_t i = tid;
+      for (; i + 3 * ST < r.n; i += 4 * ST) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = r.x[i + e * ST];
+        if (fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) < x0) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) look(x[e], i + e * ST);
       }
+      for (; i < r.n; i += ST) look(r.x[i], i);
       if (MASS && !above) {   // how many come before the bin
         seen = __reduce_add_sync(FULL_MASK, seen);
         if (lane == 0 && seen) atomicAdd(&sh->n_above, seen);
@@ -548,14 +569,14 @@ __global__ void __launch_bounds__(ST, 1024 / ST) sample_kernel(const clb200_samp
   extern __shared__ __align__(16) uint8_t sm[];
   Shared *sh = reinterpret_cast<Shared *>(sm);
   float *room = reinterpret_cast<float *>(sh + 1);   // slice + 3
-  const int row = blockIdx.x / CL, tid = threadIdx.x, lane = tid & 31;
+  const int row = blockIdx.x / CL, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Row r;
   r.sh = sh;
   r.rank = cluster_rank<CL>();
   r.base = r.rank * slice;
   r.n = r.base < static_cast<uint32_t>(s.vocab) ? min(slice, static_cast<uint32_t>(s.vocab) - r.base) : 0;
   r.per_thread = ((slice + ST - 1) / ST) | 1;   // odd: a warp's threads read different banks
-  if (tid < 128) sh->exp2_128[tid] = EXP2_128[tid];
+  if (tid < 128) sh->exp2_128[tid] = __hiloint2double(__double2hiint(EXP2_128[tid]) - (tid << 13), __double2loint(EXP2_128[tid]));
   float best = -INFINITY;
   const int64_t at = row * s.stride + r.base;
   if (s.type == T_F32) r.x = load_logits<ST>(static_cast<const float *>(s.logits) + at, room, r.n, best);
@@ -604,6 +625,9 @@ __global__ void __launch_bounds__(ST, 1024 / ST) sample_kernel(const clb200_samp
   const float heat = fmaxf(t, 1.17549435e-38f);   // the smallest normal number, whose inverse is finite
   r.inv_f = 1.0f / heat;
   r.scale = 1.4426950408889634 / static_cast<double>(heat);
+  // 64 temperatures below the largest, where a weight is below 2^-92; where rounding comes in (steps of h >= 128 temperatures / 3)
+  // still at least 42 temperatures, below 2^-60.
+  r.floor = fminf(fmaf(-64.f, heat, r.top), nextafterf(r.top, -INFINITY));
   const int k = s.top_k ? s.top_k[row] : 0;
   const float share = s.top_p ? s.top_p[row] : 1.f, least = s.min_p ? s.min_p[row] : 0.f;
   const double min_w = least > 0.f ? fmin(static_cast<double>(least), 1.0) : 0.0;
@@ -655,40 +679,57 @@ __global__ void __launch_bounds__(ST, 1024 / ST) sample_kernel(const clb200_samp
     lim = f.lim;
     if (by_k && by_p) lim = search<CL, ST, true>(r, lim, 0, static_cast<double>(share), false).lim;
   }
-  const bool every = lim.all();
-  auto kept = [&](float x, uint32_t i) -> u64 {
-    if (!every && !lim.keeps(key_of(x), r.base + i)) return 0;
-    const double w = r.weight(x);
-    return w >= min_w ? units(w) : 0ull;
-  };
-  // the kept masses by id: a thread's tokens, the threads before it, the CTAs before its own
-  u64 mine = 0, cta_total, total;
-  const uint32_t i0 = min(tid * r.per_thread, r.n), i1 = min(i0 + r.per_thread, r.n);
-  for (uint32_t i = i0; i < i1; i += E) {
-    float x[E];
-    double w[E];
+  // The kept masses by id: a warp takes a run of the slice, 32 E tokens at a time. The sums of the warps and CTAs before it say
+  // which warp goes through its run once more.
+  constexpr uint32_t STEP = 32 * E;
+  const float lowest = logit_of(lim.key);
+  const uint32_t run = (slice + SW * STEP - 1) / (SW * STEP) * STEP, i0 = min(warp * run, r.n), i1 = min(i0 + run, r.n);
+  float x[E];
+  double w[E];
+  auto weigh = [&](uint32_t i) {   // the sum of the lane's
     bool any = false;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      x[e] = i + e < i1 ? r.x[i + e] : -INFINITY;
-      if (!every && !lim.keeps(key_of(x[e]), r.base + i + e)) x[e] = -INFINITY;
+      const uint32_t q = i + 32 * e + lane;
+      x[e] = q < i1 ? r.x[q] : -INFINITY;
+      if (x[e] < lowest || (x[e] == lowest && r.base + q > lim.id)) x[e] = -INFINITY;
       any = any || x[e] != -INFINITY;
     }
-    if (!any) continue;
+    u64 sum = 0;
+    if (!__any_sync(FULL_MASK, any)) return sum;
     r.weights(x, w);
 #pragma unroll
-    for (int e = 0; e < E; ++e) mine += w[e] >= min_w ? units(w[e]) : 0ull;
-  }
+    for (int e = 0; e < E; ++e) {
+      w[e] = w[e] >= min_w ? w[e] : 0.0;
+      sum += units(w[e]);
+    }
+    return sum;
+  };
+  u64 mine = 0, cta_total, total;
+  for (uint32_t i = i0; i < i1; i += STEP) mine += weigh(i);
   u64 before = block_scan<ST>(sh, mine, cta_total);
-  before += cluster_scan<CL>(r, cta_total, total);
+  const u64 after = cluster_scan<CL>(r, cta_total, total) + __shfl_sync(FULL_MASK, before + mine, 31);
+  before += after - __shfl_sync(FULL_MASK, before + mine, 31);
+  before = __shfl_sync(FULL_MASK, before, 0);
   const u64 want = border(u, total);
-  if (before <= want && want < before + mine) {
-    for (uint32_t i = i0; i < i1; ++i) {
-      before += kept(r.x[i], i);
-      if (before > want) {
-        answer(r.base + i, r.weight(r.x[i]), total);
-        break;
+  if (before <= want && want < after) {
+    for (uint32_t i = i0; i < i1; i += STEP) {
+      u64 sum = weigh(i);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL_MASK, sum, o);
+      if (before + sum <= want) {
+        before += sum;
+        continue;
       }
+      bool done = false;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {   // (a step that is reached has weights)
+        const u64 m = units(w[e]), v = before + warp_scan(m);
+        if (!done && v - m <= want && want < v) answer(r.base + i + 32 * e + lane, w[e], total);
+        before = __shfl_sync(FULL_MASK, v, 31);
+        done = done || want < before;
+      }
+      break;
     }
   }
   cluster_sync<CL>();
