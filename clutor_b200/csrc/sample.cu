@@ -122,12 +122,14 @@ constexpr uint32_t MAX_SLICE = (SAMPLE_SMEM - sizeof(Shared)) / 4 - 3;
 // w (at most 1) in units of 2^-44, rounded to the nearest: the sum with 2^52 has it in its low bits.
 CLB_DEV u64 units(double w) { return static_cast<u64>(__double_as_longlong(fma(w, UNIT, 4503599627370496.0))) & 0xfffffffffffffull; }
 
+CLB_DEV float cleaned(float v) { return fmaxf(v, -INFINITY) + 0.f; }   // NaN as -infinity, -0 as 0
+
 struct Row {
   Shared *sh;
   float *x;              // [n] logits of tokens [base, base + n): NaN as -infinity, no -0
   uint32_t n, base, rank, per_thread;
   float top, half_top, inv_f;   // the largest logit (finite), half of it; 1 / temperature
-  float floor;           // logits up to this weigh nothing
+  float heat, floor;     // the temperature; logits up to this weigh nothing
   double top_d, scale;   // log2(e) / temperature
 
   // (top - x) / (2 temperature): halved so that it does not overflow; NaN for infinity x 0.
@@ -379,9 +381,12 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
       // the bin's keys: bins do not grow with the key, so its ends are found by halving, 32 ways at a time
       uint32_t first, after;
       const uint32_t top_key = key_of(r.top);
-      if (level == 0) {
+      if (quick) {   // any prefix of the order that reaches past bin b will do: down to a logit just below the bin's
+        first = key_of(cleaned(__fsub_rd(r.top, static_cast<float>(b + 1) * (1.0001f / BINS_PER_NAT) * r.heat)));
+        after = top_key + 1;
+      } else if (level == 0) {
         // the smallest key whose bin is at most b, and the smallest of the bins before it
-        const bool to_top = b == 0 || (!MASS && (quick || (allow_few && at + value <= MOST)));   // all from `first` on are listed
+        const bool to_top = b == 0 || (!MASS && allow_few && at + value <= MOST);   // all from `first` on are listed
         first = after = 0;
 #pragma unroll 1
         for (int sh5 = 27; sh5 > -5; sh5 -= 5) {   // 5 bits a round, the last of 2
@@ -539,8 +544,8 @@ CLB_DEV Found search(Row &r, const Limit &among, u64 want, double share, bool al
 template <int ST, typename T>
 CLB_DEV float *load_logits(const T *src, float *dst, uint32_t n, float &best) {
   constexpr uint32_t V = 16 / sizeof(T);
-  auto clean = [&](float v) {   // NaN as -infinity, -0 as 0
-    v = fmaxf(v, -INFINITY) + 0.f;
+  auto clean = [&](float v) {
+    v = cleaned(v);
     best = fmaxf(best, v);
     return v;
   };
@@ -576,13 +581,15 @@ __global__ void __launch_bounds__(ST, 1024 / ST) sample_kernel(const clb200_samp
   r.base = r.rank * slice;
   r.n = r.base < static_cast<uint32_t>(s.vocab) ? min(slice, static_cast<uint32_t>(s.vocab) - r.base) : 0;
   r.per_thread = ((slice + ST - 1) / ST) | 1;   // odd: a warp's threads read different banks
+  const float t = s.temperature ? s.temperature[row] : 1.f, share = s.top_p ? s.top_p[row] : 1.f, least = s.min_p ? s.min_p[row] : 0.f, draw = s.u[row];
+  const int k = s.top_k ? s.top_k[row] : 0;
   if (tid < 128) sh->exp2_128[tid] = __hiloint2double(__double2hiint(EXP2_128[tid]) - (tid << 13), __double2loint(EXP2_128[tid]));
   float best = -INFINITY;
   const int64_t at = row * s.stride + r.base;
   if (s.type == T_F32) r.x = load_logits<ST>(static_cast<const float *>(s.logits) + at, room, r.n, best);
   else if (s.type == T_F16) r.x = load_logits<ST>(static_cast<const __half *>(s.logits) + at, room, r.n, best);
   else r.x = load_logits<ST>(static_cast<const __nv_bfloat16 *>(s.logits) + at, room, r.n, best);
-  auto largest = [&](u64 v) {   // of the row's threads
+  auto largest = [&](u64 v, bool again) {   // of the row's threads
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(FULL_MASK, v, o));
     __syncthreads();
@@ -592,7 +599,7 @@ __global__ void __launch_bounds__(ST, 1024 / ST) sample_kernel(const clb200_samp
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(FULL_MASK, v, o));
     if constexpr (CL > 1) {
-      cluster_sync<CL>();   // what was exchanged before has been read
+      if (again) cluster_sync<CL>();   // what was exchanged before has been read
       if (tid == 0) sh->mine[3] = v;
       cluster_sync<CL>();
 #pragma unroll
@@ -600,13 +607,12 @@ __global__ void __launch_bounds__(ST, 1024 / ST) sample_kernel(const clb200_samp
     }
     return v;
   };
-  r.top = logit_of(static_cast<uint32_t>(largest(key_of(best))));
-  const float t = s.temperature ? s.temperature[row] : 1.f;
+  r.top = logit_of(static_cast<uint32_t>(largest(key_of(best), false)));
   if (r.top == -INFINITY || !(t > 0.f)) {
     u64 first = 0;   // the lowest id among the largest
     for (uint32_t i = tid; i < r.n; i += ST)
       if (r.x[i] == r.top) { first = 0xffffffffu - (r.base + i); break; }
-    first = largest(first);
+    first = largest(first, true);
     if (r.rank == 0 && tid == 0) {
       s.token[row] = r.top == -INFINITY ? -1 : static_cast<int>(0xffffffffu - static_cast<uint32_t>(first));
       if (s.prob) s.prob[row] = r.top == -INFINITY ? 0.f : 1.f;
@@ -622,16 +628,14 @@ __global__ void __launch_bounds__(ST, 1024 / ST) sample_kernel(const clb200_samp
   }
   r.half_top = 0.5f * r.top;
   r.top_d = static_cast<double>(r.top);
-  const float heat = fmaxf(t, 1.17549435e-38f);   // the smallest normal number, whose inverse is finite
+  const float heat = r.heat = fmaxf(t, 1.17549435e-38f);   // the smallest normal number, whose inverse is finite
   r.inv_f = 1.0f / heat;
   r.scale = 1.4426950408889634 / static_cast<double>(heat);
   // 64 temperatures below the largest, where a weight is below 2^-92; where rounding comes in (steps of h >= 128 temperatures / 3)
   // still at least 42 temperatures, below 2^-60.
   r.floor = fminf(fmaf(-64.f, heat, r.top), nextafterf(r.top, -INFINITY));
-  const int k = s.top_k ? s.top_k[row] : 0;
-  const float share = s.top_p ? s.top_p[row] : 1.f, least = s.min_p ? s.min_p[row] : 0.f;
   const double min_w = least > 0.f ? fmin(static_cast<double>(least), 1.0) : 0.0;
-  const double u = fmin(fmax(static_cast<double>(s.u[row]), 0.0), 1.0);   // a NaN counts as 0
+  const double u = fmin(fmax(static_cast<double>(draw), 0.0), 1.0);   // a NaN counts as 0
   const bool by_k = k > 0 && k < s.vocab, by_p = share < 1.f;
   auto border = [](double part, u64 total) { return min(static_cast<u64>(part * static_cast<double>(total)), total - 1); };
   auto answer = [&](uint32_t id, double w, u64 total) {

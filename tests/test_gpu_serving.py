@@ -274,6 +274,25 @@ def test_sample_ties_and_infinities(ctx):
         sample_check(ctx, lg, u, **kw)
 
 
+@pytest.mark.parametrize("v", [900, 20011, 100000])
+def test_sample_logits_around_zero(ctx, v):
+    """Both zeros and the smallest numbers of either sign, many times each, so that borders fall on zero and between the keys of its
+    neighbours; and sets in one bin of the first histogram, which finer ones have to divide."""
+    import torch
+    rng = np.random.default_rng(v)
+    R = 12
+    tiny = np.array([0.0, -0.0, 1e-45, -1e-45, 3e-42, -3e-42, 1.2e-38, -1.2e-38, 1e-30, -1e-30], np.float32)
+    lg = rng.choice(tiny, (R, v)).astype(np.float32)
+    lg[4:8] += rng.normal(0, 1e-3, (4, v)).astype(np.float32) * (rng.random((4, v)) < 0.5)
+    lg[8:] = -np.abs(lg[8:])
+    lg[10:, ::7] = 2.0
+    u = [float(x) for x in rng.random(R).astype(np.float32)]
+    k = [int(x) for x in rng.integers(1, v, R)]
+    for kw in ({"k": k}, {"p": [0.3] * R}, {"k": k, "p": [0.6] * R}, {"p": [0.5] * R, "t": [1e-3] * R}, {"k": k, "t": [1e-30] * R},
+               {"k": [min(40, v // 2)] * R, "t": [1e-4] * R}):
+        sample_check(ctx, torch.from_numpy(lg).cuda(), u, **kw)
+
+
 def test_sample_distribution_of_many_rows(ctx):
     """700 rows of the same logits with u on a grid: the tokens come in the order of the cumulative distribution."""
     import torch
