@@ -22,7 +22,6 @@ constexpr int NB = 2048;                     // bins of a histogram
 constexpr int CAP = 512;                     // tokens that are sorted directly, at most (a thread each)
 constexpr int E = 4;                         // tokens a thread weighs at once
 constexpr int SAMPLE_MAX_VOCAB = 1 << 18;
-constexpr int SMALL_VOCAB = 6144;            // up to this a row is a small CTA's
 constexpr double UNIT = 17592186044416.0;    // 2^44
 constexpr float BINS_PER_NAT = 64.f;         // the first histogram's bins cover 32 e-foldings: lighter weights are below 2^-44
 
@@ -569,7 +568,7 @@ CLB_DEV float *load_logits(const T *src, float *dst, uint32_t n, float &best) {
 
 // One row by CL CTAs: its logits lie in their shared memory, a slice each, and are read from memory once.
 template <int CL, int ST>
-__global__ void __launch_bounds__(ST, 1024 / ST) sample_kernel(const clb200_sampling s, const uint32_t slice) {
+__global__ void __launch_bounds__(ST, CL == 1 ? 1024 / ST : 1) sample_kernel(const clb200_sampling s, const uint32_t slice) {
   constexpr int SW = ST / 32, MOST = ST < CAP ? ST : CAP;
   extern __shared__ __align__(16) uint8_t sm[];
   Shared *sh = reinterpret_cast<Shared *>(sm);
@@ -762,6 +761,16 @@ cudaError_t launch_sample(const clb200_sampling &s, int device, cudaStream_t st)
   return cudaLaunchKernelEx(&cfg, sample_kernel<CL, ST>, s, slice);
 }
 
+template <int ST>
+cudaError_t launch_cl(int cl, const clb200_sampling &s, int device, cudaStream_t st) {
+  switch (cl) {
+    case 1: return launch_sample<1, ST>(s, device, st);
+    case 2: return launch_sample<2, ST>(s, device, st);
+    case 4: return launch_sample<4, ST>(s, device, st);
+    default: return launch_sample<8, ST>(s, device, st);
+  }
+}
+
 int check(const clb200_sampling *s, char *err, size_t errlen) {
   if (!s) { errf(err, errlen, "no arguments"); return 1; }
   if (s->rows < 0 || s->rows > (1 << 24) || s->vocab < 1 || s->vocab > SAMPLE_MAX_VOCAB) {
@@ -785,18 +794,20 @@ extern "C" int clb200_sample(clb200_ctx *c, const clb200_sampling *s, void *stre
   if (!c) { errf(err, errlen, "no context"); return 1; }
   if (s->rows == 0) return 0;
   const OnDevice on(c->device);
-  // A small vocabulary by a CTA of 256 threads, four to an SM (278 rows of 669: 14.5 us; 28.8 with 1024). Else the fewest CTAs of
-  // 1024 that hold a row, since the exchange costs more than it saves once the SMs are busy (256 rows of 50304: 89 us with one a
-  // row, 123 with two, 190 with four), and more of them for long rows while that leaves no row waiting (a GPC takes two clusters
-  // of eight: 17 rows of 151936 take 23 us with four each and 33 with eight; one takes 18.4 with eight; filters want few CTAs,
-  // sums over everything many: 8 rows of 14678 with top-k 17.4 us with one, 20.0 with four; 15 rows of 39554 without filters 15.6
-  // with one, 11.2 with four).
+  // The fewest CTAs that hold a row, since the exchange costs more than it saves once the SMs are busy (256 rows of 50304: 89 us
+  // with one a row, 123 with two, 190 with four), and more of them for long rows while that leaves no row waiting (a GPC takes two
+  // clusters of eight: 17 rows of 151936 take 23 us with four each and 33 with eight; filters want few CTAs, sums over everything
+  // many: 8 rows of 14678 with top-k 17.4 us with one, 20.0 with four; 15 rows of 39554 without filters 15.6 with one, 11.2 with
+  // four). Threads: barriers and scans cost less with fewer, passes over the logits less with more (one row of 151936 by eight CTAs:
+  // 15.0 us with 512 threads, 19.4 with 1024, 16 with 256; 100 rows of 32000: 39 and 34 with 1024), and small CTAs share an SM (1000
+  // rows of 10000: 47 us with 256, 57 with 512, 91 with 1024; 140 rows of 6000, which need not: 18.2, 16.3, 17.9).
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : c->stream;
   int cl = 1;
   while (cl < 8 && ((s->vocab + cl - 1) / cl > static_cast<int>(MAX_SLICE) || (static_cast<int64_t>(s->rows) * cl * 2 <= 128 && s->vocab >= 12288 * cl))) cl *= 2;
-  const cudaError_t e = s->vocab <= SMALL_VOCAB ? launch_sample<1, 256>(*s, c->device, st) : cl == 1 ? launch_sample<1, 1024>(*s, c->device, st)
-                        : cl == 2 ? launch_sample<2, 1024>(*s, c->device, st) : cl == 4 ? launch_sample<4, 1024>(*s, c->device, st)
-                                                                                        : launch_sample<8, 1024>(*s, c->device, st);
+  cudaError_t e;
+  if (s->vocab <= 2560 || (s->vocab <= 10240 && s->rows > c->sms)) e = launch_sample<1, 256>(*s, c->device, st);
+  else if (s->vocab <= 20480 * cl) e = launch_cl<512>(cl, *s, c->device, st);
+  else e = launch_cl<1024>(cl, *s, c->device, st);
   CUDA_OR(e, "launching the sampling");
   return 0;
 }

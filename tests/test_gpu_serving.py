@@ -441,9 +441,10 @@ def test_streams_and_two_graphs_at_once(ctx):
     ctx.status()
 
 
-@pytest.mark.parametrize("rows,vocab", [(80, 50304), (160, 1000), (80, 60001), (40, 100003), (3, 151936), (1, 8191)])
+@pytest.mark.parametrize("rows,vocab", [(80, 50304), (160, 1000), (80, 60001), (40, 100003), (3, 151936), (1, 8191),
+                                        (300, 10000), (150, 20011), (30, 30000), (60, 40000)])
 def test_sample_row_splits(ctx, rows, vocab):
-    """Every number of CTAs a row (1, 2, 4, 8)."""
+    """Every number of CTAs a row (1, 2, 4, 8), and of threads."""
     import torch
     rng = np.random.default_rng(rows + vocab)
     g = torch.Generator(device="cuda").manual_seed(vocab)
