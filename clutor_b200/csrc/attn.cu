@@ -23,8 +23,8 @@ namespace {
 // states are joined at its end, under the first loads of the next item (200 sequences of up to 300 positions, 32 heads over 8:
 // 40 us, 45 with those loads behind the join; the states handed from warp to warp through one buffer instead: 50). Products on
 // m16n8k16: at 8 of 16 rows in use they are far from the limit, while eight warps an SM with two stages each on their way cover
-// HBM's latency. 64 sequences of up to 8000 positions, 32 heads over 4 of 128: 105 us = 6.05 TB/s, 92 % of the measured copy
-// rate; one token over 500 positions 9.5 us with the join.
+// HBM's latency. 64 sequences of up to 8000 positions, 32 heads over 4 of 128: 104 us = 6.06 TB/s, 92 % of the measured copy
+// rate; one token over 500 positions 8.9 us with the join.
 constexpr int RT = 128, RW = RT / 32, RN = 16 * RW;   // threads, warps, positions per tile (16 per warp)
 
 template <int HD, int MT>
@@ -289,7 +289,9 @@ constexpr int JT = 256;
 
 // HD / 4 threads hold a row, four elements each. BY_ROW: a CTA takes as many rows as it has such groups, each going through the
 // pieces in run order (many rows in few pieces: the prompt kernel's). Else a CTA takes one row, its groups every so-many-th piece,
-// and their states are joined in group order (few rows in many pieces: a long cache's).
+// and their states are joined in group order (few rows in many pieces: a long cache's; with 128 threads 1.4 us slower there and as
+// much faster at 64 sequences). Most CTAs find nothing and end; as many as max_q allows are launched (one token over 500 positions
+// 8.9 us, 9.4 with CTAs for every row that an item could have).
 template <typename O, int HD, bool BY_ROW>
 __global__ void __launch_bounds__(JT) attn_join_kernel(const AttnArgs g) {
   constexpr int TPR = HD / 4, GROUPS = JT / TPR;
@@ -367,8 +369,8 @@ template <typename O, int HD>
 cudaError_t launch_join(const AttnArgs &g, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
   const bool by_row = g.rows > 32;
-  const int groups = JT / (HD / 4);
-  cfg.gridDim = dim3(g.nc, by_row ? (g.tpi * g.group + groups - 1) / groups : g.tpi * g.group);
+  const int groups = JT / (HD / 4), rows = std::max(std::min(g.tpi, g.a.max_q), 1) * g.group;   // the most that an item can have
+  cfg.gridDim = dim3(g.nc, by_row ? (rows + groups - 1) / groups : rows);
   cfg.blockDim = dim3(JT);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
