@@ -430,8 +430,9 @@ class Context:
             raise ClutorError("rope must be a contiguous float32 [n_pos, head_dim] tensor")
         qn = kn = 0
         if norm:
-            self._on_device(q_norm, k_norm)
             one = norm == QK_NORM_HEAD
+            if q_norm is None or k_norm is None or not (q_norm.get_device() == device == k_norm.get_device()):
+                self._on_device(q_norm, k_norm)
             if q_norm is None or k_norm is None or q_norm.dtype is not f32 or k_norm.dtype is not f32 or \
                     q_norm.numel() != (D if one else H * D) or k_norm.numel() != (D if one else KV * D) or \
                     not q_norm.is_contiguous() or not k_norm.is_contiguous():
@@ -440,15 +441,15 @@ class Context:
             qn, kn = q_norm.data_ptr(), k_norm.data_ptr()
         st = self._raw_stream(stream)
         if out is None:
-            out = _empty((T, H, D), pages.dtype, q.device, stream)
+            out = _new((T, H, D), dtype=pages.dtype, device=q.device) if stream is None else _empty((T, H, D), pages.dtype, q.device, stream)
             out_row = H * D
         elif out.shape != (T, H, D) or out.dtype is not pages.dtype or out.get_device() != device:
             raise ClutorError(f"out must be {[T, H, D]} of {pages.dtype} on cuda:{device}")
         else:
-            out_row = _rows(out)
+            out_row = _rows(out, T, H, D)
         pages.pack(self._kv, q_start, kv_len)
-        _QK.pack_into(self._args, 0, T, H, _dtype(dt), q.data_ptr(), k.data_ptr(), v.data_ptr(), _rows(q), _rows(k), _rows(v), norm,
-                      qn, kn, eps, rope.data_ptr(), rope.shape[0], 1 if pairs else 0, out.data_ptr(), out_row)
+        _QK.pack_into(self._args, 0, T, H, _dtype(dt), q.data_ptr(), k.data_ptr(), v.data_ptr(), _rows(q, T, H, D), _rows(k, T, KV, D),
+                      _rows(v, T, KV, D), norm, qn, kn, eps, rope.data_ptr(), rope.shape[0], 1 if pairs else 0, out.data_ptr(), out_row)
         if self._c_qk(self.handle, self._kv_at, self._args_at, st, self._err, 512):
             raise ClutorError(self._err.value.decode())
         return out
@@ -473,7 +474,7 @@ class Context:
         elif out.shape != (T, H, D) or (out_dtype is not None and out.dtype is not out_dtype) or out.get_device() != device:
             raise ClutorError(f"out must be {[T, H, D]} of {out_dtype or out.dtype} on cuda:{device}")
         else:
-            odt, out_row = out.dtype, _rows(out)
+            odt, out_row = out.dtype, _rows(out, T, H, D)
         pages.pack(self._kv, q_start, kv_len)
         if max_q is None:
             max_q = T
@@ -482,11 +483,14 @@ class Context:
         # the workspace depends on the heads, their size and whether few or many rows share a key/value head
         key = H, pages.n_kv, D, max_q
         size = self._work_bytes.get(key)
-        qp, qr, op, ot = q.data_ptr(), _rows(q), out.data_ptr(), _dtype(odt)
+        qp, qr, op, ot = q.data_ptr(), _rows(q, T, H, D), out.data_ptr(), _dtype(odt)
         if size is None:
             _ATTN.pack_into(self._args, 0, T, H, max_q, qp, qr, op, ot, out_row, scale, window, sinks, 0, 0)
             size = self._work_bytes[key] = lib().clb200_attention_work(self.handle, self._kv_at, self._args_at)
-        work = _empty(size, _uint8, q.device, stream) if size else None   # 0: the call says what is wrong
+        if stream is None and size:
+            work = _new(size, dtype=_uint8, device=q.device)
+        else:
+            work = _empty(size, _uint8, q.device, stream) if size else None   # 0: the call says what is wrong
         _ATTN.pack_into(self._args, 0, T, H, max_q, qp, qr, op, ot, out_row, scale, window, sinks, work.data_ptr() if size else 0, size)
         if self._c_attention(self.handle, self._kv_at, self._args_at, st, self._err, 512):
             self._work_bytes.pop(key, None)
@@ -574,10 +578,9 @@ def _dtype(d) -> int:
     return t
 
 
-def _rows(t) -> int:
-    """The stride of a [T, heads, head_dim] tensor's rows; the heads of a row must follow one another."""
+def _rows(t, T: int, H: int, D: int) -> int:
+    """The stride of the rows of t, a [T, H, D] tensor; the heads of a row must follow one another."""
     a, b, c = t.stride()
-    T, H, D = t.shape
     if c != 1 or (b != D and H > 1):
         raise ClutorError(f"the heads of a row must follow one another (strides {t.stride()} of {tuple(t.shape)})")
     return a if T > 1 else max(a, H * D)
