@@ -588,7 +588,8 @@ def _rows(t, T: int, H: int, D: int) -> int:
 
 class KvPages:
     """A paged key/value cache on the device (clb200_kv): k and v [n_pages, page_size, n_kv, head_dim] float16 or bfloat16 (the
-    same strides, head_dim contiguous), table [n_seq, width] int32: the pages of each sequence in order."""
+    same strides, head_dim contiguous), table [n_seq, width] int32: the pages of each sequence in order, a row in memory for each
+    (sequences that share pages name them in their own rows)."""
 
     __slots__ = ("k", "v", "table", "n_pages", "page_size", "n_kv", "head_dim", "dtype", "device", "_fixed")
 
@@ -604,6 +605,8 @@ class KvPages:
         row, along = table.stride() if table.dim() == 2 else (0, 0)
         if table.dim() != 2 or table.dtype is not _int32 or (width > 1 and along != 1):
             raise ClutorError("table must be an int32 [n_seq, width] tensor")
+        if n_seq > 1 and row < width:   # the kernels step from row to row by at least a row's ids
+            raise ClutorError(f"the rows of table share memory ({row} ids apart, {width} each): it must hold a row for each sequence")
         self.device = device = k.get_device()
         if device < 0 or v.get_device() != device or table.get_device() != device:
             raise ClutorError("k, v and table must lie on one CUDA device")

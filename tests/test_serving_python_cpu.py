@@ -1,0 +1,106 @@
+"""The Python side of the serving calls without a GPU: what it packs for the C entry points and what it refuses. The tensors are
+stand-ins that have a layout and an address on a device, and no memory; nothing reads the addresses."""
+import ctypes as C
+
+import pytest
+import torch
+
+import clutor_b200 as cb
+
+P = 1 << 20   # a 16-byte aligned address
+
+
+class Laid:
+    """A tensor's layout: that of `like`, a CPU or meta tensor, said to lie on cuda:`at`."""
+
+    def __init__(self, like, at=0):
+        self.like, self.at, self.dtype, self.shape, self.device = like, at, like.dtype, like.shape, torch.device("cuda", max(at, 0))
+
+    def __getattr__(self, name):   # stride, dim, numel, is_contiguous
+        return getattr(self.like, name)
+
+    def get_device(self):
+        return self.at
+
+    def data_ptr(self):
+        return P
+
+
+def ids(*shape):
+    return torch.zeros(shape, dtype=torch.int32, device="meta")
+
+
+def pages(table, n_pages=9, page=16, KV=2, D=64, dt=torch.float16):
+    kv = Laid(torch.empty(n_pages, page, KV, D, dtype=dt, device="meta"))
+    return cb.KvPages(kv, kv, Laid(table))
+
+
+class Library:
+    """Stands in for the library under a Context on device `at`: keeps the structs that the serving calls pass."""
+
+    def __init__(self, at=0):
+        self.at, self.calls, self.opened = at, [], []
+
+    def context(self, device=0):
+        self.opened.append(cb.Context(device))
+        return self.opened[-1]
+
+    def clb200_open(self, device, err, n):
+        return 1
+
+    def clb200_close(self, handle):
+        pass
+
+    def clb200_attention_work(self, handle, kv, a):
+        return 0
+
+    def _take(self, what, *at):
+        self.calls.append([S.from_buffer_copy(C.string_at(p, C.sizeof(S))) for S, p in zip(what, at)])
+        return 0
+
+    def clb200_qk_rope(self, handle, kv, a, stream, err, n):
+        return self._take((cb.KvStruct, cb.QkStruct), kv, a)
+
+    def clb200_attention(self, handle, kv, a, stream, err, n):
+        return self._take((cb.KvStruct, cb.AttnStruct), kv, a)
+
+    def clb200_sample(self, handle, a, stream, err, n):
+        return self._take((cb.SamplingStruct,), a)
+
+
+class Stream:
+    cuda_stream = 7
+
+
+@pytest.fixture
+def library(monkeypatch):
+    """A stand-in for the library, under every Context that the test opens."""
+    made = Library()
+    monkeypatch.setattr(cb, "lib", lambda: made)
+    yield made
+    for c in made.opened:
+        c.handle = None   # nothing for the real library to close
+
+
+def passed(library, p):
+    """The clb200_kv that a call on the pages p passes."""
+    n = p.table.shape[0]
+    q = Laid(torch.empty(3, 4, p.head_dim, dtype=p.dtype, device="meta"))
+    library.context().attention(q, p, Laid(ids(n + 1)), Laid(ids(n)), out=q, stream=Stream)
+    return library.calls[-1][0]
+
+
+@pytest.mark.parametrize("table,stride", [(ids(8, 5), 5), (ids(8, 7)[:, :5], 7), (ids(1, 5), 5), (ids(1, 7)[:, :5], 7), (ids(1, 5).expand(1, 5), 5),
+                                          (ids(5).as_strided((1, 5), (2, 1)), 5), (ids(4, 1), 1), (ids(3, 0), 1), (ids(0, 4), 4)])
+def test_table_rows_apart(library, table, stride):
+    s = passed(library, pages(table))
+    assert (s.n_seq, s.table_width, s.table_stride) == (*table.shape, stride)
+
+
+@pytest.mark.parametrize("table", [ids(1, 5).expand(8, 5), ids(1, 1).expand(3, 1), ids(20).as_strided((4, 5), (3, 1)),
+                                   ids(20).as_strided((2, 5), (4, 1)), ids(5).as_strided((2, 5), (0, 1))])
+def test_table_rows_that_share_memory_are_refused(table):
+    """A row of the table is read table_width ids from table_stride ids behind the row before: rows nearer to one another would be
+    read where the table does not reach."""
+    with pytest.raises(cb.ClutorError, match="rows of table"):
+        pages(table)
