@@ -276,7 +276,7 @@ def layer_struct(layer) -> MoELayer:
 
 
 class Context:
-    """A clb200 context on one CUDA device (clb200_open)."""
+    """A clb200 context on one CUDA device (clb200_open). One host thread at a time uses it, as in C."""
 
     def __init__(self, device: int = 0):
         self._err = C.create_string_buffer(512)
@@ -285,9 +285,6 @@ class Context:
             raise ClutorError(self._err.value.decode())
         self.device = device
         self._keep: list = []
-        # the serving calls' argument structs, written anew for every call
-        self._kv, self._args = C.create_string_buffer(_KV.size), C.create_string_buffer(max(_QK.size, _ATTN.size, _SAMPLING.size))
-        self._kv_at, self._args_at = C.addressof(self._kv), C.addressof(self._args)
         self._c_qk, self._c_attention, self._c_sample = lib().clb200_qk_rope, lib().clb200_attention, lib().clb200_sample
         self._work_bytes: dict = {}
 
@@ -447,10 +444,9 @@ class Context:
             raise ClutorError(f"out must be {[T, H, D]} of {pages.dtype} on cuda:{device}")
         else:
             out_row = _rows(out, T, H, D)
-        pages.pack(self._kv, q_start, kv_len)
-        _QK.pack_into(self._args, 0, T, H, _dtype(dt), q.data_ptr(), k.data_ptr(), v.data_ptr(), _rows(q, T, H, D), _rows(k, T, KV, D),
-                      _rows(v, T, KV, D), norm, qn, kn, eps, rope.data_ptr(), rope.shape[0], 1 if pairs else 0, out.data_ptr(), out_row)
-        if self._c_qk(self.handle, self._kv_at, self._args_at, st, self._err, 512):
+        args = _QK.pack(T, H, _dtype(dt), q.data_ptr(), k.data_ptr(), v.data_ptr(), _rows(q, T, H, D), _rows(k, T, KV, D),
+                        _rows(v, T, KV, D), norm, qn, kn, eps, rope.data_ptr(), rope.shape[0], 1 if pairs else 0, out.data_ptr(), out_row)
+        if self._c_qk(self.handle, pages.pack(q_start, kv_len), args, st, self._err, 512):
             raise ClutorError(self._err.value.decode())
         return out
 
@@ -459,7 +455,7 @@ class Context:
         """clb200_attention on torch CUDA tensors: q [T, n_head, head_dim] of the cache's type, the new rows of sequences whose
         keys and values (the new ones included) are in `pages`; max_q bounds the new rows of a sequence (default: T); scale
         defaults to head_dim ** -0.5. Returns [T, n_head, head_dim] (`out`, or a new tensor of out_dtype, by default q's type);
-        asynchronous. The call's workspace is allocated for the stream, so calls may overlap."""
+        asynchronous. The call's workspace is allocated for the stream, so calls may overlap on the device."""
         T, H, D = q.shape
         dt = q.dtype
         if D != pages.head_dim or dt is not pages.dtype:
@@ -475,7 +471,7 @@ class Context:
             raise ClutorError(f"out must be {[T, H, D]} of {out_dtype or out.dtype} on cuda:{device}")
         else:
             odt, out_row = out.dtype, _rows(out, T, H, D)
-        pages.pack(self._kv, q_start, kv_len)
+        kv = pages.pack(q_start, kv_len)
         if max_q is None:
             max_q = T
         if scale is None:
@@ -485,14 +481,14 @@ class Context:
         size = self._work_bytes.get(key)
         qp, qr, op, ot = q.data_ptr(), _rows(q, T, H, D), out.data_ptr(), _dtype(odt)
         if size is None:
-            _ATTN.pack_into(self._args, 0, T, H, max_q, qp, qr, op, ot, out_row, scale, window, sinks, 0, 0)
-            size = self._work_bytes[key] = lib().clb200_attention_work(self.handle, self._kv_at, self._args_at)
+            args = _ATTN.pack(T, H, max_q, qp, qr, op, ot, out_row, scale, window, sinks, 0, 0)
+            size = self._work_bytes[key] = lib().clb200_attention_work(self.handle, kv, args)
         if stream is None and size:
             work = _new(size, dtype=_uint8, device=q.device)
         else:
             work = _empty(size, _uint8, q.device, stream) if size else None   # 0: the call says what is wrong
-        _ATTN.pack_into(self._args, 0, T, H, max_q, qp, qr, op, ot, out_row, scale, window, sinks, work.data_ptr() if size else 0, size)
-        if self._c_attention(self.handle, self._kv_at, self._args_at, st, self._err, 512):
+        args = _ATTN.pack(T, H, max_q, qp, qr, op, ot, out_row, scale, window, sinks, work.data_ptr() if size else 0, size)
+        if self._c_attention(self.handle, kv, args, st, self._err, 512):
             self._work_bytes.pop(key, None)
             raise ClutorError(self._err.value.decode())
         return out
@@ -518,11 +514,11 @@ class Context:
             token = _empty(R, i32, logits.device, stream)
         if prob is None:
             prob = _empty(R, f32, logits.device, stream)
-        _SAMPLING.pack_into(self._args, 0, R, V, _dtype(logits.dtype), logits.data_ptr(), step, u.data_ptr(),
-                            0 if temperature is None else temperature.data_ptr(), 0 if top_k is None else top_k.data_ptr(),
-                            0 if top_p is None else top_p.data_ptr(), 0 if min_p is None else min_p.data_ptr(), token.data_ptr(),
-                            prob.data_ptr())
-        if self._c_sample(self.handle, self._args_at, st, self._err, 512):
+        args = _SAMPLING.pack(R, V, _dtype(logits.dtype), logits.data_ptr(), step, u.data_ptr(),
+                              0 if temperature is None else temperature.data_ptr(), 0 if top_k is None else top_k.data_ptr(),
+                              0 if top_p is None else top_p.data_ptr(), 0 if min_p is None else min_p.data_ptr(), token.data_ptr(),
+                              prob.data_ptr())
+        if self._c_sample(self.handle, args, st, self._err, 512):
             raise ClutorError(self._err.value.decode())
         return token, prob
 
@@ -538,8 +534,9 @@ class Context:
         return (_current_stream(self.device) if stream is None else stream.cuda_stream) or CUDA_STREAM_LEGACY
 
 
-# the argument structs above as byte layouts: packing one into a buffer that a context keeps costs a third of making a
-# ctypes structure, and these calls are made once a layer of every token
+# the argument structs above as byte layouts: packing one costs a third of making a ctypes structure, and these calls are made
+# once a layer of every token. A call's bytes are its own: the library runs without Python's lock, so that another thread may
+# pack the next call's meanwhile.
 _KV = struct.Struct("@PPIiiiiqqqPiiiPP0q")
 _QK = struct.Struct("@iiIPPPqqqiPPfPiiPq0q")
 _ATTN = struct.Struct("@iiiPqPIqfiiPN0q")
@@ -614,13 +611,13 @@ class KvPages:
         self.n_pages, self.page_size, self.n_kv, self.head_dim = shape
         self._fixed = (k.data_ptr(), v.data_ptr(), kind, *shape, *strides[:3], table.data_ptr(), max(row, width), width, n_seq)
 
-    def pack(self, buf, q_start, kv_len) -> None:
-        """The clb200_kv of one call's sequences, into buf."""
+    def pack(self, q_start, kv_len) -> bytes:
+        """The clb200_kv of one call's sequences."""
         n_seq, i32, device = self._fixed[-1], _int32, self.device
         if q_start.dtype is not i32 or kv_len.dtype is not i32 or q_start.shape != (n_seq + 1,) or kv_len.shape != (n_seq,) or \
                 not q_start.is_contiguous() or not kv_len.is_contiguous() or q_start.get_device() != device or kv_len.get_device() != device:
             raise ClutorError(f"q_start and kv_len must be contiguous int32 tensors of {n_seq + 1} and {n_seq} elements on cuda:{device}")
-        _KV.pack_into(buf, 0, *self._fixed, q_start.data_ptr(), kv_len.data_ptr())
+        return _KV.pack(*self._fixed, q_start.data_ptr(), kv_len.data_ptr())
 
 
 def backend() -> Backend:

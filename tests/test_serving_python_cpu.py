@@ -104,3 +104,43 @@ def test_table_rows_that_share_memory_are_refused(table):
     read where the table does not reach."""
     with pytest.raises(cb.ClutorError, match="rows of table"):
         pages(table)
+
+
+def sample_tensors(R, V):
+    f = Laid(torch.empty(R, device="meta"))
+    return Laid(torch.empty(R, V, device="meta")), f, Laid(ids(R)), f
+
+
+def test_calls_of_two_threads_keep_their_own_arguments(library, monkeypatch):
+    """The library runs without Python's lock, so a second call may be prepared while it does: a call's arguments stay as they are
+    until it returns. The second call is made here from inside the first one's."""
+    ctx = library.context()
+    kv = pages(ids(2, 5))
+    q = Laid(torch.empty(3, 4, 64, dtype=torch.float16, device="meta"))
+    kw = dict(out=q, stream=Stream)
+    ends = Laid(ids(3)), Laid(ids(2))
+    rope = Laid(torch.empty(30, 64, device="meta"))
+    k = Laid(torch.empty(3, 2, 64, dtype=torch.float16, device="meta"))
+    calls = [lambda: ctx.attention(q, kv, *ends, scale=0.5, window=9, **kw), lambda: ctx.attention(q, pages(ids(2, 3)), *ends, max_q=2, **kw),
+             lambda: ctx.qk_rope(q, k, k, kv, *ends, rope, norm=0, pairs=True, **kw),
+             lambda: ctx.qk_rope(q, k, k, pages(ids(2, 8)), *ends, rope, norm=0, eps=0.5, **kw),
+             *(lambda R=R: ctx.sample(*sample_tensors(R, 100)[:2], token=sample_tensors(R, 100)[2], prob=sample_tensors(R, 100)[3], stream=Stream)
+               for R in (3, 5))]
+    alone = []
+    for call in calls:
+        call()
+        alone.append([bytes(s) for s in library.calls[-1]])
+    for i, outer in enumerate(calls):
+        for inner in calls:
+            take, depth = Library._take, [0]
+
+            def nested(self, what, *at):
+                depth[0] += 1
+                if depth[0] == 1:
+                    inner()
+                return take(self, what, *at)   # the outer call's arguments, read after the inner call
+
+            monkeypatch.setattr(Library, "_take", nested)
+            outer()
+            monkeypatch.setattr(Library, "_take", take)
+            assert [bytes(s) for s in library.calls[-1]] == alone[i]
