@@ -412,7 +412,10 @@ class Context:
         type; rows any stride apart) are normalised, turned by position and, k and v, stored into `pages`; q_start [n_seq + 1]
         and kv_len [n_seq] int32; rope [n_pos, head_dim] float32 (cosines, then sines). Returns the turned q, [T, n_head,
         head_dim] of the cache's type (`out`, or a new tensor); asynchronous."""
-        T, H, D = q.shape
+        try:
+            T, H, D = q.shape
+        except ValueError:
+            raise ClutorError(f"q {tuple(q.shape)}: [T, n_head, head_dim]") from None
         KV, dt, f32 = pages.n_kv, q.dtype, _float32
         rows = T, KV, D
         if k.shape != rows or v.shape != rows or D != pages.head_dim:
@@ -444,8 +447,11 @@ class Context:
             raise ClutorError(f"out must be {[T, H, D]} of {pages.dtype} on cuda:{device}")
         else:
             out_row = _rows(out, T, H, D)
-        args = _QK.pack(T, H, _dtype(dt), q.data_ptr(), k.data_ptr(), v.data_ptr(), _rows(q, T, H, D), _rows(k, T, KV, D),
-                        _rows(v, T, KV, D), norm, qn, kn, eps, rope.data_ptr(), rope.shape[0], 1 if pairs else 0, out.data_ptr(), out_row)
+        try:
+            args = _QK.pack(T, H, _dtype(dt), q.data_ptr(), k.data_ptr(), v.data_ptr(), _rows(q, T, H, D), _rows(k, T, KV, D),
+                            _rows(v, T, KV, D), norm, qn, kn, eps, rope.data_ptr(), rope.shape[0], 1 if pairs else 0, out.data_ptr(), out_row)
+        except struct.error as e:
+            raise ClutorError(f"an argument is out of range: {e}") from None
         if self._c_qk(self.handle, pages.pack(q_start, kv_len), args, st, self._err, 512):
             raise ClutorError(self._err.value.decode())
         return out
@@ -456,7 +462,10 @@ class Context:
         keys and values (the new ones included) are in `pages`; max_q bounds the new rows of a sequence (default: T); scale
         defaults to head_dim ** -0.5. Returns [T, n_head, head_dim] (`out`, or a new tensor of out_dtype, by default q's type);
         asynchronous. The call's workspace is allocated for the stream, so calls may overlap on the device."""
-        T, H, D = q.shape
+        try:
+            T, H, D = q.shape
+        except ValueError:
+            raise ClutorError(f"q {tuple(q.shape)}: [T, n_head, head_dim]") from None
         dt = q.dtype
         if D != pages.head_dim or dt is not pages.dtype:
             raise ClutorError(f"q {tuple(q.shape)} of {dt} does not fit a {pages.dtype} cache of head_dim {pages.head_dim}")
@@ -481,13 +490,19 @@ class Context:
         size = self._work_bytes.get(key)
         qp, qr, op, ot = q.data_ptr(), _rows(q, T, H, D), out.data_ptr(), _dtype(odt)
         if size is None:
-            args = _ATTN.pack(T, H, max_q, qp, qr, op, ot, out_row, scale, window, sinks, 0, 0)
+            try:
+                args = _ATTN.pack(T, H, max_q, qp, qr, op, ot, out_row, scale, window, sinks, 0, 0)
+            except struct.error as e:
+                raise ClutorError(f"an argument is out of range: {e}") from None
             size = self._work_bytes[key] = lib().clb200_attention_work(self.handle, kv, args)
         if stream is None and size:
             work = _new(size, dtype=_uint8, device=q.device)
         else:
             work = _empty(size, _uint8, q.device, stream) if size else None   # 0: the call says what is wrong
-        args = _ATTN.pack(T, H, max_q, qp, qr, op, ot, out_row, scale, window, sinks, work.data_ptr() if size else 0, size)
+        try:
+            args = _ATTN.pack(T, H, max_q, qp, qr, op, ot, out_row, scale, window, sinks, work.data_ptr() if size else 0, size)
+        except struct.error as e:
+            raise ClutorError(f"an argument is out of range: {e}") from None
         if self._c_attention(self.handle, kv, args, st, self._err, 512):
             self._work_bytes.pop(key, None)
             raise ClutorError(self._err.value.decode())
@@ -499,7 +514,10 @@ class Context:
         Returns (token [rows] int32, prob [rows] float32); asynchronous."""
         if _new is None:
             _use_torch()
-        R, V = logits.shape
+        try:
+            R, V = logits.shape
+        except ValueError:
+            raise ClutorError(f"logits {tuple(logits.shape)}: [rows, vocab]") from None
         step, along = logits.stride()
         if V > 1 and along != 1:
             raise ClutorError("a row's logits must lie next to one another")

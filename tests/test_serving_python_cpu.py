@@ -144,3 +144,26 @@ def test_calls_of_two_threads_keep_their_own_arguments(library, monkeypatch):
             outer()
             monkeypatch.setattr(Library, "_take", take)
             assert [bytes(s) for s in library.calls[-1]] == alone[i]
+
+
+def test_refusals_are_the_frameworks_own(library):
+    """Tensors of another rank and numbers that no C argument holds raise what every other refusal raises."""
+    ctx, kv = library.context(), pages(ids(2, 5))
+    q, k, rope = (Laid(torch.empty(*s, dtype=d, device="meta")) for s, d in
+                  (((3, 4, 64), torch.float16), ((3, 2, 64), torch.float16), ((30, 64), torch.float32)))
+    flat, ends = Laid(torch.empty(3, 256, dtype=torch.float16, device="meta")), (Laid(ids(3)), Laid(ids(2)))
+    kw = dict(out=q, stream=Stream)
+    x, u, token, prob = sample_tensors(3, 100)
+    cases = [lambda: ctx.attention(flat, kv, *ends, **kw), lambda: ctx.attention(q, kv, *ends, out=flat, stream=Stream),
+             lambda: ctx.attention(q, kv, *ends, window=1 << 31, **kw), lambda: ctx.attention(q, kv, *ends, sinks=1 << 40, **kw),
+             lambda: ctx.attention(q, kv, *ends, max_q=1 << 31, **kw),
+             lambda: ctx.qk_rope(flat, k, k, kv, *ends, rope, norm=0, **kw), lambda: ctx.qk_rope(q, flat, k, kv, *ends, rope, norm=0, **kw),
+             lambda: ctx.qk_rope(q, k, k, kv, *ends, u, norm=0, **kw),
+             lambda: ctx.sample(u, u, token=token, prob=prob, stream=Stream), lambda: ctx.sample(rope, u, token=x, prob=prob, stream=Stream),
+             lambda: ctx.sample(Laid(torch.empty(1, 3, 100, device="meta")), u, token=token, prob=prob, stream=Stream)]
+    for f in cases:
+        with pytest.raises(cb.ClutorError):
+            f()
+    assert not library.calls
+    ctx.attention(q, kv, *ends, window=(1 << 31) - 1, **kw)
+    assert library.calls[-1][1].window == (1 << 31) - 1
