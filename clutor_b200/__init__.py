@@ -156,6 +156,7 @@ def lib() -> C.CDLL:
         L.clb200_open.restype = C.c_void_p
         L.clb200_open.argtypes = [C.c_int, C.c_char_p, C.c_size_t]
         L.clb200_close.argtypes = [C.c_void_p]
+        L.clb200_device.argtypes = [C.c_void_p]
         L.clb200_moe_ffn.argtypes = [C.c_void_p, C.POINTER(MoELayer), C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]
         L.clb200_layer_bind.argtypes = [C.c_void_p, C.POINTER(MoELayer), C.c_int, C.c_char_p, C.c_size_t]
         L.clb200_moe_ffn_dev.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]
@@ -283,7 +284,7 @@ class Context:
         self.handle = lib().clb200_open(device, self._err, 512)
         if not self.handle:
             raise ClutorError(self._err.value.decode())
-        self.device = device
+        self.device = lib().clb200_device(self.handle)   # device -1: the current one
         self._keep: list = []
         self._c_qk, self._c_attention, self._c_sample = lib().clb200_qk_rope, lib().clb200_attention, lib().clb200_sample
         self._work_bytes: dict = {}

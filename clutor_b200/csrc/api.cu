@@ -366,6 +366,8 @@ clb200_ctx *clb200_open(int device, char *err, size_t errlen) {
   return c;
 }
 
+int clb200_device(const clb200_ctx *c) { return c ? c->device : -1; }
+
 void clb200_close(clb200_ctx *c) {
   if (!c) return;
   cudaSetDevice(c->device);

@@ -57,6 +57,7 @@ typedef struct clb200_ctx clb200_ctx;
  * thread at a time, like the reference's single forward thread. */
 clb200_ctx *clb200_open(int device, char *err, size_t errlen);
 void clb200_close(clb200_ctx *c);
+int clb200_device(const clb200_ctx *c);   /* the CUDA device a context is on, or -1 without one */
 
 /* The MoE block for T tokens (1 <= T <= 512, the reference's CL_PS_B) with HOST pointers: x [T x n_embd] is read and updated
  * in place (x += resid_scale * moe); sel_out / wt_out [T x n_used] (may be NULL) receive each token's chosen experts, best

@@ -46,7 +46,10 @@ class Library:
         return self.opened[-1]
 
     def clb200_open(self, device, err, n):
-        return 1
+        return device + 10 if device >= 0 else 5   # the handle: 5 for the current device
+
+    def clb200_device(self, handle):
+        return self.at if handle == 5 else handle - 10
 
     def clb200_close(self, handle):
         pass
@@ -167,3 +170,16 @@ def test_refusals_are_the_frameworks_own(library):
     assert not library.calls
     ctx.attention(q, kv, *ends, window=(1 << 31) - 1, **kw)
     assert library.calls[-1][1].window == (1 << 31) - 1
+
+
+def test_context_on_the_current_device(library):
+    """Context(-1) is on the device that was current, and takes the tensors there."""
+    library.at = 3
+    ctx = library.context(-1)
+    assert ctx.device == 3
+    x, u, token, prob = (Laid(t.like, 3) for t in sample_tensors(3, 100))
+    ctx.sample(x, u, token=token, prob=prob, stream=Stream)
+    assert len(library.calls) == 1
+    with pytest.raises(cb.ClutorError, match="cuda:3"):
+        ctx.sample(Laid(x.like, 0), u, token=token, prob=prob, stream=Stream)
+    assert library.context(2).device == 2
