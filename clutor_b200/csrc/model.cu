@@ -9,6 +9,8 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <memory>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -534,6 +536,12 @@ int clb200_model_generate_sampled(clb200_model *m, int token, int n, const float
   if (!u) { errf(err, errlen, "no random numbers"); return 1; }
   if (token < 0 || token >= a.vocab) { errf(err, errlen, "token %d is outside the vocabulary", token); return 1; }
   if (n > a.ctx - m->pos) { errf(err, errlen, "%d more tokens do not fit the context (%d of %d used)", n, m->pos, a.ctx); return 1; }
+  clb200_sampling sp{};
+  sp.vocab = a.vocab;
+  sp.type = T_F32;
+  if (clb200_sample(m->ctx, &sp, m->stream, err, errlen)) return 1;   // no rows yet: a vocabulary that it does not take is refused before a step runs
+  const std::unique_ptr<int[]> drawn(new (std::nothrow) int[static_cast<size_t>(n)]);
+  if (!drawn) { errf(err, errlen, "no host memory for %d tokens", n); return 1; }
   cudaSetDevice(m->device);
   const size_t C = static_cast<size_t>(a.ctx);
   if (!m->sp) CUDA_OR(cudaMalloc(&m->sp, (2 * C + 4) * 4), "allocating the sampling buffers");
@@ -551,10 +559,7 @@ int clb200_model_generate_sampled(clb200_model *m, int token, int n, const float
   g.feed = 0;
   g.trace = nullptr;
   g.force_miss = m->ctx->force_miss;
-  clb200_sampling sp{};
   sp.rows = 1;
-  sp.vocab = a.vocab;
-  sp.type = T_F32;
   sp.logits = a.logits;
   sp.stride = a.vocab;
   sp.temperature = m->sp + 2 * C;
@@ -570,10 +575,13 @@ int clb200_model_generate_sampled(clb200_model *m, int token, int n, const float
     CUDA_OR(pf_feed(a.st, a.gen_out + start + i, m->stream), "feeding the token");
   }
   CUDA_OR(cudaMemcpyAsync(m->st_host, a.st, sizeof(FwdState), cudaMemcpyDeviceToHost, m->stream), "state download");
-  if (tokens_out) CUDA_OR(cudaMemcpyAsync(tokens_out, a.gen_out + start, static_cast<size_t>(n) * 4, cudaMemcpyDeviceToHost, m->stream), "tokens download");
+  CUDA_OR(cudaMemcpyAsync(drawn.get(), a.gen_out + start, static_cast<size_t>(n) * 4, cudaMemcpyDeviceToHost, m->stream), "tokens download");
   if (probs_out) CUDA_OR(cudaMemcpyAsync(probs_out, m->sp + C, static_cast<size_t>(n) * 4, cudaMemcpyDeviceToHost, m->stream), "probabilities download");
   CUDA_OR(cudaStreamSynchronize(m->stream), "generating");
   if (m->st_host->err) { errf(err, errlen, "device error %d: %s", m->st_host->err, fwd_error_text(m->st_host->err)); return 1; }
+  for (int i = 0; i < n; ++i)
+    if (drawn[i] < 0) { errf(err, errlen, "step %d left no logit above -infinity: there is no token to draw", i); return 1; }
+  if (tokens_out) std::copy(drawn.get(), drawn.get() + n, tokens_out);
   m->pos = start + n;
   return 0;
 }

@@ -384,7 +384,7 @@ __global__ void pages_kernel(int *table, int n) {
   for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) table[i] = i;
 }
 
-__global__ void feed_kernel(FwdState *state, const int *token) { state->token = state->next = *token; }
+__global__ void feed_kernel(FwdState *state, const int *token) { state->token = state->next = max(*token, 0); }
 
 __global__ void resid_add_kernel(float *x, const float *v, size_t n, float scale) {
   for (size_t i = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < n; i += static_cast<size_t>(gridDim.x) * blockDim.x)

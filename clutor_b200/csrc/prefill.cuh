@@ -49,7 +49,8 @@ cudaError_t pf_attn(const PfAttnArgs &a, cudaStream_t st);
 cudaError_t pf_pages(int *table, int n, cudaStream_t st);
 // For the paged attention of a batch: pg[0, 1] = 0, rows (its first rows) and pg[2] = kv (the sequence's length with it).
 cudaError_t pf_rows(int *pg, int rows, int kv, cudaStream_t st);
-// The token that a draw chose becomes the next step's and the last step's choice.
+// The token that a draw chose becomes the next step's and the last step's choice; where there was none to choose (-1, which ends
+// the call with an error once its steps have run) the next step takes token 0.
 cudaError_t pf_feed(FwdState *state, const int *token, cudaStream_t st);
 
 // A dense product of a batch, out [nb][rows] (= or += scale *) m [rows][cols] times plain Q8_K activations: a CTA per 32

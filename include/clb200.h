@@ -474,7 +474,8 @@ int clb200_model_generate_async(clb200_model *m, int token, int n, void *stream,
 /* Sampled generation: feeds `token`, then n times the token that clb200_sample draws from the step's logits with u[i] (host, n
  * numbers in [0, 1)) and one setting of temperature, top-k, top-p and min-p (the values that leave a filter out included);
  * tokens_out and probs_out (host, n; either may be NULL) receive the tokens and their probabilities. Temperature 0 gives
- * clb200_model_generate's tokens. */
+ * clb200_model_generate's tokens. A step whose logits are all NaN or -infinity leaves nothing to draw from: the call returns 1 with
+ * that step in err, and the position stays. */
 int clb200_model_generate_sampled(clb200_model *m, int token, int n, const float *u, float temperature, int top_k, float top_p, float min_p,
                                   int *tokens_out, float *probs_out, char *err, size_t errlen);
 int clb200_model_tokens(clb200_model *m, int start, int n, int *tokens_out, char *err, size_t errlen);
