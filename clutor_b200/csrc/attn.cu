@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(RT, RowsShape<HD, MT>::PER_SM) attn_rows_kerne
     if (i < n) {
       const int j0 = span.tile(i0 + i) * RN + warp * 16;
       if (j0 <= span.hi) {
-        const AttnSlot at0 = attn_slot(g, run.s, j0);
+        const AttnSlot at0 = attn_hidden(g, span.lo, j0, 16) ? AttnSlot{-1, 0} : attn_slot(g, run.s, j0);
         const int64_t from = (at0.page < 0 ? 0 : at0.page * kv.page_stride + at0.slot * kv.slot_stride) + run.head * kv.head_stride;
         const uint32_t dst = kv_sm + (base + i) % S::STAGES * S::STAGE;
         const int left = at0.page < 0 ? 0 : run.q.kv - j0;   // positions behind the sequence's end come as zeros

@@ -101,6 +101,12 @@ CLB_DEV bool attn_sees(const AttnArgs &g, int p, int j) {
   return j <= p && (g.a.window <= 0 || j > p - g.a.window || j < g.a.sinks);
 }
 
+// Whether no row from position lo on sees any of the n positions from j on: their page is not looked up then (a cache with a window
+// may have given it back), and they come as zeros.
+CLB_DEV bool attn_hidden(const AttnArgs &g, int lo, int j, int n) {
+  return g.a.window > 0 && j + n - 1 <= lo - g.a.window && j >= g.a.sinks;
+}
+
 // The tiles of the sequences before each sequence (prefix [n_seq + 1], shared memory). Every thread of the CTA calls it; it
 // synchronises the CTA.
 template <int N>

@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(TcAttn<HD>::THREADS, 1)
       TcItem x{};
       auto where = [&](int tile) {   // this lane's box of a tile
         const int pos = tile * N + lane * box;
-        if (lane >= boxes || pos >= x.kv) return outside;
+        if (lane >= boxes || pos >= x.kv || attn_hidden(g, x.lo, pos, box)) return outside;
         const AttnSlot at = attn_slot(g, x.s, pos);
         return at.page < 0 ? outside : at;
       };

@@ -379,8 +379,9 @@ int clb200_qk_rope(clb200_ctx *c, const clb200_kv *kv, const clb200_qk *a, void 
  * softmax over the visible j of scale * q[t][h] . k_j, head h reading key/value head h / (n_head / n_kv). Visible to position
  * p: j <= p, and with window > 0 only j > p - window or j < sinks. A row that sees nothing gets zeros. q is of the cache's
  * type, out of the cache's type or CLB200_T_F32 (scores and sums are fp32; the products of probabilities and values take the
- * probabilities in the cache's type). The values of every slot below kv_len must be finite. max_q: no sequence has more new
- * rows than this (it chooses the kernel; a longer one is reported by clb200_status and its rows are left as they were).
+ * probabilities in the cache's type). The values of every slot below kv_len must be finite; pages of which no new row of the
+ * sequence sees a position are not read, and their ids may name anything. max_q: no sequence has more new rows than this (it
+ * chooses the kernel; a longer one is reported by clb200_status and its rows are left as they were).
  * n_head / n_kv at most 16. work: clb200_attention_work bytes of device memory (on a 256-byte boundary) that the call
  * uses until it is done, so calls that may run at the same time, captured graphs among them, need one each. */
 typedef struct {
