@@ -133,6 +133,23 @@ def read_traffic(kernel: str) -> float | None:
     return None
 
 
+def reference_missing() -> str | None:
+    """Why there is no reference engine to time (one line), or None: the prebuilt oracle/_ref, or one built now from its sources."""
+    import oracle
+    if not oracle.ref_available():
+        try:
+            oracle.build(need_ref=True)
+        except RuntimeError as e:
+            return str(e)
+    return None
+
+
+def cpu_baseline(make) -> dict:
+    """The reference's figure on this host's cores, or why there is none."""
+    why = reference_missing()
+    return {"unavailable": why} if why else make()
+
+
 def cpu_reference(wl: dict, seconds: float, threads: int | None = None) -> dict:
     """The reference engine's CPU path (oracle/_ref) on a bounded sample of the workload: one layer, fresh activations per
     call, all host threads (the reference caps its pool at 16)."""
@@ -140,8 +157,6 @@ def cpu_reference(wl: dict, seconds: float, threads: int | None = None) -> dict:
 
     import oracle
     from clutor_b200 import synth
-    if not oracle.ref_available():
-        oracle.build(need_ref=True)
     nthreads = threads or min(os.cpu_count() or 1, 16)
     oracle.set_ref_threads(nthreads)
     L = synth.host_layer(E=wl["E"], FF=wl["FF"], NE=wl["NE"], K=wl["K"], gate_type=synth.TYPE_NAMES[wl["gate"]],
@@ -172,8 +187,6 @@ def model_reference(image, n_ctx: int, seconds: float, threads: int | None = Non
     import numpy as np
 
     import oracle
-    if not oracle.ref_available():
-        oracle.build(need_ref=True)
     nthreads = threads or min(os.cpu_count() or 1, 16)
     oracle.set_ref_threads(nthreads)
     image.tofile(SHM_MODEL)
@@ -206,8 +219,6 @@ def prompt_reference(image, P: int, threads: int | None = None) -> dict:
     import numpy as np
 
     import oracle
-    if not oracle.ref_available():
-        oracle.build(need_ref=True)
     nthreads = threads or min(os.cpu_count() or 1, 16)
     oracle.set_ref_threads(nthreads)
     image.tofile(SHM_MODEL)
@@ -270,7 +281,7 @@ def run_prompt(a, wl: dict) -> dict:
     ctx.set_exact(False)
     cpu = None
     if not a.no_cpu_baseline:
-        cpu = prompt_reference(image, P)
+        cpu = cpu_baseline(lambda: prompt_reference(image, P))
     mb = sm.model_bytes(spec)
     line = {"metric": PROMPT_METRIC, "value": round(P / dt, 2), "unit": "tokens/s", "n_gpus": 1, "steps": a.steps,
             "warmup": a.warmup, "ms_per_step": round(1000 * dt, 3), "higher_is_better": True, "scaling": "weak",
@@ -292,6 +303,10 @@ def run_prompt(a, wl: dict) -> dict:
 
 def run_reference_arm(a, wl, rank: int) -> None:
     if rank != 0:
+        return
+    why = reference_missing()
+    if why:
+        print(json.dumps({"impl": "reference", "unavailable": why}), flush=True)
         return
     if a.workload == "prompt":
         from clutor_b200 import synth_model as sm
@@ -425,17 +440,20 @@ def run_cache(a, wl: dict) -> dict:
     st = store.stats()
     # the policy decisions, replayed on the reference's own cache.c
     log = store.read_log()
-    ref = oracle.RefCache(store.cache_slots() - 2 * K - 1, 2 * K, NL * NE, cb.WTINYLFU)
-    mism = 0
-    for op, k, r in log:
-        if op == 1:
-            code, slot = ref.access(int(k))
-            mism += (code * 65536 + slot if code >= 0 else -1) != r
-        elif op == 2:
-            mism += ref.stage(int(k)) != r
-        else:
-            ref.unpin(int(k))
-    ref.close()
+    replay = reference_missing()
+    if replay is None:
+        ref = oracle.RefCache(store.cache_slots() - 2 * K - 1, 2 * K, NL * NE, cb.WTINYLFU)
+        mism = 0
+        for op, k, r in log:
+            if op == 1:
+                code, slot = ref.access(int(k))
+                mism += (code * 65536 + slot if code >= 0 else -1) != r
+            elif op == 2:
+                mism += ref.stage(int(k)) != r
+            else:
+                ref.unpin(int(k))
+        ref.close()
+        replay = f"{len(log)} operations, {mism} mismatches"
     # the host-to-device link: one 1 GiB copy from pinned memory
     hb = torch.empty(1 << 30, dtype=torch.uint8).pin_memory()
     db = torch.empty(1 << 30, dtype=torch.uint8, device="cuda")
@@ -453,11 +471,12 @@ def run_cache(a, wl: dict) -> dict:
     cpu = None
     if not a.no_cpu_baseline:
         dec = dict(WORKLOADS["decode"])
-        cpu = cpu_reference(dec, a.cpu_seconds)
+        cpu = cpu_baseline(lambda: cpu_reference(dec, a.cpu_seconds))
         cpu.pop("ms_per_call", None)
-        cpu["value"] = round(cpu["value"] / NL, 3)
-        cpu["unit"] = "tokens/s"
-        cpu["sample"] = cpu.get("sample", "") + f"; tokens/s = layer-tokens/s / {NL} layers, every expert in RAM"
+        if "value" in cpu:
+            cpu["value"] = round(cpu["value"] / NL, 3)
+            cpu["unit"] = "tokens/s"
+            cpu["sample"] = cpu.get("sample", "") + f"; tokens/s = layer-tokens/s / {NL} layers, every expert in RAM"
     line = {"metric": "decode tokens/s through the HBM expert cache (48 Qwen3-30B-A3B MoE layers, Q4_K)",
             "value": round(value, 3), "unit": "tokens/s", "n_gpus": 1, "steps": a.steps, "warmup": a.warmup,
             "ms_per_step": round(ms / a.steps, 4), "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
@@ -471,7 +490,7 @@ def run_cache(a, wl: dict) -> dict:
                       "prefetch_wasted": st["prefetch_wasted"], "evictions": st["evictions"],
                       "prefetch_overlap": round(1.0 - st["wait_ns"] / max(st["copy_ns"], 1), 4),
                       "copy_ms": round(st["copy_ns"] / 1e6, 3), "wait_ms": round(st["wait_ns"] / 1e6, 3),
-                      "policy_replay_on_reference": f"{len(log)} operations, {mism} mismatches",
+                      "policy_replay_on_reference": replay,
                       "smart_route": None if not smart else dict(J=smart[0], M=smart[1], tau=smart[2], **store.smart_stats())},
             "roofline": {"bound": "h2d", "achieved": round(h2d, 2), "peak": round(link, 2), "unit": "GB/s",
                          "frac": round(h2d / link, 4), "traffic": None, "peak_kind": "measured here: one 1 GiB pinned copy"},
@@ -752,7 +771,7 @@ def run_model(a, wl: dict, own_group: bool = True) -> dict | None:
                "same_tokens_as_timed_run": same}
     cpu = None
     if rank == 0 and not a.no_cpu_baseline:
-        cpu = model_reference(image, W + K + 8, a.cpu_seconds)
+        cpu = cpu_baseline(lambda: model_reference(image, W + K + 8, a.cpu_seconds))
         cpu.pop("ms_per_token", None)
     if rank == 0:
         line = {"metric": MODEL_METRIC, "value": round(value, 3), "unit": "tokens/s", "n_gpus": world, "steps": K,
@@ -887,7 +906,7 @@ def run_layers(a, wl: dict, rank: int, world: int, local: int, dist) -> dict | N
                "calls_per_step": ne, "api": "clb200_moe_ffn (host pointers, synchronous)"}
     cpu = None
     if rank == 0 and not a.no_cpu_baseline:
-        cpu = cpu_reference(wl, a.cpu_seconds)
+        cpu = cpu_baseline(lambda: cpu_reference(wl, a.cpu_seconds))
         cpu.pop("ms_per_call", None)
     line = None
     if rank == 0:
