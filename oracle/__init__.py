@@ -54,12 +54,18 @@ def build(src: str | None = None, quiet: bool = True, need_ref: bool = False) ->
                            "reference engine's c/src directory")
 
 
+class ReferenceMissing(FileNotFoundError):
+    """The reference engine is neither built (oracle/_ref) nor are its sources given (CLUTOR_REF_DIR)."""
+
+
 _libs: dict[str, C.CDLL] = {}
 
 
 def _load(path: str) -> C.CDLL:
     if path not in _libs:
         if not os.path.exists(path):
+            if path == REF_SO and not ref_dir():
+                raise ReferenceMissing(f"{path} is not built, and no reference sources are given (CLUTOR_REF_DIR)")
             raise FileNotFoundError(f"{path} is not built (run `make -C oracle`)")
         _libs[path] = C.CDLL(path)
     return _libs[path]
