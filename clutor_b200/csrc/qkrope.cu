@@ -200,8 +200,11 @@ __global__ void __launch_bounds__(QT, WARPS == 1 ? 3 : 1) qk_rope_kernel(const Q
 
 template <typename S, typename C, int HD>
 void launch(const QkArgs &g, int sms, cudaStream_t st) {
-  // a warp per token once they half fill the SMs (24 warps each)
-  if (g.a.T >= 24 * sms / 2) qk_rope_kernel<S, C, HD, 1><<<(g.a.T + QW - 1) / QW, QT, 0, st>>>(g);
+  // A warp per token once CTAs of eight tokens fill the SMs. Device time, a CTA per token and a warp per token, of 32 + 4 heads of
+  // 128 in fp32: 600 tokens 8.3 and 8.8 us, 900 10.4 and 9.2, 1200 15.0 and 12.6, 1500 20.8 and 14.4; 64 + 4 in bf16: 600 9.8 and
+  // 13.3, 900 13.0 and 13.3, 1200 19.3 and 18.3; 16 + 16 with the norm over the row: 900 15.8 and 16.3, 1200 22.8 and 20.3; heads of
+  // 256 and of 64 cross earlier (16 + 2 of 256: 900 10.4 and 8.6; 24 + 8 of 64: 300 5.7 and 5.5).
+  if (g.a.T >= QW * sms) qk_rope_kernel<S, C, HD, 1><<<(g.a.T + QW - 1) / QW, QT, 0, st>>>(g);
   else qk_rope_kernel<S, C, HD, QW><<<g.a.T, QT, 0, st>>>(g);
 }
 template <typename S, typename C>

@@ -38,7 +38,7 @@ def turned(x, w, cs, norm, pairs, eps):
     return torch.cat([re, im], -1), torch.cat([mag, mag], -1)
 
 
-MANY = [700, 0, 1, 900, 37, 400]       # 2038 new tokens: more than half of the warps that 148 SMs hold
+MANY = [700, 0, 1, 900, 37, 400]       # 2038 new tokens: a warp a token
 FEW = [3, 1, 0, 5]
 CASES = [  # new tokens, heads, kv_heads, hd, page, src, cache, norm, pairs, layout
     (MANY, 64, 4, 128, 64, "bf16", "bf16", 2, False, "slots"),
