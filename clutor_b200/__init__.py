@@ -460,8 +460,8 @@ class Context:
     def attention(self, q, pages: "KvPages", q_start, kv_len, *, max_q: int | None = None, scale: float | None = None,
                   window: int = 0, sinks: int = 0, out=None, out_dtype=None, stream=None):
         """clb200_attention on torch CUDA tensors: q [T, n_head, head_dim] of the cache's type, the new rows of sequences whose
-        keys and values (the new ones included) are in `pages`; max_q bounds the new rows of a sequence (default: T); scale
-        defaults to head_dim ** -0.5. Returns [T, n_head, head_dim] (`out`, or a new tensor of out_dtype, by default q's type);
+        keys and values (the new ones included) are in `pages`; max_q bounds the new rows of a sequence (default: T, which is
+        right but takes the kernel for chunks: give 1 where every sequence has one new row); scale defaults to head_dim ** -0.5. Returns [T, n_head, head_dim] (`out`, or a new tensor of out_dtype, by default q's type);
         asynchronous. The call's workspace is allocated for the stream, so calls may overlap on the device."""
         try:
             T, H, D = q.shape
